@@ -268,6 +268,96 @@ SSA_API int ssa_neighbor_overlap(const void* nb_a, const uint8_t* valid_a, const
                                  const uint8_t* valid_b, int64_t rows, int32_t K, int32_t nb_i64,
                                  float* out, void* stream);
 
+/*
+ * Block cache: keys and values of a serving batch in 8 bits (no counterpart
+ * in the reference, which keeps none). One layer's cache is a pool of pages
+ * of block_size tokens:
+ *   k_codes, v_codes (num_pages, n_kv, block_size, d) int8
+ *   amax   (num_pages, n_kv, 2) fp32: of the page's keys / values so far. A
+ *          code c stands for c * amax / 127, c = rint(127 x / amax) (ties to
+ *          even) of the token as it came. An amax below 2^-80 counts as 0;
+ *          where it is infinite or NaN the page stands for NaN.
+ *   bounds (num_pages, n_kv, 2, d) int8: least and greatest key code of every
+ *          channel, of complete pages only
+ *   tail   (B, n_kv, 2, block_size, d) in the model's type: the tokens of each
+ *          sequence's open (incomplete) block, from which a block whose amax
+ *          grows is quantised again -- a cache filled token by token equals one
+ *          filled at once
+ * and, shared by a model's layers,
+ *   table  (B, max_blocks) int32: the page of each of a sequence's blocks
+ *   start, lens (B) int32: lengths before and after the current step's tokens.
+ * Codes are 16-byte aligned and contiguous. Blocks behind the table and page
+ * numbers outside the pool are left out: not written, not attended. A page may
+ * stand in several sequences' tables to be read, not to be appended to.
+ */
+typedef struct {
+  int32_t B, H, n_kv, n, d; /* n: step tokens of a row of the batch (the longest) */
+  int32_t dtype;            /* ssa_dtype of q, k, v, values, tail, out */
+  int32_t block_size;       /* 16, 32 or 64 */
+  int32_t max_blocks, num_pages;
+  int32_t top;              /* select, attention with a list: blocks listed */
+  int32_t sink, local;      /* select: leading / trailing blocks always listed */
+  int32_t causal;           /* attention: token i sees positions <= start + i, else all of lens */
+  float scale;
+  int64_t q_sb, q_sh, q_sn; /* (B, H, n, d) */
+  int64_t k_sb, k_sh, k_sn; /* (B, n_kv, n, d) */
+  int64_t v_sb, v_sh, v_sn; /* (B, n_kv, n, d) */
+  int64_t o_sb, o_sh, o_sn; /* out (B, H, n, d); append: k_values, v_values (B, n_kv, n, d) */
+} ssa_cache_params;
+
+/*
+ * Hands out pages for new_lens (B) more tokens of each sequence: the block
+ * table's entries for the blocks they open, from the top of the stack
+ * free_pages (its first state[0] entries), in sequence order. start_out =
+ * lens, lens_out = lens + new_lens, state_out[0] = pages left. A sequence
+ * whose blocks exceed max_blocks gets nothing and takes nothing; from the first
+ * one that the stack cannot serve on, sequences that need a page get none.
+ * Both kinds keep their length and are counted in state_out[1] (state[1] plus
+ * their number). lens_out may be lens, and state_out state.
+ */
+SSA_API int ssa_cache_reserve(int32_t B, int32_t max_blocks, int32_t block_size, int32_t num_pages,
+                              const int32_t* lens, const int32_t* new_lens, int32_t* table,
+                              const int32_t* free_pages, const int32_t* state, int32_t* start_out,
+                              int32_t* lens_out, int32_t* state_out, void* stream);
+
+/*
+ * Appends tokens start .. lens - 1 (at most n; k, v (B, n_kv, n, d) hold them
+ * from row 0): codes, amax, bounds of completed pages, and the open block's
+ * tail. k_values, v_values (both or neither): what the new tokens' codes stand
+ * for, rounded to the model's type, 0 behind a sequence's last token.
+ */
+SSA_API int ssa_cache_append(const ssa_cache_params* p, const void* k, const void* v, int8_t* k_codes,
+                             int8_t* v_codes, float* amax, int8_t* bounds, void* tail, const int32_t* table,
+                             const int32_t* start, const int32_t* lens, void* k_values, void* v_values,
+                             void* stream);
+
+/*
+ * For each step token and kv head the `top` blocks of its sequence with the
+ * highest score amax_k * max_h sum_c max(q8[h][c] lo[c], q8[h][c] hi[c]) -- an
+ * upper bound of q8 . key over the block's keys, q8 the token's q in 8 bits
+ * under one amax for the group's heads. Blocks up to the token's own stand for
+ * election; the first `sink` and last `local` >= 1 of them are always listed
+ * (sink + local <= top); ties go to the lowest block. blocks_out (B, n, n_kv,
+ * top) int32, ascending, -1 behind (tokens behind a sequence's last: all -1).
+ */
+SSA_API int ssa_cache_select(const ssa_cache_params* p, const void* q, const int8_t* bounds, const float* amax,
+                             const int32_t* table, const int32_t* start, const int32_t* lens,
+                             int32_t* blocks_out, void* stream);
+
+/*
+ * Attention of the step's tokens over the cache: every block of the sequence,
+ * or the distinct blocks that `blocks` (B, n, n_kv, top) lists for the token
+ * and kv head (entries out of range are left out). out (B, H, n, d) per o_s*
+ * strides; lse (B, H, n) fp32, optional. Rows without a key, and rows behind a
+ * sequence's last token, are 0 with lse -inf. Needs
+ * ssa_cache_attn_workspace_size(p, blocks != NULL) bytes.
+ */
+SSA_API size_t ssa_cache_attn_workspace_size(const ssa_cache_params* p, int32_t with_blocks);
+SSA_API int ssa_cache_attn(const ssa_cache_params* p, const void* q, const int8_t* k_codes, const int8_t* v_codes,
+                           const float* amax, const int32_t* table, const int32_t* start, const int32_t* lens,
+                           const int32_t* blocks, void* out, float* lse, void* workspace,
+                           size_t workspace_bytes, void* stream);
+
 /* Error code recorded by a kernel whose bounded wait on an on-chip barrier
  * ran out (0 = none); synchronises with the device. clear != 0 resets it. */
 SSA_API int32_t ssa_device_error(int32_t clear);

@@ -44,6 +44,15 @@ class AttnParams(ctypes.Structure):
                 ("dropout_seed", ctypes.c_uint64), ("dropout_offset", ctypes.c_uint64)]
 
 
+class CacheParams(ctypes.Structure):
+    """ssa_cache_params."""
+    _fields_ = [(n, _i32) for n in ("B", "H", "n_kv", "n", "d", "dtype", "block_size", "max_blocks",
+                                    "num_pages", "top", "sink", "local", "causal")] + \
+               [("scale", ctypes.c_float)] + \
+               [(n, _i64) for n in ("q_sb", "q_sh", "q_sn", "k_sb", "k_sh", "k_sn",
+                                    "v_sb", "v_sh", "v_sn", "o_sb", "o_sh", "o_sn")]
+
+
 # name -> (restype, argtypes): exactly the declarations of include/ssa_b200.h
 SIGNATURES = {
     "ssa_graph_width": (_i32, [ctypes.POINTER(GraphParams)]),
@@ -68,6 +77,11 @@ SIGNATURES = {
     "ssa_attn_bwd_noalloc": (ctypes.c_int, [ctypes.POINTER(AttnParams), _vp, _vp, _vp, _vp, _vp, _vp,
                                             _vp, _vp, _vp, _vp, _vp]),
     "ssa_neighbor_overlap": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _vp, _vp]),
+    "ssa_cache_reserve": (ctypes.c_int, [_i32] * 4 + [_vp] * 9),
+    "ssa_cache_append": (ctypes.c_int, [ctypes.POINTER(CacheParams)] + [_vp] * 13),
+    "ssa_cache_select": (ctypes.c_int, [ctypes.POINTER(CacheParams)] + [_vp] * 8),
+    "ssa_cache_attn_workspace_size": (_sz, [ctypes.POINTER(CacheParams), _i32]),
+    "ssa_cache_attn": (ctypes.c_int, [ctypes.POINTER(CacheParams)] + [_vp] * 11 + [_sz, _vp]),
     "ssa_device_error": (_i32, [_i32]),
     "ssa_debug_set_wait_limit": (ctypes.c_int, [ctypes.c_uint32]),
     "ssa_qkv_proj_hash_supported": (_i32, [ctypes.POINTER(GraphParams), _i32]),

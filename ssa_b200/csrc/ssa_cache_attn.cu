@@ -1,0 +1,624 @@
+// ssa_cache_attn.cu -- attention of a few query tokens over the 8-bit block
+// cache, over every block of a sequence or the blocks a list names.
+//
+// s = scale q . k, k = code * amax_k / 127; out = sum 2^(s' - m) v / sum
+// 2^(s' - m) with s' = s log2(e) and a running offset m, one pass over the
+// codes. A group's query rows (its heads times its tokens) are the 8-wide
+// side of the tensor products and 16 keys or channels the 16-wide one:
+//   S^T (keys x rows)     = K . Q^T    (K codes as fp16, exact)
+//   O^T (channels x rows) = V^T . P^T  (V codes as fp16, exact)
+// so eight rows fill an instruction; q and the weights P are fp16 -- q scaled
+// by a power of two for each row (a bf16 q is then exact), P below 2^15 -- or,
+// for fp32 tensors, fp16 pairs (high part and remainder, 22 bits). Sums are
+// fp32. The step of V, which differs from page to page, goes into the
+// exponent: P = 2^(s' + log2(step) - m), and the weights' sum takes P / step.
+// mma.sync rather than tcgen05: with 8 to 32 rows the operation is bound by
+// reading the codes, and a 128-row tile would be mostly padding.
+//
+// Work is counted in groups of 64 keys over all (sequence, row tile, kv head)
+// units and cut into one equal range for each thread block, so ragged batches
+// balance; a unit that spans several blocks leaves its partial sums in the
+// workspace and k_cache_combine joins them in range order.
+#include <cuda_fp16.h>
+#include <math.h>
+
+#include "ssa_cache.cuh"
+
+namespace ssa {
+
+namespace {
+
+constexpr int kWarps = 4, kThreads = 32 * kWarps;
+constexpr int kGroup = 64;       // keys a block takes at a time: 16 for each warp
+constexpr float kEmpty = -1e30f; // offset of a row that has seen no key
+constexpr float kHead = 13.f;    // weights run up to 2^13, and 2^15 before the offset moves
+constexpr float kSlack = 2.f;
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// Codes (biased by 128) in bytes SEL picks -> two fp16: 0x6400 | u is 1024 + u.
+template <int SEL>
+__device__ __forceinline__ uint32_t codes_f16(uint32_t biased) {
+  const uint32_t h = __byte_perm(biased, 0x64646464u, SEL);
+  const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&h), __half2half2(__ushort_as_half(0x6480)));
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// High part and remainder of a pair.
+__device__ __forceinline__ void split_f16(float a, float b, uint32_t& hi, uint32_t& lo) {
+  const __half2 h = __floats2half2_rn(a, b);
+  const float2 f = __half22float2(h);
+  hi = *reinterpret_cast<const uint32_t*>(&h);
+  lo = pack_f16(a - f.x, b - f.y);
+}
+
+// D / 8 codes of one key row, channels g * D / 8 and up.
+template <int D>
+__device__ __forceinline__ void load_slice(const int8_t* row, int g, uint32_t (&w)[D / 32]) {
+  const int8_t* p = row + g * (D / 8);
+  if constexpr (D == 128) {
+    const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+    w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
+  } else if constexpr (D == 64) {
+    const uint2 u = __ldg(reinterpret_cast<const uint2*>(p));
+    w[0] = u.x; w[1] = u.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) w[i] = __ldg(reinterpret_cast<const uint32_t*>(p) + i);
+  }
+}
+
+// Units and work of the call. Without a list a unit is (sequence, kv head,
+// tile of query rows) and its work the sequence's groups of 64 keys; with one
+// it is (sequence, token, kv head, tile of heads) and its work the list's.
+struct Plan {
+  int rows, tiles_max, list_groups;
+};
+
+__device__ __forceinline__ int64_t seq_work(const CacheDev& c, const Plan& pl, int b, int rows, int* tiles, int* groups) {
+  int start, len;
+  const int fresh = cache_step_tokens(c, b, start, len);
+  if (c.blocks) {
+    *tiles = c.n * pl.tiles_max;
+    *groups = pl.list_groups;
+    return (int64_t)*tiles * c.n_kv * *groups;
+  }
+  *tiles = (int)(((int64_t)fresh * c.rep + rows - 1) / rows);
+  *groups = (len + kGroup - 1) / kGroup;
+  return (int64_t)*tiles * c.n_kv * *groups;
+}
+
+__device__ __forceinline__ int64_t block_sum64(int64_t v, int64_t* red) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  int64_t s = 0;
+  for (int i = 0; i < (int)blockDim.x / 32; ++i) s += red[i];
+  return s;
+}
+
+// Blocks that get a range: with less work than blocks the first `total`, one
+// group each, so that no range between two of a unit's is empty.
+__device__ __forceinline__ int ranges_of(int64_t total, int grid) { return total < grid ? (int)total : grid; }
+
+struct Unit {
+  int b, kv, tile, start, len, fresh, row0, nrows;  // row0: its first query row, of nrows valid ones
+  const int32_t* list;
+};
+
+template <int ROWS>
+__device__ __forceinline__ Unit unit_of(const CacheDev& c, const Plan& pl, int b, int u, int tiles) {
+  Unit x;
+  x.b = b;
+  x.fresh = cache_step_tokens(c, b, x.start, x.len);
+  x.kv = u / tiles;
+  x.tile = u - x.kv * tiles;
+  x.list = nullptr;
+  if (c.blocks) {
+    const int tok = x.tile / pl.tiles_max, ht = x.tile - tok * pl.tiles_max;
+    x.row0 = tok * c.rep + ht * ROWS;
+    x.nrows = tok < x.fresh ? min(ROWS, c.rep - ht * ROWS) : 0;
+    x.list = c.blocks + (((int64_t)b * c.n + tok) * c.n_kv + x.kv) * c.top;
+  } else {
+    x.row0 = x.tile * ROWS;
+    x.nrows = min(ROWS, x.fresh * c.rep - x.row0);
+  }
+  return x;
+}
+
+// A unit's final rows (or zeros): row r of the tile is token (row0 + r) / rep
+// and the group's head (row0 + r) % rep.
+template <bool F32>
+__device__ __forceinline__ void store_out(const CacheDev& c, const Unit& x, int r, int ch, float4 o) {
+  const int row = x.row0 + r, tok = row / c.rep, h = x.kv * c.rep + row - tok * c.rep;
+  const int64_t at = x.b * c.o_sb + h * c.o_sh + tok * c.o_sn + ch;
+  if constexpr (F32) *reinterpret_cast<float4*>(static_cast<float*>(c.out) + at) = o;
+  else
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(c.out) + at) =
+        make_uint2(f32_to_bf16_bits(o.x) | (uint32_t)f32_to_bf16_bits(o.y) << 16,
+                   f32_to_bf16_bits(o.z) | (uint32_t)f32_to_bf16_bits(o.w) << 16);
+}
+__device__ __forceinline__ void store_lse(const CacheDev& c, const Unit& x, int r, float m, float l) {
+  const int row = x.row0 + r, tok = row / c.rep, h = x.kv * c.rep + row - tok * c.rep;
+  c.lse[((int64_t)x.b * c.H + h) * c.n + tok] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+}
+
+template <int D, int NT, bool F32>
+__global__ void __launch_bounds__(kThreads) k_cache_attn(const CacheDev c, const Plan pl) {
+  constexpr int ROWS = 8 * NT, W16 = D / 16, VW = D / 32, PC = F32 ? 2 : 1, OP = D + 4;
+  extern __shared__ __align__(16) unsigned char sm[];
+  uint2* qf = reinterpret_cast<uint2*>(sm);                               // [PC][NT][W16][32]
+  float* so = reinterpret_cast<float*>(qf + PC * NT * W16 * 32);          // [kWarps][ROWS][OP]
+  float* sml = so + kWarps * ROWS * OP;                                   // [kWarps][ROWS][2]
+  __shared__ int64_t red[kWarps];
+  __shared__ int64_t s_base;
+  __shared__ int s_b;
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t = lane & 3;
+  const int bs_shift = c.bs == 16 ? 4 : c.bs == 32 ? 5 : 6;
+
+  // this block's range of the work, and the sequence it starts in
+  int64_t total;
+  if (c.blocks) {
+    total = (int64_t)c.B * c.n * pl.tiles_max * c.n_kv * pl.list_groups;
+  } else {
+    int64_t sum = 0;
+    int tiles, groups;
+    for (int b = tid; b < c.B; b += kThreads) sum += seq_work(c, pl, b, ROWS, &tiles, &groups);
+    total = block_sum64(sum, red);
+  }
+  const int nblk = ranges_of(total, gridDim.x);
+  const int64_t lo = (int)blockIdx.x < nblk ? blockIdx.x * total / nblk : total;
+  const int64_t hi = (int)blockIdx.x < nblk ? (blockIdx.x + 1) * total / nblk : total;
+  if (tid == 0) { s_b = 0; s_base = 0; }
+  __syncthreads();
+  if (c.blocks) {
+    if (lo >= hi) return;
+    const int64_t per = total / c.B;
+    if (tid == 0) { s_b = (int)(lo / per); s_base = lo / per * per; }
+  } else {
+    int64_t before = 0;
+    for (int b0 = 0; b0 < c.B; b0 += kThreads) {
+      int tiles, groups;
+      const int64_t mine = b0 + tid < c.B ? seq_work(c, pl, b0 + tid, ROWS, &tiles, &groups) : 0;
+      int64_t upto = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += x;
+      }
+      __syncthreads();
+      if (lane == 31) red[w] = upto;
+      __syncthreads();
+      int64_t all = 0;
+      for (int i = 0; i < kWarps; ++i) {
+        if (i < w) upto += red[i];
+        all += red[i];
+      }
+      const int64_t from = before + upto - mine;
+      if (lo >= from && lo < from + mine) { s_b = b0 + tid; s_base = from; }
+      if (blockIdx.x == 0 && b0 + tid < c.B) c.prefix[b0 + tid] = from;
+      before += all;
+    }
+  }
+  __syncthreads();
+  if (lo >= hi) return;
+
+  int b = s_b;
+  int64_t base = s_base;
+  for (int64_t at = lo; at < hi;) {
+    int tiles, groups;
+    const int64_t mine = seq_work(c, pl, b, ROWS, &tiles, &groups);
+    if (at >= base + mine) { base += mine; ++b; continue; }
+    const int u = (int)((at - base) / groups);
+    const int64_t ubeg = base + (int64_t)u * groups, uend = ubeg + groups;
+    const int g0 = (int)(at - ubeg), g1 = (int)((hi < uend ? hi : uend) - ubeg);
+    at = ubeg + g1;
+    const Unit x = unit_of<ROWS>(c, pl, b, u, tiles);
+
+    // Q as the products' 8-wide operand: rows scaled into fp16's range by a power of two
+    float sfac[NT][2];
+    int lim[NT][2];
+    int lim_min = INT32_MAX, lim_max = 0;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int r = nt * 8 + g;
+      const bool have = r < x.nrows;
+      const int row = x.row0 + (have ? r : 0), tok = row / c.rep, h = x.kv * c.rep + row - tok * c.rep;
+      const void* qr = row_ptr<F32 ? kDtF32 : kDtBF16>(c.q, x.b * c.q_sb + h * c.q_sh + tok * c.q_sn);
+      float4 v[W16];
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < W16; ++i) {
+        v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (have) v[i] = load4<F32 ? kDtF32 : kDtBF16>(qr, cache_word_channel<D>(i, t));
+        top = max(top, max(max(__float_as_uint(v[i].x) & 0x7fffffffu, __float_as_uint(v[i].y) & 0x7fffffffu),
+                           max(__float_as_uint(v[i].z) & 0x7fffffffu, __float_as_uint(v[i].w) & 0x7fffffffu)));
+      }
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // 2^e brings the row's largest element into [2^9, 2^10); e in [-118, 100]
+      int e = 9 - ((int)(top >> 23) - 127);
+      e = top >= 0x7f800000u ? 0 : min(e, 100);
+      const float up = __uint_as_float((uint32_t)(e + 127) << 23), down = __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+      for (int i = 0; i < W16; ++i) {
+        if (i % kWarps != w) continue;
+        uint2 hi2, lo2;
+        split_f16(v[i].x * up, v[i].y * up, hi2.x, lo2.x);
+        split_f16(v[i].z * up, v[i].w * up, hi2.y, lo2.y);
+        qf[(nt * W16 + i) * 32 + lane] = hi2;
+        if constexpr (F32) qf[((NT + nt) * W16 + i) * 32 + lane] = lo2;
+      }
+      const float mine_s = c.scale * 1.4426950408889634f * down;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        sfac[nt][k] = __shfl_sync(0xffffffffu, mine_s, (2 * t + k) * 4);
+        const int rr = nt * 8 + 2 * t + k;
+        lim[nt][k] = INT32_MAX;  // rows behind the last one: computed, never stored
+        if (rr < x.nrows) {
+          lim[nt][k] = c.causal ? x.start + (x.row0 + rr) / c.rep + 1 : x.len;
+          lim_min = min(lim_min, lim[nt][k]);
+          lim_max = max(lim_max, lim[nt][k]);
+        }
+      }
+    }
+    lim_min = __reduce_min_sync(0xffffffffu, lim_min);
+    lim_max = __reduce_max_sync(0xffffffffu, lim_max);
+    __syncthreads();
+
+    float acc[W16][NT][4], mref[NT][2], lsum[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      mref[nt][0] = mref[nt][1] = kEmpty;
+      lsum[nt][0] = lsum[nt][1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < W16; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[i][nt][k] = 0.f;
+    }
+
+    for (int s0 = g0; s0 < g1; s0 += 32) {
+      // lane l looks up this warp's 16 keys of group s0 + l
+      int page = -1, kb = 0, off = 0;
+      float2 am = make_float2(0.f, 0.f);
+      if (s0 + lane < g1) {
+        const int64_t key = (int64_t)(s0 + lane) * kGroup + w * 16;
+        const int entry = (int)(key >> bs_shift);
+        off = (int)key & (c.bs - 1);
+        const int blk = !x.list ? entry : entry < c.top ? __ldg(x.list + entry) : -1;
+        if (blk >= 0 && blk < c.max_blocks) {
+          kb = blk * c.bs + off;
+          if (kb < lim_max) page = cache_page(c, x.b, blk);
+        }
+        if (page >= 0) am = __ldg(reinterpret_cast<const float2*>(c.amax) + (int64_t)page * c.n_kv + x.kv);
+      }
+      uint32_t todo = __ballot_sync(0xffffffffu, page >= 0);
+      if (!todo) continue;
+      uint32_t kw0[W16], kw1[W16], vw[4][VW];
+      const auto row_of = [&](const int8_t* codes, int j) {
+        return codes + (((int64_t)__shfl_sync(0xffffffffu, page, j) * c.n_kv + x.kv) * c.bs + __shfl_sync(0xffffffffu, off, j)) * D;
+      };
+      const auto load_k = [&](int j) {
+        const int8_t* p = row_of(c.k_codes, j);
+        cache_load_row<D>(p + g * D, t, kw0);
+        cache_load_row<D>(p + (g + 8) * D, t, kw1);
+      };
+      const auto load_v = [&](int j) {
+        const int8_t* p = row_of(c.v_codes, j);
+        load_slice<D>(p + (2 * t) * D, g, vw[0]);
+        load_slice<D>(p + (2 * t + 1) * D, g, vw[1]);
+        load_slice<D>(p + (2 * t + 8) * D, g, vw[2]);
+        load_slice<D>(p + (2 * t + 9) * D, g, vw[3]);
+      };
+      int j = __ffs(todo) - 1;
+      load_k(j);
+      load_v(j);
+      while (true) {
+        todo &= todo - 1;
+        const int jn = todo ? __ffs(todo) - 1 : -1;
+        const float ka = __shfl_sync(0xffffffffu, am.x, j) * (1.f / 127.f);
+        const float va = __shfl_sync(0xffffffffu, am.y, j) * (1.f / 127.f);
+        const int kbj = __shfl_sync(0xffffffffu, kb, j);
+
+        float s[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) s[nt][k] = 0.f;
+#pragma unroll
+        for (int i = 0; i < W16; ++i) {
+          const uint32_t x0 = kw0[i] ^ 0x80808080u, x1 = kw1[i] ^ 0x80808080u;
+          const uint32_t a[4] = {codes_f16<0x4140>(x0), codes_f16<0x4140>(x1), codes_f16<0x4342>(x0), codes_f16<0x4342>(x1)};
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int pc = 0; pc < PC; ++pc) {
+              const uint2 bq = qf[((pc * NT + nt) * W16 + i) * 32 + lane];
+              mma_f16(s[nt], a, bq.x, bq.y);
+            }
+        }
+        if (jn >= 0) load_k(jn);
+
+        // weights 2^(s' + log2(step_v) - m + 13)
+        const float vs = va > 0.f ? va : 1.f;  // a page of zeros: any step does
+        const float lv = F32 ? log2f(vs) : __log2f(vs), iv = 1.f / vs;
+        const bool edge = kbj + 16 > lim_min;
+        bool move = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            float v = fmaf(s[nt][k], ka * sfac[nt][k & 1], lv);
+            if (edge && kbj + g + 8 * (k >> 1) >= lim[nt][k & 1]) v = -INFINITY;
+            s[nt][k] = v;
+            move |= v > mref[nt][k & 1] + (kHead + kSlack);
+          }
+        if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              float m = fmaxf(s[nt][k], s[nt][k + 2]);
+              m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+              m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+              m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+              m = fmaxf(mref[nt][k], m - kHead);
+              const float f = ex2(mref[nt][k] - m);
+              mref[nt][k] = m;
+              lsum[nt][k] *= f;
+#pragma unroll
+              for (int i = 0; i < W16; ++i) {
+                acc[i][nt][k] *= f;
+                acc[i][nt][k + 2] *= f;
+              }
+            }
+        }
+        uint32_t pf[PC][NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float p[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) p[k] = ex2(s[nt][k] - mref[nt][k & 1]);
+          lsum[nt][0] = fmaf(p[0] + p[2], iv, lsum[nt][0]);
+          lsum[nt][1] = fmaf(p[1] + p[3], iv, lsum[nt][1]);
+          if constexpr (F32) {
+            uint32_t h0, l0, h1, l1;
+            split_f16(p[0], p[1], h0, l0);
+            split_f16(p[2], p[3], h1, l1);
+            pf[0][nt][0] = transpose8x8(h0);
+            pf[0][nt][1] = transpose8x8(h1);
+            pf[PC - 1][nt][0] = transpose8x8(l0);
+            pf[PC - 1][nt][1] = transpose8x8(l1);
+          } else {
+            pf[0][nt][0] = transpose8x8(pack_f16(p[0], p[1]));
+            pf[0][nt][1] = transpose8x8(pack_f16(p[2], p[3]));
+          }
+        }
+
+        // lane group g holds channels g D/8 + ..; byte 2 i is row g of channel tile i, byte 2 i + 1 row g + 8
+#pragma unroll
+        for (int q = 0; q < VW; ++q) {
+          const uint32_t x0 = __byte_perm(vw[0][q], vw[1][q], 0x5140) ^ 0x80808080u;
+          const uint32_t x1 = __byte_perm(vw[2][q], vw[3][q], 0x5140) ^ 0x80808080u;
+          const uint32_t y0 = __byte_perm(vw[0][q], vw[1][q], 0x7362) ^ 0x80808080u;
+          const uint32_t y1 = __byte_perm(vw[2][q], vw[3][q], 0x7362) ^ 0x80808080u;
+          const uint32_t a[4] = {codes_f16<0x4140>(x0), codes_f16<0x4342>(x0), codes_f16<0x4140>(x1), codes_f16<0x4342>(x1)};
+          const uint32_t e[4] = {codes_f16<0x4140>(y0), codes_f16<0x4342>(y0), codes_f16<0x4140>(y1), codes_f16<0x4342>(y1)};
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int pc = 0; pc < PC; ++pc) {
+              mma_f16(acc[2 * q][nt], a, pf[pc][nt][0], pf[pc][nt][1]);
+              mma_f16(acc[2 * q + 1][nt], e, pf[pc][nt][0], pf[pc][nt][1]);
+            }
+        }
+        if (jn < 0) break;
+        load_v(jn);
+        j = jn;
+      }
+    }
+
+    // Join the four warps.
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        float l = lsum[nt][k];
+        l += __shfl_xor_sync(0xffffffffu, l, 4);
+        l += __shfl_xor_sync(0xffffffffu, l, 8);
+        l += __shfl_xor_sync(0xffffffffu, l, 16);
+        const int r = nt * 8 + 2 * t + k;
+        if (g == 0) {
+          sml[(w * ROWS + r) * 2] = mref[nt][k];
+          sml[(w * ROWS + r) * 2 + 1] = l;
+        }
+        float* row = so + (w * ROWS + r) * OP + g * (D / 8);
+#pragma unroll
+        for (int i = 0; i < W16; i += 2)
+          *reinterpret_cast<float4*>(row + 2 * i) =
+              make_float4(acc[i][nt][k], acc[i][nt][k + 2], acc[i + 1][nt][k], acc[i + 1][nt][k + 2]);
+      }
+    __syncthreads();
+    const bool full = g0 == 0 && g1 == groups;
+    const int64_t slot = (int64_t)blockIdx.x * 2 + (g0 == 0);
+    for (int i = tid; i < ROWS * (D / 4); i += kThreads) {
+      const int r = i / (D / 4), ch = i % (D / 4) * 4;
+      if (r >= x.nrows) break;
+      float m = kEmpty;
+#pragma unroll
+      for (int k = 0; k < kWarps; ++k) m = fmaxf(m, sml[(k * ROWS + r) * 2]);
+      float l = 0.f;
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int k = 0; k < kWarps; ++k) {
+        const float f = ex2(sml[(k * ROWS + r) * 2] - m);
+        l = fmaf(f, sml[(k * ROWS + r) * 2 + 1], l);
+        const float4 v = *reinterpret_cast<const float4*>(so + (k * ROWS + r) * OP + ch);
+        o.x = fmaf(f, v.x, o.x); o.y = fmaf(f, v.y, o.y); o.z = fmaf(f, v.z, o.z); o.w = fmaf(f, v.w, o.w);
+      }
+      if (full) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        store_out<F32>(c, x, r, ch, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+        if (ch == 0 && c.lse) store_lse(c, x, r, m, l);
+      } else {
+        *reinterpret_cast<float4*>(c.part_o + (slot * ROWS + r) * D + ch) = o;
+        if (ch == 0) *reinterpret_cast<float2*>(c.part_ml + (slot * ROWS + r) * 2) = make_float2(m, l);
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// One thread block for each unit: joins the partial sums of a unit that
+// several blocks worked on, and writes zeros to rows that have no work.
+template <int D, int NT, bool F32>
+__global__ void __launch_bounds__(kThreads) k_cache_combine(const CacheDev c, const Plan pl, const int ngrid) {
+  constexpr int ROWS = 8 * NT;
+  __shared__ int64_t red[kWarps];
+  const int tid = threadIdx.x;
+  const int per = pl.tiles_max * (c.blocks ? c.n : 1);  // row tiles a (sequence, kv head) can have
+  const int b = (int)(blockIdx.x / ((unsigned)per * c.n_kv)), u = (int)(blockIdx.x % ((unsigned)per * c.n_kv));
+  const int kv = u / per, tile = u % per;
+  int tiles, groups;
+  const int64_t mine = seq_work(c, pl, b, ROWS, &tiles, &groups);
+  Unit x = unit_of<ROWS>(c, pl, b, kv * per + tile, per);
+  const int rows_all = c.blocks ? min(ROWS, c.rep - tile % pl.tiles_max * ROWS) : min(ROWS, c.n * c.rep - x.row0);
+  const bool work = tile < tiles && mine > 0;
+  if (!work || x.nrows < rows_all) {
+    for (int i = tid; i < rows_all * (D / 4); i += kThreads) {
+      const int r = i / (D / 4), ch = i % (D / 4) * 4;
+      if (work && r < x.nrows) continue;
+      store_out<F32>(c, x, r, ch, make_float4(0.f, 0.f, 0.f, 0.f));
+      if (ch == 0 && c.lse) store_lse(c, x, r, 0.f, 0.f);
+    }
+    if (!work) return;
+  }
+  int64_t total, base;
+  if (c.blocks) {
+    total = mine * c.B;
+    base = mine * b;
+  } else {
+    int64_t sum = 0;
+    int a, e;
+    for (int i = tid; i < c.B; i += kThreads) sum += seq_work(c, pl, i, ROWS, &a, &e);
+    total = block_sum64(sum, red);
+    base = c.prefix[b];
+  }
+  const int64_t ubeg = base + ((int64_t)kv * tiles + tile) * groups, uend = ubeg + groups;
+  // block i holds [i total / nblk, (i + 1) total / nblk)
+  const int nblk = ranges_of(total, ngrid);
+  const int c0 = (int)(((ubeg + 1) * nblk - 1) / total), c1 = (int)((uend * nblk - 1) / total);
+  if (c0 == c1) return;
+  for (int i = tid; i < ROWS * (D / 4); i += kThreads) {
+    const int r = i / (D / 4), ch = i % (D / 4) * 4;
+    if (r >= x.nrows) break;
+    float m = kEmpty;
+    for (int k = c0; k <= c1; ++k) m = fmaxf(m, c.part_ml[(((int64_t)k * 2 + (k == c0)) * ROWS + r) * 2]);
+    float l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = c0; k <= c1; ++k) {
+      const int64_t slot = ((int64_t)k * 2 + (k == c0)) * ROWS + r;
+      const float2 ml = *reinterpret_cast<const float2*>(c.part_ml + slot * 2);
+      const float f = ex2(ml.x - m);
+      l = fmaf(f, ml.y, l);
+      const float4 v = *reinterpret_cast<const float4*>(c.part_o + slot * D + ch);
+      o.x = fmaf(f, v.x, o.x); o.y = fmaf(f, v.y, o.y); o.z = fmaf(f, v.z, o.z); o.w = fmaf(f, v.w, o.w);
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    store_out<F32>(c, x, r, ch, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+    if (ch == 0 && c.lse) store_lse(c, x, r, m, l);
+  }
+}
+
+// Rows of a tile: 8, 16 or 32 (the rows a group has, as far as they go).
+int tile_rows(const CacheDev& c) {
+  const int64_t rows = c.blocks ? c.rep : (int64_t)c.n * c.rep;
+  return rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
+}
+
+Plan plan_of(const CacheDev& c) {
+  Plan p;
+  p.rows = tile_rows(c);
+  p.tiles_max = (int)(((c.blocks ? c.rep : (int64_t)c.n * c.rep) + p.rows - 1) / p.rows);
+  p.list_groups = c.blocks ? (int)(((int64_t)c.top * c.bs + kGroup - 1) / kGroup) : 0;
+  return p;
+}
+
+int64_t units_of(const CacheDev& c, const Plan& p) {
+  return (int64_t)c.B * c.n_kv * p.tiles_max * (c.blocks ? c.n : 1);
+}
+
+template <int D, int NT, bool F32>
+cudaError_t run_attn(const CacheDev& c, const Plan& pl, cudaStream_t st) {
+  constexpr int ROWS = 8 * NT;
+  const size_t smem = (size_t)(F32 ? 2 : 1) * NT * (D / 16) * 32 * 8 + (size_t)kWarps * ROWS * (D + 4 + 2) * 4;
+  cudaError_t e = cudaFuncSetAttribute(k_cache_attn<D, NT, F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return e;
+  const int64_t units = units_of(c, pl);
+  if (units > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  k_cache_attn<D, NT, F32><<<c.grid, kThreads, smem, st>>>(c, pl);
+  note_launch();
+  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  k_cache_combine<D, NT, F32><<<(unsigned)units, kThreads, 0, st>>>(c, pl, c.grid);
+  note_launch();
+  return cudaGetLastError();
+}
+
+template <int D, bool F32>
+cudaError_t run_attn_rows(const CacheDev& c, cudaStream_t st) {
+  const Plan pl = plan_of(c);
+  return pl.rows == 8 ? run_attn<D, 1, F32>(c, pl, st) : pl.rows == 16 ? run_attn<D, 2, F32>(c, pl, st)
+                                                                       : run_attn<D, 4, F32>(c, pl, st);
+}
+
+template <bool F32>
+cudaError_t run_attn_d(const CacheDev& c, cudaStream_t st) {
+  return c.d == 32 ? run_attn_rows<32, F32>(c, st) : c.d == 64 ? run_attn_rows<64, F32>(c, st)
+         : c.d == 96 ? run_attn_rows<96, F32>(c, st) : run_attn_rows<128, F32>(c, st);
+}
+
+}  // namespace
+
+size_t cache_attn_workspace_layout(CacheDev* c, void* ws) {
+  const Plan p = plan_of(*c);
+  const int64_t groups = p.list_groups ? p.list_groups : ((int64_t)c->max_blocks * c->bs + kGroup - 1) / kGroup;
+  const int64_t most = units_of(*c, p) * groups;  // no use for more blocks than groups
+  const int64_t full = 148 * (p.rows == 8 ? 4 : p.rows == 16 ? 3 : 2);
+  c->grid = (int)(most < full ? most : full);
+  const size_t o_pre = ((size_t)(c->B + 1) * 8 + 255) / 256 * 256;
+  const size_t o_ml = o_pre + ((size_t)c->grid * 2 * p.rows * 2 * 4 + 255) / 256 * 256;
+  char* base = static_cast<char*>(ws);
+  c->prefix = reinterpret_cast<int64_t*>(base);
+  c->part_ml = reinterpret_cast<float*>(base + o_pre);
+  c->part_o = reinterpret_cast<float*>(base + o_ml);
+  return o_ml + (size_t)c->grid * 2 * p.rows * c->d * 4;
+}
+
+cudaError_t launch_cache_attn(const CacheDev& c, cudaStream_t st) {
+  return c.dtype == kDtF32 ? run_attn_d<true>(c, st) : run_attn_d<false>(c, st);
+}
+
+}  // namespace ssa

@@ -475,6 +475,136 @@ int ssa_attn_bwd_csr(const ssa_attn_params* p, const void* q, const void* k, con
 }
 
 // neighbor_overlap: per-row Jaccard similarity of two neighbor sets.
+static int check_cache(const ssa_cache_params* p, const void* table, const void* start, const void* lens) {
+  if (!p) return fail(SSA_ERR_INVALID, "params is NULL");
+  if (p->B < 1 || p->n_kv < 1 || p->n < 1 || p->max_blocks < 1 || p->num_pages < 1)
+    return fail(SSA_ERR_INVALID, "B,n_kv,n,max_blocks,num_pages must be >= 1");
+  if (p->dtype != SSA_F32 && p->dtype != SSA_BF16) return fail(SSA_ERR_INVALID, "dtype must be F32 or BF16");
+  if (p->d != 32 && p->d != 64 && p->d != 96 && p->d != 128)
+    return fail(SSA_ERR_UNSUPPORTED, "the block cache supports head dims 32, 64, 96 and 128 (got %d)", p->d);
+  if (p->block_size != 16 && p->block_size != 32 && p->block_size != 64)
+    return fail(SSA_ERR_UNSUPPORTED, "block_size must be 16, 32 or 64 (got %d)", p->block_size);
+  if ((int64_t)p->max_blocks * p->block_size > (int64_t(1) << 30))
+    return fail(SSA_ERR_UNSUPPORTED, "max_blocks * block_size exceeds 2^30");
+  if (!table || !start || !lens) return fail(SSA_ERR_INVALID, "table/start/lens are NULL");
+  return SSA_OK;
+}
+
+static int check_heads(const ssa_cache_params* p) {
+  if (p->H < 1) return fail(SSA_ERR_INVALID, "H must be >= 1");
+  if (p->H % p->n_kv)
+    return fail(SSA_ERR_INVALID, "num_heads (%d) must be divisible by num_kv_heads (%d)", p->H, p->n_kv);
+  if ((int64_t)p->n * (p->H / p->n_kv) > (int64_t(1) << 30)) return fail(SSA_ERR_UNSUPPORTED, "too many query rows");
+  return SSA_OK;
+}
+
+static ssa::CacheDev cache_dev(const ssa_cache_params* p) {
+  ssa::CacheDev c;
+  memset(&c, 0, sizeof(c));
+  c.B = p->B; c.H = p->H; c.n_kv = p->n_kv; c.rep = p->H / p->n_kv; c.n = p->n; c.d = p->d; c.dtype = p->dtype;
+  c.bs = p->block_size; c.max_blocks = p->max_blocks; c.num_pages = p->num_pages;
+  c.top = p->top; c.sink = p->sink; c.local = p->local; c.causal = p->causal; c.scale = p->scale;
+  c.q_sb = p->q_sb; c.q_sh = p->q_sh; c.q_sn = p->q_sn;
+  c.k_sb = p->k_sb; c.k_sh = p->k_sh; c.k_sn = p->k_sn;
+  c.v_sb = p->v_sb; c.v_sh = p->v_sh; c.v_sn = p->v_sn;
+  c.o_sb = p->o_sb; c.o_sh = p->o_sh; c.o_sn = p->o_sn;
+  return c;
+}
+
+int ssa_cache_reserve(int32_t B, int32_t max_blocks, int32_t block_size, int32_t num_pages, const int32_t* lens,
+                      const int32_t* new_lens, int32_t* table, const int32_t* free_pages, const int32_t* state,
+                      int32_t* start_out, int32_t* lens_out, int32_t* state_out, void* stream) {
+  if (B < 1 || max_blocks < 1 || block_size < 1 || num_pages < 1)
+    return fail(SSA_ERR_INVALID, "B,max_blocks,block_size,num_pages must be >= 1");
+  if ((int64_t)max_blocks * block_size > (int64_t(1) << 30))
+    return fail(SSA_ERR_UNSUPPORTED, "max_blocks * block_size exceeds 2^30");
+  if (!lens || !new_lens || !table || !free_pages || !state || !start_out || !lens_out || !state_out)
+    return fail(SSA_ERR_INVALID, "NULL lens/new_lens/table/free_pages/state or outputs");
+  if (start_out == lens || start_out == lens_out) return fail(SSA_ERR_INVALID, "start_out must be a buffer of its own");
+  ssa::ReserveDev r;
+  r.B = B; r.max_blocks = max_blocks; r.bs = block_size; r.num_pages = num_pages;
+  r.lens = lens; r.new_lens = new_lens; r.table = table; r.free_pages = free_pages; r.state = state;
+  r.start_out = start_out; r.lens_out = lens_out; r.state_out = state_out;
+  cudaError_t e = ssa::launch_cache_reserve(r, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "cache reserve launch");
+  return SSA_OK;
+}
+
+int ssa_cache_append(const ssa_cache_params* p, const void* k, const void* v, int8_t* k_codes, int8_t* v_codes,
+                     float* amax, int8_t* bounds, void* tail, const int32_t* table, const int32_t* start,
+                     const int32_t* lens, void* k_values, void* v_values, void* stream) {
+  int rc;
+  if ((rc = check_cache(p, table, start, lens))) return rc;
+  if ((rc = check_rows("k", k, p->dtype, p->d, p->k_sb, p->k_sh, p->k_sn))) return rc;
+  if ((rc = check_rows("v", v, p->dtype, p->d, p->v_sb, p->v_sh, p->v_sn))) return rc;
+  if (!k_codes || !v_codes || !amax || !bounds || !tail || !aligned(k_codes, 16) || !aligned(v_codes, 16) ||
+      !aligned(amax, 8) || !aligned(bounds, 16) || !aligned(tail, 16))
+    return fail(SSA_ERR_INVALID, "cache buffers must be non-null and 16-byte aligned");
+  if (!k_values != !v_values) return fail(SSA_ERR_INVALID, "k_values and v_values come together");
+  if (k_values && ((rc = check_rows("k_values", k_values, p->dtype, p->d, p->o_sb, p->o_sh, p->o_sn)) ||
+                   (rc = check_rows("v_values", v_values, p->dtype, p->d, p->o_sb, p->o_sh, p->o_sn))))
+    return rc;
+  ssa::CacheDev c = cache_dev(p);
+  c.k = k; c.v = v; c.k_codes = k_codes; c.v_codes = v_codes; c.amax = amax; c.bounds = bounds; c.tail = tail;
+  c.table = table; c.start = start; c.lens = lens; c.k_values = k_values; c.v_values = v_values;
+  cudaError_t e = ssa::launch_cache_append(c, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "cache append launch");
+  return SSA_OK;
+}
+
+int ssa_cache_select(const ssa_cache_params* p, const void* q, const int8_t* bounds, const float* amax,
+                     const int32_t* table, const int32_t* start, const int32_t* lens, int32_t* blocks_out,
+                     void* stream) {
+  int rc;
+  if ((rc = check_cache(p, table, start, lens)) || (rc = check_heads(p))) return rc;
+  if ((rc = check_rows("q", q, p->dtype, p->d, p->q_sb, p->q_sh, p->q_sn))) return rc;
+  if (!bounds || !amax || !blocks_out || !aligned(bounds, 16) || !aligned(amax, 8))
+    return fail(SSA_ERR_INVALID, "bounds/amax/blocks_out must be non-null and aligned");
+  if (p->sink < 0 || p->local < 1 || p->top < 1 || p->sink > p->top - p->local)
+    return fail(SSA_ERR_INVALID, "top=%d must be at least sink (%d >= 0) + local (%d >= 1)", p->top, p->sink, p->local);
+  ssa::CacheDev c = cache_dev(p);
+  if (ssa::cache_select_smem(c) > 220 * 1024)
+    return fail(SSA_ERR_UNSUPPORTED, "too many blocks in a table (%d) for the selection's on-chip scores", p->max_blocks);
+  c.q = q; c.bounds = const_cast<int8_t*>(bounds); c.amax = const_cast<float*>(amax);
+  c.table = table; c.start = start; c.lens = lens; c.blocks_out = blocks_out;
+  cudaError_t e = ssa::launch_cache_select(c, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "cache select launch");
+  return SSA_OK;
+}
+
+size_t ssa_cache_attn_workspace_size(const ssa_cache_params* p, int32_t with_blocks) {
+  if (!p || p->B < 1 || p->n_kv < 1 || p->n < 1 || p->H < p->n_kv || p->d < 1 || p->block_size < 1 || p->max_blocks < 1) return 0;
+  ssa::CacheDev c = cache_dev(p);
+  static const int32_t any = 0;
+  c.blocks = with_blocks ? &any : nullptr;
+  return ssa::cache_attn_workspace_layout(&c, nullptr);
+}
+
+int ssa_cache_attn(const ssa_cache_params* p, const void* q, const int8_t* k_codes, const int8_t* v_codes,
+                   const float* amax, const int32_t* table, const int32_t* start, const int32_t* lens,
+                   const int32_t* blocks, void* out, float* lse, void* workspace, size_t workspace_bytes,
+                   void* stream) {
+  int rc;
+  if ((rc = check_cache(p, table, start, lens)) || (rc = check_heads(p))) return rc;
+  if ((rc = check_rows("q", q, p->dtype, p->d, p->q_sb, p->q_sh, p->q_sn))) return rc;
+  if ((rc = check_rows("out", out, p->dtype, p->d, p->o_sb, p->o_sh, p->o_sn))) return rc;
+  if (!k_codes || !v_codes || !amax || !aligned(k_codes, 16) || !aligned(v_codes, 16) || !aligned(amax, 8))
+    return fail(SSA_ERR_INVALID, "k_codes/v_codes/amax must be non-null and aligned");
+  if (blocks && (p->top < 1 || (int64_t)p->top * p->block_size > (int64_t(1) << 30)))
+    return fail(SSA_ERR_INVALID, "top=%d out of range", p->top);
+  ssa::CacheDev c = cache_dev(p);
+  c.blocks = blocks;
+  const size_t need = ssa::cache_attn_workspace_layout(&c, nullptr);
+  if (!workspace || workspace_bytes < need || !aligned(workspace, 16))
+    return fail(SSA_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", need, workspace_bytes);
+  ssa::cache_attn_workspace_layout(&c, workspace);
+  c.q = q; c.k_codes = const_cast<int8_t*>(k_codes); c.v_codes = const_cast<int8_t*>(v_codes);
+  c.amax = const_cast<float*>(amax); c.table = table; c.start = start; c.lens = lens; c.out = out; c.lse = lse;
+  cudaError_t e = ssa::launch_cache_attn(c, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "cache attention launch");
+  return SSA_OK;
+}
+
 int ssa_neighbor_overlap(const void* nb_a, const uint8_t* valid_a, const void* nb_b, const uint8_t* valid_b,
                          int64_t rows, int32_t K, int32_t nb_i64, float* out, void* stream) {
   if (rows < 0 || K < 1) return fail(SSA_ERR_INVALID, "rows=%lld, K=%d", (long long)rows, K);

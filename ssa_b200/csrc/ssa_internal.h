@@ -194,4 +194,52 @@ cudaError_t launch_build_csr(const AttnDev& a, cudaStream_t st);
 // build_csr: sort the edges first (else a.skey / sid / seg hold a built index).
 cudaError_t launch_attn_bwd(const AttnDev& a, bool build_csr, cudaStream_t st);
 
+// One layer of the 8-bit block cache (include/ssa_b200.h, "Block cache").
+struct CacheDev {
+  int B, H, n_kv, rep, n, d, dtype, bs, max_blocks, num_pages;
+  int top, sink, local, causal;
+  float scale;
+  int64_t q_sb, q_sh, q_sn, k_sb, k_sh, k_sn, v_sb, v_sh, v_sn, o_sb, o_sh, o_sn;
+  const void* q;
+  const void* k;
+  const void* v;
+  int8_t* k_codes;        // [num_pages][n_kv][bs][d]
+  int8_t* v_codes;
+  float* amax;            // [num_pages][n_kv][2]
+  int8_t* bounds;         // [num_pages][n_kv][2][d]
+  void* tail;             // [B][n_kv][2][bs][d], the model's type
+  const int32_t* table;   // [B][max_blocks]
+  const int32_t* start;   // [B] lengths before the step
+  const int32_t* lens;    // [B] and after it
+  void* k_values;         // append: what the new tokens' codes stand for, or null
+  void* v_values;
+  int32_t* blocks_out;    // select: [B][n][n_kv][top]
+  const int32_t* blocks;  // attention: the same list, or null for every block
+  void* out;
+  float* lse;
+  // attention workspace
+  int64_t* prefix;        // [B + 1] work before each sequence
+  float* part_o;          // [2 * grid][rows][d] unnormalised outputs
+  float* part_ml;         // [2 * grid][rows][2] their exponent offset and weight sum
+  int grid;
+};
+struct ReserveDev {
+  int B, max_blocks, bs, num_pages;
+  const int32_t* lens;
+  const int32_t* new_lens;
+  int32_t* table;
+  const int32_t* free_pages;
+  const int32_t* state;
+  int32_t* start_out;
+  int32_t* lens_out;
+  int32_t* state_out;
+};
+cudaError_t launch_cache_reserve(const ReserveDev& r, cudaStream_t st);
+cudaError_t launch_cache_append(const CacheDev& c, cudaStream_t st);
+size_t cache_select_smem(const CacheDev& c);
+cudaError_t launch_cache_select(const CacheDev& c, cudaStream_t st);
+// Fills the workspace pointers of c (ws may be null) and c->grid; bytes needed.
+size_t cache_attn_workspace_layout(CacheDev* c, void* ws);
+cudaError_t launch_cache_attn(const CacheDev& c, cudaStream_t st);
+
 }  // namespace ssa

@@ -15,7 +15,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from ._lib import AttnParams, GraphParams, SSA_BF16, SSA_F32, check
+from ._lib import AttnParams, CacheParams, GraphParams, SSA_BF16, SSA_F32, check
 
 
 def _require_cuda(*ts: torch.Tensor):
@@ -415,6 +415,162 @@ def gather_attention(q, k, v, nb, valid, scale: float, fp32w: bool = False, drop
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return GatherAttention.apply(q, k, v, nb, valid, scale, fp32w, dropout, csr)
     return attn_fwd(q, k, v, nb, valid, scale, fp32w, want_lse=False, dropout=dropout)[0]
+
+
+# ---------------------------------------------------------------------------
+# 8-bit block cache (include/ssa_b200.h, "Block cache"; ssa_b200/cache.py
+# holds the buffers)
+# ---------------------------------------------------------------------------
+def _cache_tensor(name, t, dtype, shape, dev):
+    """Cache buffers are read and written where they lie: their type, shape,
+    device and contiguity are checked, never mended by a copy."""
+    if t.dtype != dtype or tuple(t.shape) != shape or t.device != dev or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape} on {dev}, got "
+                         f"{t.dtype} {tuple(t.shape)}{'' if t.is_contiguous() else ' (strided)'} on {t.device}")
+    return t.data_ptr()
+
+
+def _cache_call(dev, name, *args):
+    """One launch on dev's current stream, whichever device is current."""
+    fn = getattr(_lib.load(), name)
+    if torch.cuda.current_device() == dev.index:
+        rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    if rc:
+        check(rc, name)
+
+
+def cache_reserve(lens: torch.Tensor, new_lens: torch.Tensor, table: torch.Tensor, free: torch.Tensor,
+                  state: torch.Tensor, block_size: int, out=None):
+    """Pages for new_lens (B,) more tokens of each sequence (ssa_cache_reserve):
+    fills `table` (B, max_blocks) from the stack `free` (num_pages,), whose
+    first state[0] entries are free. Returns (start, lens, state): the lengths
+    before and after, and [pages left, sequences refused so far]. A sequence
+    that the table or the pool cannot hold keeps its length. All int32. out:
+    the three result tensors (lens and state may be the inputs themselves)."""
+    dev = _require_cuda(lens, new_lens, table, free, state)
+    if lens.dim() != 1 or table.dim() != 2 or free.dim() != 1:
+        raise ValueError("cache_reserve: lens (B,), table (B, max_blocks) and free (num_pages,) expected")
+    B, mb = lens.shape[0], table.shape[1]
+    if out is None:
+        out = torch.empty_like(lens), torch.empty_like(lens), torch.empty_like(state)
+    i32, c = torch.int32, _cache_tensor
+    start, after, st = out
+    pl, ps = c("lens", lens, i32, (B,), dev), c("state", state, i32, (2,), dev)
+    _cache_call(dev, "ssa_cache_reserve", B, mb, block_size, free.shape[0], pl,
+                c("new_lens", new_lens, i32, (B,), dev), c("table", table, i32, (B, mb), dev),
+                c("free", free, i32, (free.shape[0],), dev), ps, c("start", start, i32, (B,), dev),
+                c("lens (out)", after, i32, (B,), dev), c("state (out)", st, i32, (2,), dev))
+    return start, after, st
+
+
+def _cache_lens(table, start, lens, dev):
+    B = table.shape[0]
+    return (_cache_tensor("table", table, torch.int32, tuple(table.shape), dev),
+            _cache_tensor("start", start, torch.int32, (B,), dev), _cache_tensor("lens", lens, torch.int32, (B,), dev))
+
+
+def cache_append(k: torch.Tensor, v: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor, amax: torch.Tensor,
+                 bounds: torch.Tensor, tail: torch.Tensor, table: torch.Tensor, start: torch.Tensor,
+                 lens: torch.Tensor, want_values: bool = False):
+    """Appends the step's tokens k, v (B, n_kv, n, d) -- row i of sequence b is
+    position start[b] + i, rows from lens[b] - start[b] on are padding -- to
+    the cache in 8 bits (ssa_cache_append). Writes k_codes, v_codes, amax,
+    bounds and tail in place; with want_values returns (k, v) as the cache now
+    holds them, (B, n_kv, n, d) in the input's type, 0 for padding."""
+    dev = _require_cuda(k, v, k_codes, v_codes, amax, bounds, tail, table, start, lens)
+    if k.dtype != v.dtype or k.shape != v.shape:
+        raise ValueError(f"k {k.dtype} {tuple(k.shape)} and v {v.dtype} {tuple(v.shape)} differ")
+    k, ksb, ksh, ksn = _rows(k)
+    v, vsb, vsh, vsn = _rows(v)
+    B, n_kv, n, d = k.shape
+    if k_codes.dim() != 4 or table.dim() != 2 or table.shape[0] != B:
+        raise ValueError(f"k_codes {tuple(k_codes.shape)} / table {tuple(table.shape)} do not match k {tuple(k.shape)}")
+    P, bs = k_codes.shape[0], k_codes.shape[2]
+    if n == 0 or B == 0:
+        return (k.clone(), v.clone()) if want_values else None
+    c, i8 = _cache_tensor, torch.int8
+    ptrs = (c("k_codes", k_codes, i8, (P, n_kv, bs, d), dev), c("v_codes", v_codes, i8, (P, n_kv, bs, d), dev),
+            c("amax", amax, torch.float32, (P, n_kv, 2), dev), c("bounds", bounds, i8, (P, n_kv, 2, d), dev),
+            c("tail", tail, k.dtype, (B, n_kv, 2, bs, d), dev), *_cache_lens(table, start, lens, dev))
+    kv = vv = None
+    os_ = (0, 0, 0)
+    if want_values:
+        both = torch.empty((2, B, n, n_kv, d), dtype=k.dtype, device=dev)
+        kv, vv = both[0].transpose(1, 2), both[1].transpose(1, 2)
+        os_ = (n * n_kv * d, d, n_kv * d)
+    p = CacheParams(B, n_kv, n_kv, n, d, _dtype_code(k), bs, table.shape[1], P, 0, 0, 0, 0, 0.0, 0, 0, 0,
+                    ksb, ksh, ksn, vsb, vsh, vsn, *os_)
+    _cache_call(dev, "ssa_cache_append", p, k.data_ptr(), v.data_ptr(), *ptrs,
+                kv.data_ptr() if want_values else None, vv.data_ptr() if want_values else None)
+    return (kv, vv) if want_values else None
+
+
+def cache_select(q: torch.Tensor, bounds: torch.Tensor, amax: torch.Tensor, table: torch.Tensor,
+                 start: torch.Tensor, lens: torch.Tensor, top: int, block_size: int, sink: int = 1,
+                 local: int = 1) -> torch.Tensor:
+    """For each token of q (B, H, n, d) and kv head the `top` blocks of its
+    sequence that may hold the largest q.k (ssa_cache_select): (B, n, n_kv,
+    top) int32 block numbers, ascending, -1 behind. The first `sink` blocks and
+    the last `local` up to the token's own are always among them."""
+    dev = _require_cuda(q, bounds, amax, table, start, lens)
+    q, qsb, qsh, qsn = _rows(q)
+    B, H, n, d = q.shape
+    if bounds.dim() != 4 or table.dim() != 2 or table.shape[0] != B:
+        raise ValueError(f"bounds {tuple(bounds.shape)} / table {tuple(table.shape)} do not match q {tuple(q.shape)}")
+    P, n_kv = bounds.shape[:2]
+    out = torch.empty((B, n, n_kv, top), dtype=torch.int32, device=dev)
+    if n == 0 or B == 0:
+        return out
+    p = CacheParams(B, H, n_kv, n, d, _dtype_code(q), block_size, table.shape[1], P, top, sink, local, 1, 0.0,
+                    qsb, qsh, qsn)
+    _cache_call(dev, "ssa_cache_select", p, q.data_ptr(),
+                _cache_tensor("bounds", bounds, torch.int8, (P, n_kv, 2, d), dev),
+                _cache_tensor("amax", amax, torch.float32, (P, n_kv, 2), dev), *_cache_lens(table, start, lens, dev),
+                out.data_ptr())
+    return out
+
+
+def cache_attention(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor, amax: torch.Tensor,
+                    table: torch.Tensor, start: torch.Tensor, lens: torch.Tensor, scale: float,
+                    blocks: Optional[torch.Tensor] = None, causal: bool = True, want_lse: bool = False):
+    """Attention of the step's tokens q (B, H, n, d) over the 8-bit cache
+    (ssa_cache_attn): every block of a sequence, or the distinct blocks that
+    `blocks` (B, n, n_kv, top) names (cache_select). Token i of sequence b sits
+    at position start[b] + i and sees keys up to itself (causal) or all lens[b].
+    Returns out (B, H, n, d) in the (B, n, H, d) layout the output projection
+    reads and, with want_lse, the fp32 log of the weights' sum (B, H, n). Rows
+    without a key and padding rows are 0 and -inf. Inference only: no gradient."""
+    dev = _require_cuda(q, k_codes, v_codes, amax, table, start, lens, blocks)
+    if q.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("cache_attention has no gradient: call it under torch.no_grad()")
+    q, qsb, qsh, qsn = _rows(q)
+    B, H, n, d = q.shape
+    if k_codes.dim() != 4 or table.dim() != 2 or table.shape[0] != B:
+        raise ValueError(f"k_codes {tuple(k_codes.shape)} / table {tuple(table.shape)} do not match q {tuple(q.shape)}")
+    P, n_kv, bs = k_codes.shape[:3]
+    out = torch.empty((B, n, H, d), dtype=q.dtype, device=dev).transpose(1, 2)
+    lse = torch.empty((B, H, n), dtype=torch.float32, device=dev) if want_lse else None
+    if n and B:
+        top, pb = 0, None
+        if blocks is not None:
+            if blocks.dim() != 4:
+                raise ValueError(f"blocks (B, n, n_kv, top) expected, got {tuple(blocks.shape)}")
+            top = blocks.shape[3]
+            pb = _cache_tensor("blocks", blocks, torch.int32, (B, n, n_kv, top), dev)
+        p = CacheParams(B, H, n_kv, n, d, _dtype_code(q), bs, table.shape[1], P, top, 0, 0, 1 if causal else 0, scale,
+                        qsb, qsh, qsn, 0, 0, 0, 0, 0, 0, n * H * d, d, H * d)
+        ws_bytes = _lib.load().ssa_cache_attn_workspace_size(p, pb is not None)
+        ws = torch.empty(max(ws_bytes, 1), dtype=torch.uint8, device=dev)
+        _cache_call(dev, "ssa_cache_attn", p, q.data_ptr(),
+                    _cache_tensor("k_codes", k_codes, torch.int8, (P, n_kv, bs, d), dev),
+                    _cache_tensor("v_codes", v_codes, torch.int8, (P, n_kv, bs, d), dev),
+                    _cache_tensor("amax", amax, torch.float32, (P, n_kv, 2), dev),
+                    *_cache_lens(table, start, lens, dev), pb, out.data_ptr(),
+                    lse.data_ptr() if want_lse else None, ws.data_ptr(), ws_bytes)
+    return (out, lse) if want_lse else out
 
 
 def neighbor_overlap(nb_a: torch.Tensor, nb_b: torch.Tensor, valid_a: torch.Tensor,
