@@ -103,16 +103,75 @@ __global__ void __launch_bounds__(kReserveThreads) k_cache_reserve(const Reserve
 // step stay far inside the fp32 range.
 constexpr float kTinyAmax = 0x1p-80f;
 
-// rint(127 x / amax), ties to even, as in exact arithmetic. 127 / amax and
-// the product are each within 2^-24 of their values, so t is within 2e-5 of
-// the quotient; only where that could decide the rounding is the quotient
+// rint(127 x / amax), ties to even, as in exact arithmetic. inv = 127 / amax
+// and the product are each within 2^-24 of their values, so t is within 2e-5
+// of the quotient; only where that could decide the rounding is the quotient
 // formed in 64 bits (127 x is exact there, and a quotient that is not a tie
 // is further than 2^-53 from one).
-__device__ __forceinline__ int quantize(float x, float inv, float amax) {
-  const float t = x * inv;
-  float r = rintf(t);
-  if (fabsf(t - r) > 0.4999f) r = (float)rint((double)x * 127.0 / (double)amax);
-  return (int)r;
+constexpr float kRound = 12582912.f;  // 1.5 2^23: t + kRound is rounded to a whole number, its low byte the code
+
+__device__ __noinline__ float quantize_exact(float x, float amax) {
+  return kRound + (float)rint((double)x * 127.0 / (double)amax);
+}
+
+// Four codes of x as bytes; r: the codes as floats. inv = 0: all zero.
+__device__ __forceinline__ uint32_t quantize4(const float4& x, float inv, float amax, float4& r) {
+  const float4 t = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+  float4 b = make_float4(t.x + kRound, t.y + kRound, t.z + kRound, t.w + kRound);
+  r = make_float4(b.x - kRound, b.y - kRound, b.z - kRound, b.w - kRound);
+  const float far = fmaxf(fmaxf(fabsf(t.x - r.x), fabsf(t.y - r.y)), fmaxf(fabsf(t.z - r.z), fabsf(t.w - r.w)));
+  if (far > 0.4999f) {
+    b = make_float4(quantize_exact(x.x, amax), quantize_exact(x.y, amax), quantize_exact(x.z, amax), quantize_exact(x.w, amax));
+    r = make_float4(b.x - kRound, b.y - kRound, b.z - kRound, b.w - kRound);
+  }
+  const uint32_t lo = __byte_perm(__float_as_uint(b.x), __float_as_uint(b.y), 0x0040);
+  const uint32_t hi = __byte_perm(__float_as_uint(b.z), __float_as_uint(b.w), 0x0040);
+  return __byte_perm(lo, hi, 0x5410);
+}
+
+// Four consecutive elements as they lie in memory, and packed minima and
+// maxima of them (NaN stays).
+template <int DT>
+struct Vec4;
+template <>
+struct Vec4<kDtF32> {
+  float4 v;
+  __device__ __forceinline__ void zero() { v = make_float4(0.f, 0.f, 0.f, 0.f); }
+  __device__ __forceinline__ void load(const void* p) { v = *static_cast<const float4*>(p); }
+  __device__ __forceinline__ void load_nc(const void* p) { v = __ldg(static_cast<const float4*>(p)); }
+  __device__ __forceinline__ void store(void* p) const { *static_cast<float4*>(p) = v; }
+  __device__ __forceinline__ float4 f() const { return v; }
+  static __device__ __forceinline__ float mn(float a, float b) { float r; asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
+  static __device__ __forceinline__ float mx(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
+  __device__ __forceinline__ void min_with(const Vec4& o) { v = make_float4(mn(v.x, o.v.x), mn(v.y, o.v.y), mn(v.z, o.v.z), mn(v.w, o.v.w)); }
+  __device__ __forceinline__ void max_with(const Vec4& o) { v = make_float4(mx(v.x, o.v.x), mx(v.y, o.v.y), mx(v.z, o.v.z), mx(v.w, o.v.w)); }
+  __device__ __forceinline__ void from(const float4& x) { v = x; }
+};
+template <>
+struct Vec4<kDtBF16> {
+  uint2 v;
+  __device__ __forceinline__ void zero() { v = make_uint2(0u, 0u); }
+  __device__ __forceinline__ void load(const void* p) { v = *static_cast<const uint2*>(p); }
+  __device__ __forceinline__ void load_nc(const void* p) { v = __ldg(static_cast<const uint2*>(p)); }
+  __device__ __forceinline__ void store(void* p) const { *static_cast<uint2*>(p) = v; }
+  __device__ __forceinline__ float4 f() const {
+    return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16),
+                       __uint_as_float(v.y & 0xffff0000u));
+  }
+  static __device__ __forceinline__ uint32_t mn(uint32_t a, uint32_t b) { uint32_t r; asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
+  static __device__ __forceinline__ uint32_t mx(uint32_t a, uint32_t b) { uint32_t r; asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
+  __device__ __forceinline__ void min_with(const Vec4& o) { v = make_uint2(mn(v.x, o.v.x), mn(v.y, o.v.y)); }
+  __device__ __forceinline__ void max_with(const Vec4& o) { v = make_uint2(mx(v.x, o.v.x), mx(v.y, o.v.y)); }
+  __device__ __forceinline__ void from(const float4& x) {
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(v.x) : "f"(x.y), "f"(x.x));
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(v.y) : "f"(x.w), "f"(x.z));
+  }
+};
+
+// |x| as an integer orders like |x|, with infinities and NaN above.
+__device__ __forceinline__ uint32_t abs_top(const float4& x) {
+  return max(max(__float_as_uint(x.x) & 0x7fffffffu, __float_as_uint(x.y) & 0x7fffffffu),
+             max(__float_as_uint(x.z) & 0x7fffffffu, __float_as_uint(x.w) & 0x7fffffffu));
 }
 
 // Threads of a block: at most 8 vectors of four elements each, and a whole
@@ -121,104 +180,109 @@ template <int D, int BS>
 constexpr int kAppendThreads = BS * D / 16 < (D == 96 ? 192 : 256) ? BS * D / 16 : (D == 96 ? 192 : 256);
 
 // One block of a sequence, one kv head, K or V: read the block's tokens (old
-// ones from the tail, new ones from the step's input), their amax, the codes.
+// ones from the tail, new ones from the step's input), their least and
+// greatest values -- which give the amax and, rounding being monotone, the
+// bounds -- then the codes. The tokens stay in registers as they came.
 template <int DT, int D, int BS>
 __device__ __forceinline__ void append_block(const CacheDev& c, int b, int kv, int s, int blk, int start, int len,
-                                             uint32_t* red) {
+                                             float4* red) {
+  using V = Vec4<DT>;
   constexpr int kT = kAppendThreads<D, BS>;
   constexpr int kVec = D / 4, kRg = kT / kVec, kPasses = BS / kRg;
+  constexpr int kSize = DT == kDtF32 ? 4 : 2;
   const int tid = threadIdx.x, cv = tid % kVec, r0 = tid / kVec;
   const int p0 = blk * BS;
   const int page = p0 < len ? cache_page(c, b, blk) : -1;  // a block of padding is only cleared in the values
-  const void* in = s ? c.v : c.k;
-  const int64_t in_off = s ? b * c.v_sb + kv * c.v_sh : b * c.k_sb + kv * c.k_sh;
-  const int64_t in_sn = s ? c.v_sn : c.k_sn;
-  const int64_t tail_off = (((int64_t)b * c.n_kv + kv) * 2 + s) * BS * D;
-  float4 x[kPasses];
-  uint32_t top = 0;
+  // rows of the block: [0, old) from the tail, [old, end) from the input, the rest absent
+  const int old = page < 0 ? 0 : max(0, min(BS, start - p0)), end = page < 0 ? 0 : min(BS, len - p0);
+  const int64_t sn = s ? c.v_sn : c.k_sn;
+  const char* in = static_cast<const char*>(s ? c.v : c.k) +
+                   ((s ? b * c.v_sb + kv * c.v_sh : b * c.k_sb + kv * c.k_sh) + (int64_t)(p0 - start) * sn + cv * 4) * kSize;
+  char* tail = static_cast<char*>(c.tail) + (((((int64_t)b * c.n_kv + kv) * 2 + s) * BS) * D + cv * 4) * kSize;
+  V x[kPasses];
 #pragma unroll
   for (int p = 0; p < kPasses; ++p) {
-    const int row = p * kRg + r0, pos = p0 + row;
-    x[p] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (page >= 0 && pos < len) {
-      // tail rows written by this block are never read by it: plain loads
-      if (pos < start) {
-        const void* t = row_ptr<DT>(c.tail, tail_off + (int64_t)row * D);
-        if constexpr (DT == kDtF32) x[p] = *reinterpret_cast<const float4*>(static_cast<const float*>(t) + cv * 4);
-        else {
-          const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(t) + cv * 4);
-          x[p] = make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u),
-                             __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xffff0000u));
-        }
-      } else {
-        x[p] = load4<DT>(row_ptr<DT>(in, in_off + (int64_t)(pos - start) * in_sn), cv * 4);
-      }
-    }
-    // |x| as an integer orders like |x|, with infinities and NaN above
-    const uint32_t a = max(__float_as_uint(x[p].x) & 0x7fffffffu, __float_as_uint(x[p].y) & 0x7fffffffu);
-    const uint32_t e = max(__float_as_uint(x[p].z) & 0x7fffffffu, __float_as_uint(x[p].w) & 0x7fffffffu);
-    top = max(top, max(a, e));
+    const int row = p * kRg + r0;
+    x[p].zero();
+    if (row >= old && row < end) x[p].load_nc(in + row * sn * kSize);
   }
+  if (old) {
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+      const int row = p * kRg + r0;
+      if (row < old) x[p].load(tail + (int64_t)row * D * kSize);
+    }
+  }
+  // Absent rows are zero: the amax does not see them, and bounds are of whole blocks.
+  V lo = x[0], hi = x[0];
+#pragma unroll
+  for (int p = 1; p < kPasses; ++p) {
+    lo.min_with(x[p]);
+    hi.max_with(x[p]);
+  }
+  uint32_t top = max(abs_top(lo.f()), abs_top(hi.f()));
   top = __reduce_max_sync(0xffffffffu, top);
-  if ((tid & 31) == 0) red[tid >> 5] = top;
+  uint32_t* rt = reinterpret_cast<uint32_t*>(red);
+  if ((tid & 31) == 0) rt[tid >> 5] = top;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kT / 32; ++i) top = max(top, red[i]);
+  for (int i = 0; i < kT / 32; ++i) top = max(top, rt[i]);
   float amax = __uint_as_float(top);
   if (amax < kTinyAmax) amax = 0.f;
-  const float inv = amax > 0.f && amax < INFINITY ? __fdiv_rn(127.f, amax) : 0.f;
+  const bool finite = amax > 0.f && amax < INFINITY;
+  const float inv = finite ? __fdiv_rn(127.f, amax) : 0.f;
   const float step = __fdiv_rn(amax, 127.f);
   if (tid == 0 && page >= 0) c.amax[((int64_t)page * c.n_kv + kv) * 2 + s] = amax;
-  int8_t* codes = (s ? c.v_codes : c.k_codes) + ((int64_t)page * c.n_kv + kv) * BS * D;
-  void* values = s ? c.v_values : c.k_values;
-  const bool open = p0 + BS > len, whole = !open && s == 0;
-  uint32_t lo = 0x7f7f7f7fu, hi = 0x81818181u;
+  if (!finite) {  // no codes: zeros, which stand for 0 or for NaN
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) x[p].zero();
+    lo.zero();
+    hi.zero();
+    // 0 * step is the value of every code: 0, or NaN of an amax that is infinite or NaN
+  }
+  int8_t* codes = (s ? c.v_codes : c.k_codes) + ((int64_t)page * c.n_kv + kv) * BS * D + cv * 4;
+  char* values = static_cast<char*>(s ? c.v_values : c.k_values);
+  const bool open = p0 + BS > len;
+  if (values) values += (b * c.o_sb + kv * c.o_sh + (int64_t)(p0 - start) * c.o_sn + cv * 4) * kSize;
 #pragma unroll
   for (int p = 0; p < kPasses; ++p) {
-    const int row = p * kRg + r0, pos = p0 + row;
-    const bool have = page >= 0 && pos < len;
-    int q0 = 0, q1 = 0, q2 = 0, q3 = 0;
-    if (inv > 0.f) {
-      q0 = quantize(x[p].x, inv, amax); q1 = quantize(x[p].y, inv, amax);
-      q2 = quantize(x[p].z, inv, amax); q3 = quantize(x[p].w, inv, amax);
+    const int row = p * kRg + r0;
+    const bool have = row < end;
+    float4 r;
+    const uint32_t q = quantize4(x[p].f(), inv, amax, r);
+    if (have) *reinterpret_cast<uint32_t*>(codes + row * D) = q;
+    if (values && p0 + row >= start && p0 + row - start < c.n) {
+      V o;
+      o.zero();
+      if (have) o.from(make_float4(r.x * step, r.y * step, r.z * step, r.w * step));
+      o.store(values + row * c.o_sn * kSize);
     }
-    const uint32_t q = (q0 & 255) | (q1 & 255) << 8 | (q2 & 255) << 16 | (uint32_t)(q3 & 255) << 24;
-    if (have) *reinterpret_cast<uint32_t*>(codes + row * D + cv * 4) = q;
-    lo = __vmins4(lo, q);
-    hi = __vmaxs4(hi, q);
-    if (pos >= start && pos - start < c.n) {
-      if (values) {
-        const int64_t at = b * c.o_sb + kv * c.o_sh + (int64_t)(pos - start) * c.o_sn + cv * 4;
-        const float v0 = have ? q0 * step : 0.f, v1 = have ? q1 * step : 0.f;
-        const float v2 = have ? q2 * step : 0.f, v3 = have ? q3 * step : 0.f;
-        if constexpr (DT == kDtF32) *reinterpret_cast<float4*>(static_cast<float*>(values) + at) = make_float4(v0, v1, v2, v3);
-        else
-          *reinterpret_cast<uint2*>(static_cast<uint16_t*>(values) + at) =
-              make_uint2(f32_to_bf16_bits(v0) | (uint32_t)f32_to_bf16_bits(v1) << 16,
-                         f32_to_bf16_bits(v2) | (uint32_t)f32_to_bf16_bits(v3) << 16);
-      }
-      if (open && have) {
-        void* t = row_ptr_mut<DT>(c.tail, tail_off + (int64_t)row * D + cv * 4);
-        if constexpr (DT == kDtF32) *static_cast<float4*>(t) = x[p];
-        else
-          *static_cast<uint2*>(t) = make_uint2(__float_as_uint(x[p].x) >> 16 | (__float_as_uint(x[p].y) & 0xffff0000u),
-                                               __float_as_uint(x[p].z) >> 16 | (__float_as_uint(x[p].w) & 0xffff0000u));
+  }
+  if (open) {  // the open block's new tokens, as they came (zeroed above where there are no codes: read again)
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+      const int row = p * kRg + r0;
+      if (row >= old && row < end) {
+        if (!finite) x[p].load_nc(in + row * sn * kSize);
+        x[p].store(tail + (int64_t)row * D * kSize);
       }
     }
   }
   __syncthreads();  // red is free again
-  if (whole && page >= 0) {
-    red[tid] = lo;
-    red[kT + tid] = hi;
+  if (!open && s == 0 && page >= 0) {
+    V* rl = reinterpret_cast<V*>(red);
+    rl[tid] = lo;
+    rl[kT + tid] = hi;
     __syncthreads();
     if (tid < kVec) {
       for (int i = 1; i < kRg; ++i) {
-        lo = __vmins4(lo, red[i * kVec + tid]);
-        hi = __vmaxs4(hi, red[kT + i * kVec + tid]);
+        lo.min_with(rl[i * kVec + tid]);
+        hi.max_with(rl[kT + i * kVec + tid]);
       }
-      int8_t* bd = c.bounds + ((int64_t)page * c.n_kv + kv) * 2 * D + tid * 4;
-      *reinterpret_cast<uint32_t*>(bd) = lo;
-      *reinterpret_cast<uint32_t*>(bd + D) = hi;
+      float4 r;
+      uint32_t* bd = reinterpret_cast<uint32_t*>(c.bounds + ((int64_t)page * c.n_kv + kv) * 2 * D) + tid;
+      bd[0] = quantize4(lo.f(), inv, amax, r);
+      bd[D / 4] = quantize4(hi.f(), inv, amax, r);
     }
     __syncthreads();
   }
@@ -229,7 +293,7 @@ __device__ __forceinline__ void append_block(const CacheDev& c, int b, int kv, i
 // that order.
 template <int DT, int D, int BS>
 __global__ void __launch_bounds__(kAppendThreads<D, BS>) k_cache_append(const CacheDev c, const int nt) {
-  __shared__ uint32_t red[2 * kAppendThreads<D, BS>];
+  __shared__ float4 red[(DT == kDtF32 ? 2 : 1) * kAppendThreads<D, BS>];
   int64_t i = blockIdx.x;
   const int j = (int)(i % nt);
   i /= nt;
@@ -314,8 +378,7 @@ __global__ void __launch_bounds__(kSelThreads) k_cache_select(const CacheDev c) 
     uint32_t top = 0;
     for (int i = tid; i < c.rep * (D / 4); i += kSelThreads) {
       const float4 x = load4<DT>(row_ptr<DT>(c.q, q0 + (int64_t)(i / (D / 4)) * c.q_sh), i % (D / 4) * 4);
-      top = max(top, max(max(__float_as_uint(x.x) & 0x7fffffffu, __float_as_uint(x.y) & 0x7fffffffu),
-                         max(__float_as_uint(x.z) & 0x7fffffffu, __float_as_uint(x.w) & 0x7fffffffu)));
+      top = max(top, abs_top(x));
     }
     top = __reduce_max_sync(0xffffffffu, top);
     if (lane == 0) red[w] = top;
@@ -329,12 +392,10 @@ __global__ void __launch_bounds__(kSelThreads) k_cache_select(const CacheDev c) 
       uint32_t neg = 0, pos = 0;
       if (head < c.rep && inv > 0.f) {
         const float4 x = load4<DT>(row_ptr<DT>(c.q, q0 + (int64_t)head * c.q_sh), cache_word_channel<D>(wd, ln & 3));
-        const int v[4] = {quantize(x.x, inv, amax), quantize(x.y, inv, amax), quantize(x.z, inv, amax), quantize(x.w, inv, amax)};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          neg |= (uint32_t)(min(v[e], 0) & 255) << (8 * e);
-          pos |= (uint32_t)max(v[e], 0) << (8 * e);
-        }
+        float4 r;
+        const uint32_t v = quantize4(x, inv, amax, r), sign = (v >> 7 & 0x01010101u) * 255u;
+        neg = v & sign;
+        pos = v & ~sign;
       }
       qf[((ht * 2 + 0) * (D / 16) + wd) * 32 + ln] = neg;
       qf[((ht * 2 + 1) * (D / 16) + wd) * 32 + ln] = pos;

@@ -178,6 +178,7 @@ __global__ void __launch_bounds__(kThreads) k_cache_attn(const CacheDev c, const
   __shared__ int s_b;
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t = lane & 3;
   const int bs_shift = c.bs == 16 ? 4 : c.bs == 32 ? 5 : 6;
+  asm volatile("griddepcontrol.launch_dependents;");  // k_cache_combine may take its place and wait
 
   // this block's range of the work, and the sequence it starts in
   int64_t total;
@@ -222,6 +223,7 @@ __global__ void __launch_bounds__(kThreads) k_cache_attn(const CacheDev c, const
       if (blockIdx.x == 0 && b0 + tid < c.B) c.prefix[b0 + tid] = from;
       before += all;
     }
+    if (blockIdx.x == 0 && tid == 0) c.prefix[c.B] = total;
   }
   __syncthreads();
   if (lo >= hi) return;
@@ -492,65 +494,70 @@ __global__ void __launch_bounds__(kThreads) k_cache_attn(const CacheDev c, const
   }
 }
 
-// One thread block for each unit: joins the partial sums of a unit that
-// several blocks worked on, and writes zeros to rows that have no work.
+// One warp for each query row: joins the partial sums of a unit that several
+// blocks worked on, in range order, and writes zeros to rows without work. It
+// is launched while k_cache_attn still runs and waits for it behind its set-up.
 template <int D, int NT, bool F32>
-__global__ void __launch_bounds__(kThreads) k_cache_combine(const CacheDev c, const Plan pl, const int ngrid) {
-  constexpr int ROWS = 8 * NT;
-  __shared__ int64_t red[kWarps];
-  const int tid = threadIdx.x;
+__global__ void __launch_bounds__(kThreads) k_cache_combine(const CacheDev c, const Plan pl, const int ngrid,
+                                                            const int rows_used, const int64_t nrows) {
+  constexpr int ROWS = 8 * NT, E = D / 32;
+  const int lane = threadIdx.x & 31;
+  const int64_t id = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+  // Every warp waits, so that this kernel's end implies the other's.
+  if (id >= nrows) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    return;
+  }
+  const int r = (int)(id % rows_used);
   const int per = pl.tiles_max * (c.blocks ? c.n : 1);  // row tiles a (sequence, kv head) can have
-  const int b = (int)(blockIdx.x / ((unsigned)per * c.n_kv)), u = (int)(blockIdx.x % ((unsigned)per * c.n_kv));
+  const int64_t unit = id / rows_used;
+  const int b = (int)(unit / ((int64_t)per * c.n_kv)), u = (int)(unit % ((int64_t)per * c.n_kv));
   const int kv = u / per, tile = u % per;
   int tiles, groups;
   const int64_t mine = seq_work(c, pl, b, ROWS, &tiles, &groups);
-  Unit x = unit_of<ROWS>(c, pl, b, kv * per + tile, per);
-  const int rows_all = c.blocks ? min(ROWS, c.rep - tile % pl.tiles_max * ROWS) : min(ROWS, c.n * c.rep - x.row0);
-  const bool work = tile < tiles && mine > 0;
-  if (!work || x.nrows < rows_all) {
-    for (int i = tid; i < rows_all * (D / 4); i += kThreads) {
-      const int r = i / (D / 4), ch = i % (D / 4) * 4;
-      if (work && r < x.nrows) continue;
-      store_out<F32>(c, x, r, ch, make_float4(0.f, 0.f, 0.f, 0.f));
-      if (ch == 0 && c.lse) store_lse(c, x, r, 0.f, 0.f);
+  const Unit x = unit_of<ROWS>(c, pl, b, u, per);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (r >= (c.blocks ? c.rep - tile % pl.tiles_max * ROWS : c.n * c.rep - x.row0)) return;
+  const int row = x.row0 + r, tok = row / c.rep, h = kv * c.rep + row - tok * c.rep;
+  const int64_t at = x.b * c.o_sb + h * c.o_sh + tok * c.o_sn;
+  float m = kEmpty, l = 0.f, o[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) o[i] = 0.f;
+  if (tile < tiles && mine > 0 && r < x.nrows) {
+    const int64_t total = c.blocks ? mine * c.B : c.prefix[c.B], base = c.blocks ? mine * b : c.prefix[b];
+    const int64_t ubeg = base + ((int64_t)kv * tiles + tile) * groups, uend = ubeg + groups;
+    // block i holds [i total / nblk, (i + 1) total / nblk)
+    const int nblk = ranges_of(total, ngrid);
+    const int c0 = (int)(((ubeg + 1) * nblk - 1) / total), c1 = (int)((uend * nblk - 1) / total);
+    if (c0 == c1) return;  // that block stored the row
+    const auto slot = [&](int k) { return ((int64_t)k * 2 + (k == c0)) * ROWS + r; };
+    for (int k = c0 + lane; k <= c1; k += 32) m = fmaxf(m, c.part_ml[slot(k) * 2]);
+#pragma unroll
+    for (int q = 16; q; q >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, q));
+    for (int k0 = c0; k0 <= c1; k0 += 32) {
+      float f = 0.f;
+      if (k0 + lane <= c1) {
+        const float2 ml = *reinterpret_cast<const float2*>(c.part_ml + slot(k0 + lane) * 2);
+        f = ex2(ml.x - m);
+        l = fmaf(f, ml.y, l);
+      }
+      const int cnt = min(32, c1 - k0 + 1);
+#pragma unroll 4
+      for (int j = 0; j < cnt; ++j) {
+        const float fj = __shfl_sync(0xffffffffu, f, j);
+        const float* p = c.part_o + slot(k0 + j) * D + lane;
+#pragma unroll
+        for (int i = 0; i < E; ++i) o[i] = fmaf(fj, p[32 * i], o[i]);
+      }
     }
-    if (!work) return;
+#pragma unroll
+    for (int q = 16; q; q >>= 1) l += __shfl_xor_sync(0xffffffffu, l, q);
   }
-  int64_t total, base;
-  if (c.blocks) {
-    total = mine * c.B;
-    base = mine * b;
-  } else {
-    int64_t sum = 0;
-    int a, e;
-    for (int i = tid; i < c.B; i += kThreads) sum += seq_work(c, pl, i, ROWS, &a, &e);
-    total = block_sum64(sum, red);
-    base = c.prefix[b];
-  }
-  const int64_t ubeg = base + ((int64_t)kv * tiles + tile) * groups, uend = ubeg + groups;
-  // block i holds [i total / nblk, (i + 1) total / nblk)
-  const int nblk = ranges_of(total, ngrid);
-  const int c0 = (int)(((ubeg + 1) * nblk - 1) / total), c1 = (int)((uend * nblk - 1) / total);
-  if (c0 == c1) return;
-  for (int i = tid; i < ROWS * (D / 4); i += kThreads) {
-    const int r = i / (D / 4), ch = i % (D / 4) * 4;
-    if (r >= x.nrows) break;
-    float m = kEmpty;
-    for (int k = c0; k <= c1; ++k) m = fmaxf(m, c.part_ml[(((int64_t)k * 2 + (k == c0)) * ROWS + r) * 2]);
-    float l = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int k = c0; k <= c1; ++k) {
-      const int64_t slot = ((int64_t)k * 2 + (k == c0)) * ROWS + r;
-      const float2 ml = *reinterpret_cast<const float2*>(c.part_ml + slot * 2);
-      const float f = ex2(ml.x - m);
-      l = fmaf(f, ml.y, l);
-      const float4 v = *reinterpret_cast<const float4*>(c.part_o + slot * D + ch);
-      o.x = fmaf(f, v.x, o.x); o.y = fmaf(f, v.y, o.y); o.z = fmaf(f, v.z, o.z); o.w = fmaf(f, v.w, o.w);
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    store_out<F32>(c, x, r, ch, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
-    if (ch == 0 && c.lse) store_lse(c, x, r, m, l);
-  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int i = 0; i < E; ++i)
+    store1<F32 ? kDtF32 : kDtBF16>(row_ptr_mut<F32 ? kDtF32 : kDtBF16>(c.out, at), lane + 32 * i, o[i] * inv);
+  if (lane == 0 && c.lse) store_lse(c, x, r, m, l);
 }
 
 // Rows of a tile: 8, 16 or 32 (the rows a group has, as far as they go).
@@ -582,9 +589,21 @@ cudaError_t run_attn(const CacheDev& c, const Plan& pl, cudaStream_t st) {
   k_cache_attn<D, NT, F32><<<c.grid, kThreads, smem, st>>>(c, pl);
   note_launch();
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  k_cache_combine<D, NT, F32><<<(unsigned)units, kThreads, 0, st>>>(c, pl, c.grid);
+  const int rows_used = (int)((c.blocks ? c.rep : (int64_t)c.n * c.rep) < ROWS ? (c.blocks ? c.rep : c.n * c.rep) : ROWS);
+  const int64_t nrows = units * rows_used;
+  if ((nrows + kWarps - 1) / kWarps > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((nrows + kWarps - 1) / kWarps));
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, k_cache_combine<D, NT, F32>, c, pl, (int)c.grid, rows_used, nrows);
   note_launch();
-  return cudaGetLastError();
+  return e;
 }
 
 template <int D, bool F32>
