@@ -73,21 +73,49 @@ __device__ __forceinline__ void split_f16(float a, float b, uint32_t& hi, uint32
   lo = pack_f16(a - f.x, b - f.y);
 }
 
-// D / 8 codes of one key row, channels g * D / 8 and up.
+// A staged tile: 16 key rows of D code bytes, as 16-byte chunks exchanged
+// within 128 bytes so that the eight rows of an 8x8 tile lie in eight banks
+// of 16 bytes (rows of 96 bytes are spaced as rows of 128).
 template <int D>
-__device__ __forceinline__ void load_slice(const int8_t* row, int g, uint32_t (&w)[D / 32]) {
-  const int8_t* p = row + g * (D / 8);
-  if constexpr (D == 128) {
-    const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
-    w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
-  } else if constexpr (D == 64) {
-    const uint2 u = __ldg(reinterpret_cast<const uint2*>(p));
-    w[0] = u.x; w[1] = u.y;
-  } else {
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) w[i] = __ldg(reinterpret_cast<const uint32_t*>(p) + i);
-  }
+constexpr int kPitch = D == 96 ? 128 : D;
+template <int D>
+__device__ __forceinline__ int tile_at(int row, int chunk) {
+  constexpr int kRows = 128 / kPitch<D>;  // rows in 128 bytes
+  return row * kPitch<D> + ((chunk ^ (row / kRows & (kPitch<D> / 16 - 1))) << 4);
 }
+
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy8(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+
+// Shared memory of a block: for each warp a ring of staged tiles (keys and
+// values of 16 keys a stage), used for the warp's partial output afterwards;
+// what comes with each stage; the query operand.
+constexpr int kStages = 4;
+template <int D, int NT, bool F32>
+struct Smem {
+  static constexpr int kTile = 16 * kPitch<D>;
+  static constexpr int kRing = kStages * 2 * kTile, kOut = 8 * NT * (D + 4) * 4;
+  static constexpr int kWarp = kRing > kOut ? kRing : kOut;
+  static constexpr int kMeta = kWarps * kWarp;                           // [kWarps][kStages] {amax k, v, first key, -}
+  static constexpr int kMl = kMeta + kWarps * kStages * 16;              // [kWarps][8 NT] {offset, sum}
+  static constexpr int kQ = kMl + kWarps * 8 * NT * 8;                   // [F32 ? 2 : 1][NT][D / 16][32] uint2
+  static constexpr int kBytes = kQ + (F32 ? 2 : 1) * NT * (D / 16) * 32 * 8;
+};
+// Blocks that share an SM (registers for 16 and 32 rows, the rings for 8).
+constexpr int blocks_per_sm(int d, int rows) { return rows == 32 ? 2 : rows == 16 || d >= 96 ? 3 : 4; }
 
 // Units and work of the call. Without a list a unit is (sequence, kv head,
 // tile of query rows) and its work the sequence's groups of 64 keys; with one
@@ -167,12 +195,13 @@ __device__ __forceinline__ void store_lse(const CacheDev& c, const Unit& x, int 
 }
 
 template <int D, int NT, bool F32>
-__global__ void __launch_bounds__(kThreads) k_cache_attn(const CacheDev c, const Plan pl) {
-  constexpr int ROWS = 8 * NT, W16 = D / 16, VW = D / 32, PC = F32 ? 2 : 1, OP = D + 4;
-  extern __shared__ __align__(16) unsigned char sm[];
-  uint2* qf = reinterpret_cast<uint2*>(sm);                               // [PC][NT][W16][32]
-  float* so = reinterpret_cast<float*>(qf + PC * NT * W16 * 32);          // [kWarps][ROWS][OP]
-  float* sml = so + kWarps * ROWS * OP;                                   // [kWarps][ROWS][2]
+__global__ void __launch_bounds__(kThreads, blocks_per_sm(D, 8 * NT)) k_cache_attn(const CacheDev c, const Plan pl) {
+  using Sm = Smem<D, NT, F32>;
+  constexpr int ROWS = 8 * NT, W16 = D / 16, PC = F32 ? 2 : 1, OP = D + 4;
+  constexpr int kDt = F32 ? kDtF32 : kDtBF16;
+  extern __shared__ __align__(128) unsigned char sm[];
+  uint2* qf = reinterpret_cast<uint2*>(sm + Sm::kQ);
+  float* sml = reinterpret_cast<float*>(sm + Sm::kMl);
   __shared__ int64_t red[kWarps];
   __shared__ int64_t s_base;
   __shared__ int s_b;
@@ -240,22 +269,81 @@ __global__ void __launch_bounds__(kThreads) k_cache_attn(const CacheDev c, const
     at = ubeg + g1;
     const Unit x = unit_of<ROWS>(c, pl, b, u, tiles);
 
+    // keys a row of the tile sees: at least lim_min, at most lim_max
+    const int lim_max = x.nrows <= 0 ? 0 : c.causal ? x.start + (x.row0 + x.nrows - 1) / c.rep + 1 : x.len;
+    const int lim_min = c.causal ? x.start + x.row0 / c.rep + 1 : x.len;
+
+    // The warp's 16 keys of each group, in order, through its ring. Lane l
+    // holds the page of group s0 + l, and of group s0 + 32 + l (loaded ahead).
+    unsigned char* ring = sm + w * Sm::kWarp;
+    const uint32_t ring_a = smem_addr(ring), meta_a = smem_addr(sm + Sm::kMeta + w * kStages * 16);
+    int page, kb, off, page_n, kb_n, off_n;
+    const auto look_up = [&](int s0, int& pg, int& first, int& o) {
+      pg = -1;
+      if (s0 + lane < g1) {
+        const int64_t key = (int64_t)(s0 + lane) * kGroup + w * 16;
+        const int entry = (int)(key >> bs_shift);
+        o = (int)key & (c.bs - 1);
+        const int blk = !x.list ? entry : entry < c.top ? __ldg(x.list + entry) : -1;
+        if (blk >= 0 && blk < c.max_blocks) {
+          first = blk * c.bs + o;
+          if (first < lim_max) pg = cache_page(c, x.b, blk);
+        }
+      }
+    };
+    int s0 = g0;
+    look_up(s0, page, kb, off);
+    look_up(s0 + 32, page_n, kb_n, off_n);
+    uint32_t todo = __ballot_sync(0xffffffffu, page >= 0);
+    int issued = 0, used = 0;
+    const auto issue = [&]() {
+      while (!todo && s0 + 32 < g1) {
+        s0 += 32;
+        page = page_n; kb = kb_n; off = off_n;
+        look_up(s0 + 32, page_n, kb_n, off_n);
+        todo = __ballot_sync(0xffffffffu, page >= 0);
+      }
+      if (todo) {
+        const int j = __ffs(todo) - 1, st = issued & (kStages - 1);
+        todo &= todo - 1;
+        const int64_t head = (int64_t)__shfl_sync(0xffffffffu, page, j) * c.n_kv + x.kv;
+        const int64_t row = head * c.bs + __shfl_sync(0xffffffffu, off, j);
+        const int first = __shfl_sync(0xffffffffu, kb, j);
+        const int8_t* ks = c.k_codes + row * D + lane * 16;
+        const int8_t* vs = c.v_codes + row * D + lane * 16;
+        const uint32_t at = ring_a + st * 2 * Sm::kTile;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+          const int id = i * 32 + lane, to = tile_at<D>(id / W16, id % W16);
+          copy16(at + to, ks + i * 512);
+          copy16(at + Sm::kTile + to, vs + i * 512);
+        }
+        if (lane == 0) {
+          copy8(meta_a + st * 16, c.amax + head * 2);
+          *reinterpret_cast<int*>(sm + Sm::kMeta + (w * kStages + st) * 16 + 8) = first;
+        }
+        ++issued;
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) issue();
+
     // Q as the products' 8-wide operand: rows scaled into fp16's range by a power of two
     float sfac[NT][2];
     int lim[NT][2];
-    int lim_min = INT32_MAX, lim_max = 0;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int r = nt * 8 + g;
       const bool have = r < x.nrows;
       const int row = x.row0 + (have ? r : 0), tok = row / c.rep, h = x.kv * c.rep + row - tok * c.rep;
-      const void* qr = row_ptr<F32 ? kDtF32 : kDtBF16>(c.q, x.b * c.q_sb + h * c.q_sh + tok * c.q_sn);
+      const void* qr = row_ptr<kDt>(c.q, x.b * c.q_sb + h * c.q_sh + tok * c.q_sn);
       float4 v[W16];
       uint32_t top = 0;
 #pragma unroll
       for (int i = 0; i < W16; ++i) {
         v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (have) v[i] = load4<F32 ? kDtF32 : kDtBF16>(qr, cache_word_channel<D>(i, t));
+        if (have) v[i] = load4<kDt>(qr, i * 16 + t * 4);
         top = max(top, max(max(__float_as_uint(v[i].x) & 0x7fffffffu, __float_as_uint(v[i].y) & 0x7fffffffu),
                            max(__float_as_uint(v[i].z) & 0x7fffffffu, __float_as_uint(v[i].w) & 0x7fffffffu)));
       }
@@ -280,15 +368,9 @@ __global__ void __launch_bounds__(kThreads) k_cache_attn(const CacheDev c, const
         sfac[nt][k] = __shfl_sync(0xffffffffu, mine_s, (2 * t + k) * 4);
         const int rr = nt * 8 + 2 * t + k;
         lim[nt][k] = INT32_MAX;  // rows behind the last one: computed, never stored
-        if (rr < x.nrows) {
-          lim[nt][k] = c.causal ? x.start + (x.row0 + rr) / c.rep + 1 : x.len;
-          lim_min = min(lim_min, lim[nt][k]);
-          lim_max = max(lim_max, lim[nt][k]);
-        }
+        if (rr < x.nrows) lim[nt][k] = c.causal ? x.start + (x.row0 + rr) / c.rep + 1 : x.len;
       }
     }
-    lim_min = __reduce_min_sync(0xffffffffu, lim_min);
-    lim_max = __reduce_max_sync(0xffffffffu, lim_max);
     __syncthreads();
 
     float acc[W16][NT][4], mref[NT][2], lsum[NT][2];
@@ -302,146 +384,118 @@ __global__ void __launch_bounds__(kThreads) k_cache_attn(const CacheDev c, const
         for (int k = 0; k < 4; ++k) acc[i][nt][k] = 0.f;
     }
 
-    for (int s0 = g0; s0 < g1; s0 += 32) {
-      // lane l looks up this warp's 16 keys of group s0 + l
-      int page = -1, kb = 0, off = 0;
-      float2 am = make_float2(0.f, 0.f);
-      if (s0 + lane < g1) {
-        const int64_t key = (int64_t)(s0 + lane) * kGroup + w * 16;
-        const int entry = (int)(key >> bs_shift);
-        off = (int)key & (c.bs - 1);
-        const int blk = !x.list ? entry : entry < c.top ? __ldg(x.list + entry) : -1;
-        if (blk >= 0 && blk < c.max_blocks) {
-          kb = blk * c.bs + off;
-          if (kb < lim_max) page = cache_page(c, x.b, blk);
-        }
-        if (page >= 0) am = __ldg(reinterpret_cast<const float2*>(c.amax) + (int64_t)page * c.n_kv + x.kv);
+    // row and half of the 8x8 tile whose row address this lane gives
+    const int mrow = lane & 15, mchunk = lane >> 4;
+    while (true) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+      __syncwarp();  // the oldest stage is there for the whole warp, and the one before it free
+      issue();
+      if (used == issued) break;
+      const int st = used & (kStages - 1);
+      ++used;
+      const uint32_t ka_at = ring_a + st * 2 * Sm::kTile, va_at = ka_at + Sm::kTile;
+      const float4 meta = *reinterpret_cast<const float4*>(sm + Sm::kMeta + (w * kStages + st) * 16);
+      const float ka = meta.x * (1.f / 127.f), va = meta.y * (1.f / 127.f);
+      const int kbj = __float_as_int(meta.z);
+
+      float s[NT][4], s2[NT][4];  // two chains
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s[nt][k] = s2[nt][k] = 0.f;
+#pragma unroll
+      for (int i = 0; i < W16; i += 2) {
+        uint32_t x4[4];  // rows 0-7 and 8-15 of chunk i, then of chunk i + 1: channels 4 t .. 4 t + 3
+        ldmatrix4(x4, ka_at + tile_at<D>(mrow, i + mchunk));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x4[k] ^= 0x80808080u;
+        const uint32_t a[4] = {codes_f16<0x4140>(x4[0]), codes_f16<0x4140>(x4[1]), codes_f16<0x4342>(x4[0]), codes_f16<0x4342>(x4[1])};
+        const uint32_t e[4] = {codes_f16<0x4140>(x4[2]), codes_f16<0x4140>(x4[3]), codes_f16<0x4342>(x4[2]), codes_f16<0x4342>(x4[3])};
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int pc = 0; pc < PC; ++pc) {
+            const uint2 b0 = qf[((pc * NT + nt) * W16 + i) * 32 + lane], b1 = qf[((pc * NT + nt) * W16 + i + 1) * 32 + lane];
+            mma_f16(s[nt], a, b0.x, b0.y);
+            mma_f16(s2[nt], e, b1.x, b1.y);
+          }
       }
-      uint32_t todo = __ballot_sync(0xffffffffu, page >= 0);
-      if (!todo) continue;
-      uint32_t kw0[W16], kw1[W16], vw[4][VW];
-      const auto row_of = [&](const int8_t* codes, int j) {
-        return codes + (((int64_t)__shfl_sync(0xffffffffu, page, j) * c.n_kv + x.kv) * c.bs + __shfl_sync(0xffffffffu, off, j)) * D;
-      };
-      const auto load_k = [&](int j) {
-        const int8_t* p = row_of(c.k_codes, j);
-        cache_load_row<D>(p + g * D, t, kw0);
-        cache_load_row<D>(p + (g + 8) * D, t, kw1);
-      };
-      const auto load_v = [&](int j) {
-        const int8_t* p = row_of(c.v_codes, j);
-        load_slice<D>(p + (2 * t) * D, g, vw[0]);
-        load_slice<D>(p + (2 * t + 1) * D, g, vw[1]);
-        load_slice<D>(p + (2 * t + 8) * D, g, vw[2]);
-        load_slice<D>(p + (2 * t + 9) * D, g, vw[3]);
-      };
-      int j = __ffs(todo) - 1;
-      load_k(j);
-      load_v(j);
-      while (true) {
-        todo &= todo - 1;
-        const int jn = todo ? __ffs(todo) - 1 : -1;
-        const float ka = __shfl_sync(0xffffffffu, am.x, j) * (1.f / 127.f);
-        const float va = __shfl_sync(0xffffffffu, am.y, j) * (1.f / 127.f);
-        const int kbj = __shfl_sync(0xffffffffu, kb, j);
 
-        float s[NT][4];
+      // weights 2^(s' + log2(step_v) - m + 13)
+      const float vs = va > 0.f ? va : 1.f;  // a page of zeros: any step does
+      const float lv = F32 ? log2f(vs) : __log2f(vs), iv = 1.f / vs;
+      const bool edge = kbj + 16 > lim_min;
+      bool move = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          float v = fmaf(s[nt][k] + s2[nt][k], ka * sfac[nt][k & 1], lv);
+          if (edge && kbj + g + 8 * (k >> 1) >= lim[nt][k & 1]) v = -INFINITY;
+          s[nt][k] = v;
+          move |= v > mref[nt][k & 1] + (kHead + kSlack);
+        }
+      if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) s[nt][k] = 0.f;
+          for (int k = 0; k < 2; ++k) {
+            float m = fmaxf(s[nt][k], s[nt][k + 2]);
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+            m = fmaxf(mref[nt][k], m - kHead);
+            const float f = ex2(mref[nt][k] - m);
+            mref[nt][k] = m;
+            lsum[nt][k] *= f;
 #pragma unroll
-        for (int i = 0; i < W16; ++i) {
-          const uint32_t x0 = kw0[i] ^ 0x80808080u, x1 = kw1[i] ^ 0x80808080u;
-          const uint32_t a[4] = {codes_f16<0x4140>(x0), codes_f16<0x4140>(x1), codes_f16<0x4342>(x0), codes_f16<0x4342>(x1)};
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int pc = 0; pc < PC; ++pc) {
-              const uint2 bq = qf[((pc * NT + nt) * W16 + i) * 32 + lane];
-              mma_f16(s[nt], a, bq.x, bq.y);
+            for (int i = 0; i < W16; ++i) {
+              acc[i][nt][k] *= f;
+              acc[i][nt][k + 2] *= f;
             }
+          }
+      }
+      uint32_t pf[PC][NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float p[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) p[k] = ex2(s[nt][k] - mref[nt][k & 1]);
+        lsum[nt][0] = fmaf(p[0] + p[2], iv, lsum[nt][0]);
+        lsum[nt][1] = fmaf(p[1] + p[3], iv, lsum[nt][1]);
+        if constexpr (F32) {
+          uint32_t h0, l0, h1, l1;
+          split_f16(p[0], p[1], h0, l0);
+          split_f16(p[2], p[3], h1, l1);
+          pf[0][nt][0] = transpose8x8(h0);
+          pf[0][nt][1] = transpose8x8(h1);
+          pf[PC - 1][nt][0] = transpose8x8(l0);
+          pf[PC - 1][nt][1] = transpose8x8(l1);
+        } else {
+          pf[0][nt][0] = transpose8x8(pack_f16(p[0], p[1]));
+          pf[0][nt][1] = transpose8x8(pack_f16(p[2], p[3]));
         }
-        if (jn >= 0) load_k(jn);
+      }
 
-        // weights 2^(s' + log2(step_v) - m + 13)
-        const float vs = va > 0.f ? va : 1.f;  // a page of zeros: any step does
-        const float lv = F32 ? log2f(vs) : __log2f(vs), iv = 1.f / vs;
-        const bool edge = kbj + 16 > lim_min;
-        bool move = false;
+      // transposed as pairs of codes: a lane has channels 2 g, 2 g + 1 of keys 2 t, 2 t + 1
+#pragma unroll
+      for (int i = 0; i < W16; i += 2) {
+        uint32_t x4[4];  // keys 0-7 and 8-15 of chunk i, then of chunk i + 1
+        ldmatrix4_trans(x4, va_at + tile_at<D>(mrow, i + mchunk));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x4[k] ^= 0x80808080u;
+        const uint32_t a[4] = {codes_f16<0x4240>(x4[0]), codes_f16<0x4341>(x4[0]), codes_f16<0x4240>(x4[1]), codes_f16<0x4341>(x4[1])};
+        const uint32_t e[4] = {codes_f16<0x4240>(x4[2]), codes_f16<0x4341>(x4[2]), codes_f16<0x4240>(x4[3]), codes_f16<0x4341>(x4[3])};
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            float v = fmaf(s[nt][k], ka * sfac[nt][k & 1], lv);
-            if (edge && kbj + g + 8 * (k >> 1) >= lim[nt][k & 1]) v = -INFINITY;
-            s[nt][k] = v;
-            move |= v > mref[nt][k & 1] + (kHead + kSlack);
+          for (int pc = 0; pc < PC; ++pc) {
+            mma_f16(acc[i][nt], a, pf[pc][nt][0], pf[pc][nt][1]);
+            mma_f16(acc[i + 1][nt], e, pf[pc][nt][0], pf[pc][nt][1]);
           }
-        if (__any_sync(0xffffffffu, move)) {
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              float m = fmaxf(s[nt][k], s[nt][k + 2]);
-              m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
-              m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
-              m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-              m = fmaxf(mref[nt][k], m - kHead);
-              const float f = ex2(mref[nt][k] - m);
-              mref[nt][k] = m;
-              lsum[nt][k] *= f;
-#pragma unroll
-              for (int i = 0; i < W16; ++i) {
-                acc[i][nt][k] *= f;
-                acc[i][nt][k + 2] *= f;
-              }
-            }
-        }
-        uint32_t pf[PC][NT][2];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float p[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) p[k] = ex2(s[nt][k] - mref[nt][k & 1]);
-          lsum[nt][0] = fmaf(p[0] + p[2], iv, lsum[nt][0]);
-          lsum[nt][1] = fmaf(p[1] + p[3], iv, lsum[nt][1]);
-          if constexpr (F32) {
-            uint32_t h0, l0, h1, l1;
-            split_f16(p[0], p[1], h0, l0);
-            split_f16(p[2], p[3], h1, l1);
-            pf[0][nt][0] = transpose8x8(h0);
-            pf[0][nt][1] = transpose8x8(h1);
-            pf[PC - 1][nt][0] = transpose8x8(l0);
-            pf[PC - 1][nt][1] = transpose8x8(l1);
-          } else {
-            pf[0][nt][0] = transpose8x8(pack_f16(p[0], p[1]));
-            pf[0][nt][1] = transpose8x8(pack_f16(p[2], p[3]));
-          }
-        }
-
-        // lane group g holds channels g D/8 + ..; byte 2 i is row g of channel tile i, byte 2 i + 1 row g + 8
-#pragma unroll
-        for (int q = 0; q < VW; ++q) {
-          const uint32_t x0 = __byte_perm(vw[0][q], vw[1][q], 0x5140) ^ 0x80808080u;
-          const uint32_t x1 = __byte_perm(vw[2][q], vw[3][q], 0x5140) ^ 0x80808080u;
-          const uint32_t y0 = __byte_perm(vw[0][q], vw[1][q], 0x7362) ^ 0x80808080u;
-          const uint32_t y1 = __byte_perm(vw[2][q], vw[3][q], 0x7362) ^ 0x80808080u;
-          const uint32_t a[4] = {codes_f16<0x4140>(x0), codes_f16<0x4342>(x0), codes_f16<0x4140>(x1), codes_f16<0x4342>(x1)};
-          const uint32_t e[4] = {codes_f16<0x4140>(y0), codes_f16<0x4342>(y0), codes_f16<0x4140>(y1), codes_f16<0x4342>(y1)};
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int pc = 0; pc < PC; ++pc) {
-              mma_f16(acc[2 * q][nt], a, pf[pc][nt][0], pf[pc][nt][1]);
-              mma_f16(acc[2 * q + 1][nt], e, pf[pc][nt][0], pf[pc][nt][1]);
-            }
-        }
-        if (jn < 0) break;
-        load_v(jn);
-        j = jn;
       }
     }
+    __syncwarp();
 
     // Join the four warps.
 #pragma unroll
@@ -457,11 +511,10 @@ __global__ void __launch_bounds__(kThreads) k_cache_attn(const CacheDev c, const
           sml[(w * ROWS + r) * 2] = mref[nt][k];
           sml[(w * ROWS + r) * 2 + 1] = l;
         }
-        float* row = so + (w * ROWS + r) * OP + g * (D / 8);
+        float* row = reinterpret_cast<float*>(ring) + r * OP + 2 * g;
 #pragma unroll
-        for (int i = 0; i < W16; i += 2)
-          *reinterpret_cast<float4*>(row + 2 * i) =
-              make_float4(acc[i][nt][k], acc[i][nt][k + 2], acc[i + 1][nt][k], acc[i + 1][nt][k + 2]);
+        for (int i = 0; i < W16; ++i)
+          *reinterpret_cast<float2*>(row + 16 * i) = make_float2(acc[i][nt][k], acc[i][nt][k + 2]);
       }
     __syncthreads();
     const bool full = g0 == 0 && g1 == groups;
@@ -478,7 +531,7 @@ __global__ void __launch_bounds__(kThreads) k_cache_attn(const CacheDev c, const
       for (int k = 0; k < kWarps; ++k) {
         const float f = ex2(sml[(k * ROWS + r) * 2] - m);
         l = fmaf(f, sml[(k * ROWS + r) * 2 + 1], l);
-        const float4 v = *reinterpret_cast<const float4*>(so + (k * ROWS + r) * OP + ch);
+        const float4 v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(sm + k * Sm::kWarp) + r * OP + ch);
         o.x = fmaf(f, v.x, o.x); o.y = fmaf(f, v.y, o.y); o.z = fmaf(f, v.z, o.z); o.w = fmaf(f, v.w, o.w);
       }
       if (full) {
@@ -581,7 +634,7 @@ int64_t units_of(const CacheDev& c, const Plan& p) {
 template <int D, int NT, bool F32>
 cudaError_t run_attn(const CacheDev& c, const Plan& pl, cudaStream_t st) {
   constexpr int ROWS = 8 * NT;
-  const size_t smem = (size_t)(F32 ? 2 : 1) * NT * (D / 16) * 32 * 8 + (size_t)kWarps * ROWS * (D + 4 + 2) * 4;
+  constexpr size_t smem = Smem<D, NT, F32>::kBytes;
   cudaError_t e = cudaFuncSetAttribute(k_cache_attn<D, NT, F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return e;
   const int64_t units = units_of(c, pl);
@@ -625,7 +678,7 @@ size_t cache_attn_workspace_layout(CacheDev* c, void* ws) {
   const Plan p = plan_of(*c);
   const int64_t groups = p.list_groups ? p.list_groups : ((int64_t)c->max_blocks * c->bs + kGroup - 1) / kGroup;
   const int64_t most = units_of(*c, p) * groups;  // no use for more blocks than groups
-  const int64_t full = 148 * (p.rows == 8 ? 4 : p.rows == 16 ? 3 : 2);
+  const int64_t full = 148 * blocks_per_sm(c->d, p.rows);
   c->grid = (int)(most < full ? most : full);
   const size_t o_pre = ((size_t)(c->B + 1) * 8 + 255) / 256 * 256;
   const size_t o_ml = o_pre + ((size_t)c->grid * 2 * p.rows * 2 * 4 + 255) / 256 * 256;
