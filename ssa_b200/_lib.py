@@ -7,11 +7,13 @@ called, the call raises.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 import threading
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(PKG, "libssa_b200.so")
+TORCH_PATH = os.path.join(PKG, "_ssa_torch.so")
 
 SSA_OK, SSA_ERR_INVALID, SSA_ERR_UNSUPPORTED, SSA_ERR_WORKSPACE, SSA_ERR_CUDA, SSA_ERR_DEVICE = range(6)
 SSA_F32, SSA_BF16 = 0, 1
@@ -104,6 +106,7 @@ GRAPH_STAGES = ("hash_keys", "bucket_trim", "hash_queries", "scan_sample", "rows
                 "rows_final", "select_fma")
 
 _lib = None
+_torch_ext = None
 _lock = threading.Lock()
 
 
@@ -120,13 +123,30 @@ def load():
         if _lib is None:
             if not os.path.exists(LIB_PATH):
                 raise SSAError(f"{LIB_PATH} is missing: build it with `python -m ssa_b200.build`")
-            L = ctypes.CDLL(LIB_PATH)
+            L = ctypes.CDLL(LIB_PATH, mode=ctypes.RTLD_GLOBAL)  # _ssa_torch.so finds the C ABI in it
             for name, (res, args) in SIGNATURES.items():
                 fn = getattr(L, name)
                 fn.restype = res
                 fn.argtypes = args
             _lib = L
     return _lib
+
+
+def load_torch():
+    """The module of the block cache's operators for torch tensors
+    (_ssa_torch.so; raises if it has not been built)."""
+    global _torch_ext
+    if _torch_ext is None:
+        load()
+        with _lock:
+            if _torch_ext is None:
+                if not os.path.exists(TORCH_PATH):
+                    raise SSAError(f"{TORCH_PATH} is missing: build it with `python -m ssa_b200.build`")
+                spec = importlib.util.spec_from_file_location("_ssa_torch", TORCH_PATH)
+                m = importlib.util.module_from_spec(spec)
+                spec.loader.exec_module(m)
+                _torch_ext = m
+    return _torch_ext
 
 
 def check(rc: int, what: str):

@@ -4,7 +4,10 @@
 
 Each .cu file is compiled by nvcc for `-gencode arch=compute_100a,code=sm_100a`
 (in parallel), then linked into one shared library with the static CUDA
-runtime. The library exports only the C ABI of include/ssa_b200.h.
+runtime. The library exports only the C ABI of include/ssa_b200.h. Then
+`ssa_b200/_ssa_torch.so`, the Python module of the block cache's operators for
+torch tensors (ssa_torch.cpp), is compiled against torch's headers and linked
+to that library beside it.
 """
 from __future__ import annotations
 
@@ -13,6 +16,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 PKG = os.path.dirname(os.path.abspath(__file__))
@@ -20,6 +24,7 @@ ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 OBJ_DIR = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "libssa_b200.so")
+TORCH_LIB = os.path.join(PKG, "_ssa_torch.so")
 SOURCES = ["ssa_graph.cu", "ssa_select_tc.cu", "ssa_hash_tc.cu", "ssa_select_rows.cu", "ssa_attn.cu", "ssa_cache.cu",
            "ssa_cache_attn.cu", "ssa_capi.cu"]
 HEADERS = ["ssa_common.cuh", "ssa_internal.h", "ssa_select_common.cuh", "ssa_tcgen05.cuh",
@@ -45,6 +50,8 @@ def _stale(target: str, deps) -> bool:
 
 def build(force: bool = False, verbose: bool = False) -> str:
     os.makedirs(OBJ_DIR, exist_ok=True)
+    pool = ThreadPoolExecutor(max_workers=1)
+    ext = pool.submit(build_torch, force, verbose)  # beside the .cu files
     hdrs = [os.path.join(CSRC, h) for h in HEADERS] + [os.path.join(ROOT, "include", "ssa_b200.h")]
     jobs = []
     for src in SOURCES:
@@ -75,7 +82,32 @@ def build(force: bool = False, verbose: bool = False) -> str:
         os.replace(tmp, LIB)
         if verbose:
             print("linked", LIB)
+    ext.result()
+    pool.shutdown()
     return LIB
+
+
+def build_torch(force: bool = False, verbose: bool = False) -> str:
+    """_ssa_torch.so from ssa_torch.cpp. It resolves the C ABI at load time
+    from the libssa_b200.so that ssa_b200._lib has loaded."""
+    src = os.path.join(CSRC, "ssa_torch.cpp")
+    if not (force or _stale(TORCH_LIB, [src, os.path.join(ROOT, "include", "ssa_b200.h")])):
+        return TORCH_LIB
+    import torch
+    from torch.utils import cpp_extension as ext
+    inc = [f"-I{p}" for p in ext.include_paths() + ["/usr/local/cuda/include", sysconfig.get_paths()["include"]]]
+    lib = [f"-L{p}" for p in ext.library_paths()]
+    tmp = TORCH_LIB + f".tmp{os.getpid()}"
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-DTORCH_EXTENSION_NAME=_ssa_torch",
+           "-DTORCH_API_INCLUDE_EXTENSION_H", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *inc, src, "-o", tmp, *lib, "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for {src}:\n{r.stderr}")
+    os.replace(tmp, TORCH_LIB)
+    if verbose:
+        print("linked", TORCH_LIB)
+    return TORCH_LIB
 
 
 def main(argv=None):

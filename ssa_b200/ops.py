@@ -10,13 +10,12 @@ transpose or a GQA repeat.
 from __future__ import annotations
 
 import ctypes
-import struct
 from typing import Optional, Tuple
 
 import torch
 
 from . import _lib
-from ._lib import AttnParams, CacheParams, GraphParams, SSA_BF16, SSA_F32, check
+from ._lib import AttnParams, GraphParams, SSA_BF16, SSA_F32, check
 
 
 def _require_cuda(*ts: torch.Tensor):
@@ -420,42 +419,15 @@ def gather_attention(q, k, v, nb, valid, scale: float, fp32w: bool = False, drop
 
 # ---------------------------------------------------------------------------
 # 8-bit block cache (include/ssa_b200.h, "Block cache"; ssa_b200/cache.py
-# holds the buffers)
+# holds the buffers). Checks, allocation and launch are in csrc/ssa_torch.cpp.
 # ---------------------------------------------------------------------------
-def _cache_tensor(name, t, dtype, shape, dev):
-    """Cache buffers are read and written where they lie: their type, shape,
-    device (an index) and contiguity are checked, never mended by a copy."""
-    if t.dtype is not dtype or t.shape != shape or t.get_device() != dev or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape} on cuda:{dev}, got "
-                         f"{t.dtype} {tuple(t.shape)}{'' if t.is_contiguous() else ' (strided)'} on {t.device}")
-    return t.data_ptr()
+_torch_ext = None
 
 
-def _cache_device(t):
-    if not t.is_cuda:
-        _require_cuda(t)
-    return t.get_device()
-
-
-def _cache_call(dev, name, *args):
-    """One launch on dev's current stream, whichever device is current."""
-    fn = getattr(_lib.load(), name)
-    st = torch._C._cuda_getCurrentRawStream(dev)
-    if torch._C._cuda_getDevice() == dev:
-        rc = fn(*args, st)
-    else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, st)
-    if rc:
-        check(rc, name)
-
-
-_PACK = struct.Struct("13if12q")
-
-
-def _cache_params(*fields):
-    """CacheParams(*fields), packed at once: filling it field by field takes as long as a launch."""
-    return CacheParams.from_buffer_copy(_PACK.pack(*fields))
+def _load_torch():
+    global _torch_ext
+    _torch_ext = _lib.load_torch()
+    return _torch_ext
 
 
 def cache_reserve(lens: torch.Tensor, new_lens: torch.Tensor, table: torch.Tensor, free: torch.Tensor,
@@ -466,26 +438,7 @@ def cache_reserve(lens: torch.Tensor, new_lens: torch.Tensor, table: torch.Tenso
     before and after, and [pages left, sequences refused so far]. A sequence
     that the table or the pool cannot hold keeps its length. All int32. out:
     the three result tensors (lens and state may be the inputs themselves)."""
-    dev = _cache_device(lens)
-    if lens.dim() != 1 or table.dim() != 2 or free.dim() != 1:
-        raise ValueError("cache_reserve: lens (B,), table (B, max_blocks) and free (num_pages,) expected")
-    B, mb = lens.shape[0], table.shape[1]
-    if out is None:
-        out = torch.empty_like(lens), torch.empty_like(lens), torch.empty_like(state)
-    i32, c = torch.int32, _cache_tensor
-    start, after, st = out
-    pl, ps = c("lens", lens, i32, (B,), dev), c("state", state, i32, (2,), dev)
-    _cache_call(dev, "ssa_cache_reserve", B, mb, block_size, free.shape[0], pl,
-                c("new_lens", new_lens, i32, (B,), dev), c("table", table, i32, (B, mb), dev),
-                c("free", free, i32, (free.shape[0],), dev), ps, c("start", start, i32, (B,), dev),
-                c("lens (out)", after, i32, (B,), dev), c("state (out)", st, i32, (2,), dev))
-    return start, after, st
-
-
-def _cache_lens(table, start, lens, dev):
-    B = table.shape[0]
-    return (_cache_tensor("table", table, torch.int32, tuple(table.shape), dev),
-            _cache_tensor("start", start, torch.int32, (B,), dev), _cache_tensor("lens", lens, torch.int32, (B,), dev))
+    return (_torch_ext or _load_torch()).cache_reserve(lens, new_lens, table, free, state, block_size, out)
 
 
 def cache_append(k: torch.Tensor, v: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor, amax: torch.Tensor,
@@ -496,33 +449,8 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, k_codes: torch.Tensor, v_code
     the cache in 8 bits (ssa_cache_append). Writes k_codes, v_codes, amax,
     bounds and tail in place; with want_values returns (k, v) as the cache now
     holds them, (B, n_kv, n, d) in the input's type, 0 for padding."""
-    dev = _cache_device(k)
-    if v.get_device() != dev:
-        _require_cuda(k, v)
-    if k.dtype != v.dtype or k.shape != v.shape:
-        raise ValueError(f"k {k.dtype} {tuple(k.shape)} and v {v.dtype} {tuple(v.shape)} differ")
-    k, ksb, ksh, ksn = _rows(k)
-    v, vsb, vsh, vsn = _rows(v)
-    B, n_kv, n, d = k.shape
-    if k_codes.dim() != 4 or table.dim() != 2 or table.shape[0] != B:
-        raise ValueError(f"k_codes {tuple(k_codes.shape)} / table {tuple(table.shape)} do not match k {tuple(k.shape)}")
-    P, bs = k_codes.shape[0], k_codes.shape[2]
-    if n == 0 or B == 0:
-        return (k.clone(), v.clone()) if want_values else None
-    c, i8 = _cache_tensor, torch.int8
-    ptrs = (c("k_codes", k_codes, i8, (P, n_kv, bs, d), dev), c("v_codes", v_codes, i8, (P, n_kv, bs, d), dev),
-            c("amax", amax, torch.float32, (P, n_kv, 2), dev), c("bounds", bounds, i8, (P, n_kv, 2, d), dev),
-            c("tail", tail, k.dtype, (B, n_kv, 2, bs, d), dev), *_cache_lens(table, start, lens, dev))
-    kv = vv = None
-    os_ = (0, 0, 0)
-    if want_values:
-        kv, vv = torch.empty((2, B, n, n_kv, d), dtype=k.dtype, device=k.device).transpose(2, 3).unbind(0)
-        os_ = (n * n_kv * d, d, n_kv * d)
-    p = _cache_params(B, n_kv, n_kv, n, d, _dtype_code(k), bs, table.shape[1], P, 0, 0, 0, 0, 0.0, 0, 0, 0,
-                      ksb, ksh, ksn, vsb, vsh, vsn, *os_)
-    _cache_call(dev, "ssa_cache_append", p, k.data_ptr(), v.data_ptr(), *ptrs,
-                kv.data_ptr() if want_values else None, vv.data_ptr() if want_values else None)
-    return (kv, vv) if want_values else None
+    return (_torch_ext or _load_torch()).cache_append(k, v, k_codes, v_codes, amax, bounds, tail, table, start, lens,
+                                                      want_values)
 
 
 def cache_select(q: torch.Tensor, bounds: torch.Tensor, amax: torch.Tensor, table: torch.Tensor,
@@ -532,22 +460,7 @@ def cache_select(q: torch.Tensor, bounds: torch.Tensor, amax: torch.Tensor, tabl
     sequence that may hold the largest q.k (ssa_cache_select): (B, n, n_kv,
     top) int32 block numbers, ascending, -1 behind. The first `sink` blocks and
     the last `local` up to the token's own are always among them."""
-    dev = _cache_device(q)
-    q, qsb, qsh, qsn = _rows(q)
-    B, H, n, d = q.shape
-    if bounds.dim() != 4 or table.dim() != 2 or table.shape[0] != B:
-        raise ValueError(f"bounds {tuple(bounds.shape)} / table {tuple(table.shape)} do not match q {tuple(q.shape)}")
-    P, n_kv = bounds.shape[:2]
-    out = torch.empty((B, n, n_kv, top), dtype=torch.int32, device=q.device)
-    if n == 0 or B == 0:
-        return out
-    p = _cache_params(B, H, n_kv, n, d, _dtype_code(q), block_size, table.shape[1], P, top, sink, local, 1, 0.0,
-                      qsb, qsh, qsn, 0, 0, 0, 0, 0, 0, 0, 0, 0)
-    _cache_call(dev, "ssa_cache_select", p, q.data_ptr(),
-                _cache_tensor("bounds", bounds, torch.int8, (P, n_kv, 2, d), dev),
-                _cache_tensor("amax", amax, torch.float32, (P, n_kv, 2), dev), *_cache_lens(table, start, lens, dev),
-                out.data_ptr())
-    return out
+    return (_torch_ext or _load_torch()).cache_select(q, bounds, amax, table, start, lens, top, block_size, sink, local)
 
 
 def cache_attention(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor, amax: torch.Tensor,
@@ -560,33 +473,8 @@ def cache_attention(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tenso
     Returns out (B, H, n, d) in the (B, n, H, d) layout the output projection
     reads and, with want_lse, the fp32 log of the weights' sum (B, H, n). Rows
     without a key and padding rows are 0 and -inf. Inference only: no gradient."""
-    dev = _cache_device(q)
-    if q.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError("cache_attention has no gradient: call it under torch.no_grad()")
-    q, qsb, qsh, qsn = _rows(q)
-    B, H, n, d = q.shape
-    if k_codes.dim() != 4 or table.dim() != 2 or table.shape[0] != B:
-        raise ValueError(f"k_codes {tuple(k_codes.shape)} / table {tuple(table.shape)} do not match q {tuple(q.shape)}")
-    P, n_kv, bs = k_codes.shape[:3]
-    out = torch.empty((B, n, H, d), dtype=q.dtype, device=q.device).transpose(1, 2)
-    lse = torch.empty((B, H, n), dtype=torch.float32, device=q.device) if want_lse else None
-    if n and B:
-        top, pb = 0, None
-        if blocks is not None:
-            if blocks.dim() != 4:
-                raise ValueError(f"blocks (B, n, n_kv, top) expected, got {tuple(blocks.shape)}")
-            top = blocks.shape[3]
-            pb = _cache_tensor("blocks", blocks, torch.int32, (B, n, n_kv, top), dev)
-        p = _cache_params(B, H, n_kv, n, d, _dtype_code(q), bs, table.shape[1], P, top, 0, 0, 1 if causal else 0,
-                          scale, qsb, qsh, qsn, 0, 0, 0, 0, 0, 0, n * H * d, d, H * d)
-        ws_bytes = _lib.load().ssa_cache_attn_workspace_size(p, pb is not None)
-        ws = torch.empty(max(ws_bytes, 1), dtype=torch.uint8, device=q.device)
-        _cache_call(dev, "ssa_cache_attn", p, q.data_ptr(),
-                    _cache_tensor("k_codes", k_codes, torch.int8, (P, n_kv, bs, d), dev),
-                    _cache_tensor("v_codes", v_codes, torch.int8, (P, n_kv, bs, d), dev),
-                    _cache_tensor("amax", amax, torch.float32, (P, n_kv, 2), dev),
-                    *_cache_lens(table, start, lens, dev), pb, out.data_ptr(),
-                    lse.data_ptr() if want_lse else None, ws.data_ptr(), ws_bytes)
+    out, lse = (_torch_ext or _load_torch()).cache_attention(q, k_codes, v_codes, amax, table, start, lens, scale, blocks,
+                                                             causal, want_lse)
     return (out, lse) if want_lse else out
 
 
