@@ -16,9 +16,6 @@ namespace ssa {
 
 namespace {
 
-// ---------------------------------------------------------------- reserve
-constexpr int kReserveThreads = 1024;
-
 // Inclusive scan of v over the block; total in the last return. `part` holds
 // one int for each warp.
 __device__ __forceinline__ int block_scan(int v, int* part, int& total) {
@@ -31,70 +28,94 @@ __device__ __forceinline__ int block_scan(int v, int* part, int& total) {
   __syncthreads();
   if (lane == 31) part[w] = v;
   __syncthreads();
-  int before = 0, all = 0;
-  for (int i = 0; i < nw; ++i) {
-    const int x = part[i];
-    if (i < w) before += x;
-    all += x;
-  }
-  total = all;
-  return v + before;
+  const int x = lane < nw ? part[lane] : 0;
+  total = __reduce_add_sync(0xffffffffu, x);
+  return v + __reduce_add_sync(0xffffffffu, lane < w ? x : 0);
 }
+
+// ---------------------------------------------------------------- reserve
+constexpr int kReserveThreads = 1024;
+constexpr int kReserveCluster = 8;
 
 // A sequence's pages are taken from the top of the free stack in sequence
 // order, so the stack position of every page follows from a prefix sum of the
 // needs. A sequence whose pages no longer fit gets none, nor does a later one
-// that needs any.
+// that needs any: those served are a prefix, and the last served sum is what
+// the stack loses.
+//
+// One thread block for one step of up to 1024 sequences; a cluster of eight,
+// each with every eighth sequence's table row, where prompts open many pages:
+// writing the rows is a chain of load latencies (1024 prompts of up to 128
+// pages: 36 us in one block).
 __global__ void __launch_bounds__(kReserveThreads) k_cache_reserve(const ReserveDev r) {
   __shared__ int part[32];
   __shared__ int s_at[kReserveThreads], s_held[kReserveThreads], s_need[kReserveThreads];
-  int count = r.state[0];
+  __shared__ int s_given, s_refused;
+  const int rank = blockIdx.x, ranks = gridDim.x, threads = blockDim.x;
+  const int lane = threadIdx.x & 31;
   const int failed = r.state[1];
-  if (count > r.num_pages) count = r.num_pages;
-  if (count < 0) count = 0;
-  int64_t before = 0;
-  int given_all = 0, rejected = 0;
-  for (int b0 = 0; b0 < r.B; b0 += kReserveThreads) {
-    const int b = b0 + threadIdx.x;
-    int len = 0, more = 0;
-    if (b < r.B) {
-      len = max(r.lens[b], 0);
-      more = max(r.new_lens[b], 0);
+  const int count = max(0, min(r.state[0], r.num_pages));
+  if (threadIdx.x == 0) s_given = s_refused = 0;
+  // With several blocks the lengths are written after all of them have read
+  // theirs (lens_out may be lens): in a second pass, by the first block.
+  for (int pass = 0; pass < (ranks > 1 ? 2 : 1); ++pass) {
+    const bool rows = pass == 0, lengths = ranks == 1 || pass == 1;
+    if (pass) {
+      asm volatile("barrier.cluster.arrive;\n\tbarrier.cluster.wait;" ::: "memory");
+      if (rank) return;
     }
-    const int64_t after = (int64_t)len + more;
-    const int held = (len + r.bs - 1) / r.bs;
-    const int64_t want = (after + r.bs - 1) / r.bs;
-    const bool wide = want > r.max_blocks;
-    const int need = wide ? 0 : (int)(want - held);
-    int total;
-    const int upto = block_scan(need, part, total);
-    const bool ok = !wide && (need == 0 || before + upto <= count);
-    const int given = ok ? need : 0;
-    s_at[threadIdx.x] = count - 1 - (int)(before + upto - need);
-    s_held[threadIdx.x] = held;
-    s_need[threadIdx.x] = given;
-    if (b < r.B) {
-      r.start_out[b] = len;
-      r.lens_out[b] = ok ? (int)after : len;
+    int64_t before = 0;
+    for (int b0 = 0; b0 < r.B; b0 += threads) {
+      const int b = b0 + threadIdx.x;
+      int len = 0, more = 0;
+      if (b < r.B) {
+        len = max(r.lens[b], 0);
+        more = max(r.new_lens[b], 0);
+      }
+      const int64_t after = (int64_t)len + more;
+      const int held = (int)(((int64_t)len + r.bs - 1) / r.bs);
+      const int64_t want = (after + r.bs - 1) / r.bs;
+      const bool wide = want > r.max_blocks;
+      const int need = wide ? 0 : (int)(want - held);
+      int total;
+      const int upto = block_scan(need, part, total);
+      const bool ok = !wide && (need == 0 || before + upto <= count);
+      if (lengths) {
+        if (b < r.B) {
+          r.start_out[b] = len;
+          r.lens_out[b] = ok ? (int)after : len;
+        }
+        const int given = __reduce_max_sync(0xffffffffu, ok && need ? (int)before + upto : 0);
+        const int refused = __popc(__ballot_sync(0xffffffffu, b < r.B && !ok));
+        if (lane == 0 && given) atomicMax(&s_given, given);
+        if (lane == 0 && refused) atomicAdd(&s_refused, refused);
+      }
+      if (rows) {
+        s_at[threadIdx.x] = count - 1 - (int)(before + upto - need);
+        s_held[threadIdx.x] = held;
+        s_need[threadIdx.x] = ok ? need : 0;
+        __syncthreads();
+        const int many = min(threads, r.B - b0);
+        for (int i = (threadIdx.x >> 5) * ranks + rank; i < many; i += (threads >> 5) * ranks) {
+          const int m = s_need[i], at = s_at[i];
+          int32_t* row = r.table + (int64_t)(b0 + i) * r.max_blocks + s_held[i];
+          for (int j = lane; j < m; j += 128) {
+            int pg[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) pg[e] = j + 32 * e < m ? r.free_pages[at - j - 32 * e] : 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (j + 32 * e < m) row[j + 32 * e] = pg[e];
+          }
+        }
+      }
+      before += total;
+      __syncthreads();
     }
-    __syncthreads();
-    const int lane = threadIdx.x & 31;
-    for (int i = threadIdx.x >> 5; i < kReserveThreads && b0 + i < r.B; i += kReserveThreads / 32) {
-      const int m = s_need[i], at = s_at[i];
-      int32_t* row = r.table + (int64_t)(b0 + i) * r.max_blocks + s_held[i];
-      for (int j = lane; j < m; j += 32) row[j] = r.free_pages[at - j];
-    }
-    int sum;
-    block_scan(given, part, sum);
-    given_all += sum;
-    block_scan(b < r.B && !ok, part, sum);
-    rejected += sum;
-    before += total;
-    __syncthreads();
   }
   if (threadIdx.x == 0) {
-    r.state_out[0] = count - given_all;
-    r.state_out[1] = failed + rejected;
+    r.state_out[0] = count - s_given;
+    r.state_out[1] = failed + s_refused;
   }
 }
 
@@ -120,7 +141,7 @@ __device__ __forceinline__ uint32_t quantize4(const float4& x, float inv, float 
   float4 b = make_float4(t.x + kRound, t.y + kRound, t.z + kRound, t.w + kRound);
   r = make_float4(b.x - kRound, b.y - kRound, b.z - kRound, b.w - kRound);
   const float far = fmaxf(fmaxf(fabsf(t.x - r.x), fabsf(t.y - r.y)), fmaxf(fabsf(t.z - r.z), fabsf(t.w - r.w)));
-  if (far > 0.4999f) {
+  if (far > 0.49998f) {
     b = make_float4(quantize_exact(x.x, amax), quantize_exact(x.y, amax), quantize_exact(x.z, amax), quantize_exact(x.w, amax));
     r = make_float4(b.x - kRound, b.y - kRound, b.z - kRound, b.w - kRound);
   }
@@ -199,17 +220,17 @@ __device__ __forceinline__ void append_block(const CacheDev& c, int b, int kv, i
   const char* in = static_cast<const char*>(s ? c.v : c.k) +
                    ((s ? b * c.v_sb + kv * c.v_sh : b * c.k_sb + kv * c.k_sh) + (int64_t)(p0 - start) * sn + cv * 4) * kSize;
   char* tail = static_cast<char*>(c.tail) + (((((int64_t)b * c.n_kv + kv) * 2 + s) * BS) * D + cv * 4) * kSize;
+  const bool whole = old == 0 && end == BS;  // a complete block of new tokens: no row to leave out
   V x[kPasses];
+  if (whole) {
 #pragma unroll
-  for (int p = 0; p < kPasses; ++p) {
-    const int row = p * kRg + r0;
-    x[p].zero();
-    if (row >= old && row < end) x[p].load_nc(in + row * sn * kSize);
-  }
-  if (old) {
+    for (int p = 0; p < kPasses; ++p) x[p].load_nc(in + (p * kRg + r0) * sn * kSize);
+  } else {
 #pragma unroll
     for (int p = 0; p < kPasses; ++p) {
       const int row = p * kRg + r0;
+      x[p].zero();
+      if (row >= old && row < end) x[p].load_nc(in + row * sn * kSize);
       if (row < old) x[p].load(tail + (int64_t)row * D * kSize);
     }
   }
@@ -244,18 +265,39 @@ __device__ __forceinline__ void append_block(const CacheDev& c, int b, int kv, i
   char* values = static_cast<char*>(s ? c.v_values : c.k_values);
   const bool open = p0 + BS > len;
   if (values) values += (b * c.o_sb + kv * c.o_sh + (int64_t)(p0 - start) * c.o_sn + cv * 4) * kSize;
+  if (whole) {
+    if (values) {
+      values += r0 * c.o_sn * kSize;
+      const int64_t stride = kRg * c.o_sn * kSize;
 #pragma unroll
-  for (int p = 0; p < kPasses; ++p) {
-    const int row = p * kRg + r0;
-    const bool have = row < end;
-    float4 r;
-    const uint32_t q = quantize4(x[p].f(), inv, amax, r);
-    if (have) *reinterpret_cast<uint32_t*>(codes + row * D) = q;
-    if (values && p0 + row >= start && p0 + row - start < c.n) {
-      V o;
-      o.zero();
-      if (have) o.from(make_float4(r.x * step, r.y * step, r.z * step, r.w * step));
-      o.store(values + row * c.o_sn * kSize);
+      for (int p = 0; p < kPasses; ++p, values += stride) {
+        float4 r;
+        *reinterpret_cast<uint32_t*>(codes + (p * kRg + r0) * D) = quantize4(x[p].f(), inv, amax, r);
+        V o;
+        o.from(make_float4(r.x * step, r.y * step, r.z * step, r.w * step));
+        o.store(values);
+      }
+    } else {
+#pragma unroll
+      for (int p = 0; p < kPasses; ++p) {
+        float4 r;
+        *reinterpret_cast<uint32_t*>(codes + (p * kRg + r0) * D) = quantize4(x[p].f(), inv, amax, r);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+      const int row = p * kRg + r0;
+      const bool have = row < end;
+      float4 r;
+      const uint32_t q = quantize4(x[p].f(), inv, amax, r);
+      if (have) *reinterpret_cast<uint32_t*>(codes + row * D) = q;
+      if (values && p0 + row >= start && p0 + row - start < c.n) {
+        V o;
+        o.zero();
+        if (have) o.from(make_float4(r.x * step, r.y * step, r.z * step, r.w * step));
+        o.store(values + row * c.o_sn * kSize);
+      }
     }
   }
   if (open) {  // the open block's new tokens, as they came (zeroed above where there are no codes: read again)
@@ -292,7 +334,7 @@ __device__ __forceinline__ void append_block(const CacheDev& c, int b, int kv, i
 // the tail and the last one may write it, so one thread block does both, in
 // that order.
 template <int DT, int D, int BS>
-__global__ void __launch_bounds__(kAppendThreads<D, BS>) k_cache_append(const CacheDev c, const int nt) {
+__global__ void __launch_bounds__(kAppendThreads<D, BS>, DT == kDtF32 ? 2 : 4) k_cache_append(const CacheDev c, const int nt) {
   __shared__ float4 red[(DT == kDtF32 ? 2 : 1) * kAppendThreads<D, BS>];
   int64_t i = blockIdx.x;
   const int j = (int)(i % nt);
@@ -341,19 +383,33 @@ __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, ui
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Ordered like the double, 0 below every number.
+// Ordered like the double, above 0 and below ~0 - 1 (which no number reaches,
+// but a NaN might).
 __device__ __forceinline__ unsigned long long order_key(double v) {
   const unsigned long long u = (unsigned long long)__double_as_longlong(v + 0.0);  // -0 -> 0
-  return (u >> 63) ? ~u : u | (1ull << 63);
+  const unsigned long long k = (u >> 63) ? ~u : u | (1ull << 63);
+  return max(1ull, min(k, ~0ull - 2));
 }
 
-// One thread block per (sequence, token, kv head). The bound of a block is
-// sum_c max(q lo_c, q hi_c) = q- . lo + q+ . hi (q-, q+ the negative and
-// positive parts): a product of 8-bit rows of length 2 d, exact in the
-// tensor cores' 32-bit sums; times amax it is exact in 64 bits, so the
-// order of two blocks never depends on how the sum was formed.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+// The first block of the cluster's copy of a shared variable.
+template <typename T>
+__device__ __forceinline__ uint32_t at_rank0(const T* p) {
+  uint32_t a;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(p))));
+  return a;
+}
+
+// One cluster of thread blocks per (sequence, token, kv head). The bound of a
+// block is sum_c max(q lo_c, q hi_c) = q- . lo + q+ . hi (q-, q+ the negative
+// and positive parts): a product of 8-bit rows of length 2 d, exact in the
+// tensor cores' 32-bit sums; times amax it is exact in 64 bits, so the order
+// of two blocks never depends on how the sum was formed. The cluster's blocks
+// score equal parts into the first one's shared memory, which then narrows
+// the range of keys in which the last listed one lies, 256 bins at a time.
 template <int DT, int D>
-__global__ void __launch_bounds__(kSelThreads) k_cache_select(const CacheDev c) {
+__global__ void __launch_bounds__(kSelThreads, 2) k_cache_select(const CacheDev c) {
   extern __shared__ __align__(16) unsigned char sm[];
   const int nht = (c.rep + 7) / 8;                                   // tiles of 8 heads
   uint32_t* qf = reinterpret_cast<uint32_t*>(sm);                    // [nht][2][D / 16][32]: words of q-, q+
@@ -361,25 +417,36 @@ __global__ void __launch_bounds__(kSelThreads) k_cache_select(const CacheDev c) 
   __shared__ uint32_t red[32];
   __shared__ int hist[256];
   __shared__ int part[32];
-  __shared__ int s_bin, s_rem, s_full;
+  __shared__ unsigned long long s_lo[64], s_hi[64];  // for each warp of the cluster: range of the keys not forced
+  __shared__ int s_forced[64], s_bin, s_above, s_cnt, s_n;
+  __shared__ int s_idx[kSelThreads];
+  uint32_t rank, ranks;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t = lane & 3;
-  int64_t u = blockIdx.x;
+  const int64_t unit = blockIdx.x / ranks;
+  int64_t u = unit;
   const int kv = (int)(u % c.n_kv);
   u /= c.n_kv;
   const int tok = (int)(u % c.n), b = (int)(u / c.n);
-  int32_t* out = c.blocks_out + (int64_t)blockIdx.x * c.top;
+  int32_t* out = c.blocks_out + unit * c.top;
   int start, len;
   const int fresh = cache_step_tokens(c, b, start, len);
   const int here = tok < fresh ? (start + tok) / c.bs + 1 : 0;       // blocks that stand for election
+  const bool few = here <= c.top;
 
-  if (here > c.top) {
+  if (few) {
+    if (rank) return;
+    for (int i = tid; i < here; i += kSelThreads) keys[i] = cache_page(c, b, i) < 0 ? 0ull : ~0ull;
+    __syncthreads();
+  } else {
+    if (ranks > 1) cluster_arrive();  // waited for before the first block's memory is written
+    if (tid == 0) s_n = 0;
     // q in 8 bits, one amax for the group's heads
     const int64_t q0 = b * c.q_sb + (int64_t)kv * c.rep * c.q_sh + (int64_t)tok * c.q_sn;
     uint32_t top = 0;
-    for (int i = tid; i < c.rep * (D / 4); i += kSelThreads) {
-      const float4 x = load4<DT>(row_ptr<DT>(c.q, q0 + (int64_t)(i / (D / 4)) * c.q_sh), i % (D / 4) * 4);
-      top = max(top, abs_top(x));
-    }
+    for (int i = tid; i < c.rep * (D / 4); i += kSelThreads)
+      top = max(top, abs_top(load4<DT>(row_ptr<DT>(c.q, q0 + (int64_t)(i / (D / 4)) * c.q_sh), i % (D / 4) * 4)));
     top = __reduce_max_sync(0xffffffffu, top);
     if (lane == 0) red[w] = top;
     __syncthreads();
@@ -391,9 +458,10 @@ __global__ void __launch_bounds__(kSelThreads) k_cache_select(const CacheDev c) 
       const int head = ht * 8 + (ln >> 2);
       uint32_t neg = 0, pos = 0;
       if (head < c.rep && inv > 0.f) {
-        const float4 x = load4<DT>(row_ptr<DT>(c.q, q0 + (int64_t)head * c.q_sh), cache_word_channel<D>(wd, ln & 3));
         float4 r;
-        const uint32_t v = quantize4(x, inv, amax, r), sign = (v >> 7 & 0x01010101u) * 255u;
+        const uint32_t v = quantize4(load4<DT>(row_ptr<DT>(c.q, q0 + (int64_t)head * c.q_sh), cache_word_channel<D>(wd, ln & 3)),
+                                     inv, amax, r);
+        const uint32_t sign = (v >> 7 & 0x01010101u) * 255u;
         neg = v & sign;
         pos = v & ~sign;
       }
@@ -401,122 +469,252 @@ __global__ void __launch_bounds__(kSelThreads) k_cache_select(const CacheDev c) 
       qf[((ht * 2 + 1) * (D / 16) + wd) * 32 + ln] = pos;
     }
     __syncthreads();
+    if (ranks > 1) cluster_wait();
 
-    // 16 blocks a warp
-    for (int u16 = w; u16 * 16 < here; u16 += kSelThreads / 32) {
-      const int e0 = u16 * 16 + g, e1 = e0 + 8;
-      const int pg0 = e0 < here ? cache_page(c, b, e0) : -1, pg1 = e1 < here ? cache_page(c, b, e1) : -1;
-      uint32_t lo0[D / 16], hi0[D / 16], lo1[D / 16], hi1[D / 16];
-      const int8_t* r0 = c.bounds + ((int64_t)max(pg0, 0) * c.n_kv + kv) * 2 * D;
-      const int8_t* r1 = c.bounds + ((int64_t)max(pg1, 0) * c.n_kv + kv) * 2 * D;
-      cache_load_row<D>(r0, t, lo0);
-      cache_load_row<D>(r1, t, lo1);
-      cache_load_row<D>(r0 + D, t, hi0);
-      cache_load_row<D>(r1 + D, t, hi1);
-      const float am0 = __ldg(c.amax + ((int64_t)max(pg0, 0) * c.n_kv + kv) * 2);
-      const float am1 = __ldg(c.amax + ((int64_t)max(pg1, 0) * c.n_kv + kv) * 2);
-      int best0 = INT32_MIN, best1 = INT32_MIN;
+    // 32 blocks a warp at a time, as two tiles of 16
+    const uint32_t keys0 = at_rank0(keys);
+    unsigned long long my_lo = ~0ull, my_hi = 0;
+    int my_forced = 0;
+    const int stride = (int)ranks * (kSelThreads / 32) * 32;
+    int e0 = ((int)rank * (kSelThreads / 32) + w) * 32;
+    int page = e0 + lane < here ? cache_page(c, b, e0 + lane) : -1;
+    for (; e0 < here; e0 += stride) {
+      const float am = __ldg(c.amax + ((int64_t)max(page, 0) * c.n_kv + kv) * 2);
+      uint32_t lo[2][2][D / 16], hi[2][2][D / 16];  // [tile][row g / g + 8]
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int pg = max(__shfl_sync(0xffffffffu, page, h * 16 + e * 8 + g), 0);
+          const int8_t* p = c.bounds + ((int64_t)pg * c.n_kv + kv) * 2 * D;
+          cache_load_row<D>(p, t, lo[h][e]);
+          cache_load_row<D>(p + D, t, hi[h][e]);
+        }
+      const int now = page;
+      page = e0 + stride + lane < here ? cache_page(c, b, e0 + stride + lane) : -1;
+      int best[2][2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) best[h][0] = best[h][1] = INT32_MIN;
       for (int ht = 0; ht < nht; ++ht) {
-        int acc[4] = {0, 0, 0, 0};
+        int acc[2][4] = {};
         const uint32_t* fn = qf + (ht * 2) * (D / 16) * 32 + lane;
         const uint32_t* fp = fn + (D / 16) * 32;
 #pragma unroll
         for (int k = 0; k < D / 32; ++k) {
-          mma_s8(acc, lo0[2 * k], lo1[2 * k], lo0[2 * k + 1], lo1[2 * k + 1], fn[2 * k * 32], fn[(2 * k + 1) * 32]);
-          mma_s8(acc, hi0[2 * k], hi1[2 * k], hi0[2 * k + 1], hi1[2 * k + 1], fp[2 * k * 32], fp[(2 * k + 1) * 32]);
-        }
-        const int h = ht * 8 + 2 * t;
-        if (h < c.rep) { best0 = max(best0, acc[0]); best1 = max(best1, acc[2]); }
-        if (h + 1 < c.rep) { best0 = max(best0, acc[1]); best1 = max(best1, acc[3]); }
-      }
-      best0 = max(best0, __shfl_xor_sync(0xffffffffu, best0, 1));
-      best1 = max(best1, __shfl_xor_sync(0xffffffffu, best1, 1));
-      best0 = max(best0, __shfl_xor_sync(0xffffffffu, best0, 2));
-      best1 = max(best1, __shfl_xor_sync(0xffffffffu, best1, 2));
-      if (t == 0) {
-        if (e0 < here)
-          keys[e0] = pg0 < 0 ? 0ull : e0 < c.sink || e0 >= here - c.local ? ~0ull : order_key((double)best0 * (double)am0);
-        if (e1 < here)
-          keys[e1] = pg1 < 0 ? 0ull : e1 < c.sink || e1 >= here - c.local ? ~0ull : order_key((double)best1 * (double)am1);
-      }
-    }
-    __syncthreads();
-  } else {
-    for (int i = tid; i < here; i += kSelThreads) keys[i] = cache_page(c, b, i) < 0 ? 0ull : ~0ull;
-    __syncthreads();
-  }
-
-  // The top-th largest key, eight bits at a time from the highest.
-  unsigned long long prefix = 0, mask = 0;
-  int rem = c.top;
-  for (int shift = 56; shift >= 0 && here > c.top; shift -= 8) {
-    hist[tid] = 0;
-    __syncthreads();
-    for (int i = tid; i < here; i += kSelThreads) {
-      const unsigned long long k = keys[i];
-      if ((k & mask) == prefix) atomicAdd(&hist[(int)(k >> shift) & 255], 1);
-    }
-    __syncthreads();
-    if (w == 0) {
-      // lane l holds bins 255 - 8 l .. 248 - 8 l, so an inclusive scan counts from the top
-      int sum = 0;
+          const uint32_t n0 = fn[2 * k * 32], n1 = fn[(2 * k + 1) * 32], p0 = fp[2 * k * 32], p1 = fp[(2 * k + 1) * 32];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum += hist[255 - lane * 8 - e];
-      int upto = sum;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int x = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += x;
-      }
-      int above = upto - sum;
-      if (above < rem && upto >= rem) {
-        for (int e = 0; e < 8; ++e) {
-          const int bin = 255 - lane * 8 - e, n = hist[bin];
-          if (above + n >= rem) {
-            s_bin = bin;
-            s_rem = rem - above;
-            s_full = n == rem - above;
-            break;
+          for (int h = 0; h < 2; ++h) {
+            mma_s8(acc[h], lo[h][0][2 * k], lo[h][1][2 * k], lo[h][0][2 * k + 1], lo[h][1][2 * k + 1], n0, n1);
+            mma_s8(acc[h], hi[h][0][2 * k], hi[h][1][2 * k], hi[h][0][2 * k + 1], hi[h][1][2 * k + 1], p0, p1);
           }
-          above += n;
+        }
+        const int head = ht * 8 + 2 * t;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (head < c.rep) { best[h][0] = max(best[h][0], acc[h][0]); best[h][1] = max(best[h][1], acc[h][2]); }
+          if (head + 1 < c.rep) { best[h][0] = max(best[h][0], acc[h][1]); best[h][1] = max(best[h][1], acc[h][3]); }
         }
       }
+      // lane l takes block e0 + l: tile l / 16, row l % 16 -> the quad of row g = l % 8
+      int mine = 0;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          int v = best[h][e];
+          v = max(v, __shfl_xor_sync(0xffffffffu, v, 1));
+          v = max(v, __shfl_xor_sync(0xffffffffu, v, 2));
+          v = __shfl_sync(0xffffffffu, v, (lane & 7) * 4);
+          if (lane >> 3 == h * 2 + e) mine = v;
+        }
+      const int blk = e0 + lane;
+      if (blk < here) {
+        unsigned long long k = 0;
+        if (now >= 0) {
+          if (blk < c.sink || blk >= here - c.local) {
+            k = ~0ull;
+            ++my_forced;
+          } else {
+            k = order_key((double)mine * (double)am);
+            my_lo = min(my_lo, k);
+            my_hi = max(my_hi, k);
+          }
+        }
+        asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(keys0 + blk * 8), "l"(k) : "memory");
+      }
     }
-    __syncthreads();
-    prefix |= (unsigned long long)s_bin << shift;
-    mask |= 255ull << shift;
-    rem = s_rem;
-    if (s_full) break;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      my_lo = min(my_lo, __shfl_xor_sync(0xffffffffu, my_lo, o));
+      my_hi = max(my_hi, __shfl_xor_sync(0xffffffffu, my_hi, o));
+    }
+    my_forced = __reduce_add_sync(0xffffffffu, my_forced);
+    if (lane == 0) {
+      const int slot = (int)rank * (kSelThreads / 32) + w;
+      asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(at_rank0(&s_lo[slot])), "l"(my_lo) : "memory");
+      asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(at_rank0(&s_hi[slot])), "l"(my_hi) : "memory");
+      asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at_rank0(&s_forced[slot])), "r"(my_forced) : "memory");
+    }
+    __syncwarp();
+    if (ranks > 1) {
+      cluster_arrive();
+      cluster_wait();
+      if (rank) return;
+    } else {
+      __syncthreads();
+    }
   }
-  if (here <= c.top) { prefix = 0; mask = ~0ull; rem = 0; }  // every block with a page
 
-  // Ascending block order; among equal keys the lowest blocks.
-  int written = 0, ties = 0;
-  for (int i0 = 0; i0 < here; i0 += kSelThreads) {
-    const int i = i0 + tid;
-    const unsigned long long k = i < here ? keys[i] : 0ull;
-    const bool eq = i < here && k != 0 && (k & mask) == prefix && here > c.top;
-    int n_eq, n_take;
-    const int rank = block_scan(eq, part, n_eq) - eq + ties;
-    const bool take = i < here && k != 0 && ((k & mask) > prefix || (eq && rank < rem));
-    const int at = block_scan(take, part, n_take) - take + written;
-    if (take && at < c.top) out[at] = i;
-    ties += n_eq;
-    written += n_take;
+  // Keys from `above` up are listed, and those of ~0 (forced, or chosen below).
+  unsigned long long above = ~0ull;
+  unsigned long long tie = 0;  // a key of which only the first `rem` blocks are listed
+  int rem = 0;
+  if (!few) {
+    unsigned long long lo = ~0ull, hi = 0;
+    rem = c.top;
+    for (int i = 0; i < (int)ranks * (kSelThreads / 32); ++i) {
+      lo = min(lo, s_lo[i]);
+      hi = max(hi, s_hi[i]);
+      rem -= s_forced[i];
+    }
+    while (rem > 0 && lo <= hi) {  // lo > hi: nothing but forced blocks
+      const int bits = hi == lo ? 0 : 64 - __clzll((long long)(hi - lo));
+      const int sh = max(0, bits - 8);
+      hist[tid] = 0;
+      __syncthreads();
+      for (int i = tid; i < here; i += kSelThreads) {
+        const unsigned long long k = keys[i];
+        if (k >= lo && k <= hi) atomicAdd(&hist[(int)((k - lo) >> sh)], 1);
+      }
+      __syncthreads();
+      if (w == 0) {
+        // lane l holds bins 255 - 8 l .. 248 - 8 l, so an inclusive scan counts from the top
+        int sum = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum += hist[255 - lane * 8 - e];
+        int upto = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int x = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto += x;
+        }
+        int over = upto - sum;
+        const bool last = lane == 31 && upto < rem;  // fewer keys than places: down to the lowest bin
+        if ((over < rem && upto >= rem) || last) {
+          for (int e = 0; e < 8; ++e) {
+            const int bin = 255 - lane * 8 - e, n = hist[bin];
+            if (over + n >= rem || (last && e == 7)) {
+              s_bin = bin;
+              s_above = over;
+              s_cnt = n;
+              break;
+            }
+            over += n;
+          }
+        }
+      }
+      __syncthreads();
+      const unsigned long long from = lo + ((unsigned long long)s_bin << sh);
+      const unsigned long long upto = from + ((1ull << sh) - 1);
+      const int cnt = s_cnt;
+      rem -= s_above;
+      if (cnt <= rem) {  // the whole bin
+        above = from;
+        rem = 0;
+        break;
+      }
+      above = upto + 1;  // no key is ~0 - 1 or above but forced ones: no overflow
+      if (cnt <= kSelThreads) {
+        // rank the bin's keys against each other; a key of equal value ranks by its block
+        for (int i = tid; i < here; i += kSelThreads)
+          if (keys[i] >= from && keys[i] <= upto) s_idx[atomicAdd(&s_n, 1)] = i;
+        __syncthreads();
+        unsigned long long k = 0;
+        int place = 0, i = 0;
+        if (tid < cnt) {
+          i = s_idx[tid];
+          k = keys[i];
+          for (int j = 0; j < cnt; ++j) {
+            const int o = s_idx[j];
+            place += keys[o] > k || (keys[o] == k && o < i);
+          }
+        }
+        __syncthreads();
+        if (tid < cnt) keys[i] = place < rem ? ~0ull : 0ull;
+        __syncthreads();
+        rem = 0;
+        break;
+      }
+      if (sh == 0) {  // more equal keys than places
+        tie = from;
+        break;
+      }
+      lo = from;
+      hi = upto;
+    }
+  } else {
+    above = 1;
   }
-  for (int i = written + tid; i < c.top; i += kSelThreads) out[i] = -1;
+
+  // Ascending block order: each thread a run of blocks, one scan of the counts.
+  const int run = (here + kSelThreads - 1) / kSelThreads;
+  const int i0 = min(here, tid * run), i1 = min(here, i0 + run);
+  int ties_before = 0, total;
+  if (tie) {
+    int n = 0;
+    for (int i = i0; i < i1; ++i) n += keys[i] == tie;
+    ties_before = block_scan(n, part, total) - n;
+  }
+  int n = 0, seen = ties_before;
+  for (int i = i0; i < i1; ++i) {
+    const unsigned long long k = keys[i];
+    n += k >= above || (tie && k == tie && seen++ < rem);
+  }
+  int at = block_scan(n, part, total) - n;
+  seen = ties_before;
+  for (int i = i0; i < i1; ++i) {
+    const unsigned long long k = keys[i];
+    if (k >= above || (tie && k == tie && seen++ < rem)) {
+      if (at < c.top) out[at] = i;
+      ++at;
+    }
+  }
+  for (int i = total + tid; i < c.top; i += kSelThreads) out[i] = -1;
+}
+
+// Blocks of a cluster: enough of them to fill the GPU twice, none with less
+// than one round of its eight warps (256 blocks) to score.
+int select_ranks(const CacheDev& c) {
+  const int64_t units = (int64_t)c.B * c.n * c.n_kv;
+  int ranks = 1;
+  while (ranks < 8 && units * ranks < 2 * 148 && c.max_blocks > ranks * kSelThreads) ranks *= 2;
+  return ranks;
 }
 
 template <int DT, int D>
 cudaError_t run_select(const CacheDev& c, cudaStream_t st) {
-  const int64_t grid = (int64_t)c.B * c.n * c.n_kv;
+  const int ranks = select_ranks(c);
+  const int64_t grid = (int64_t)c.B * c.n * c.n_kv * ranks;
   if (grid > 0x7fffffff) return cudaErrorInvalidConfiguration;
   const size_t smem = cache_select_smem(c);
-  cudaError_t e = cudaFuncSetAttribute(k_cache_select<DT, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e != cudaSuccess) return e;
-  k_cache_select<DT, D><<<(unsigned)grid, kSelThreads, smem, st>>>(c);
+  if (smem > 40 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(k_cache_select<DT, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(kSelThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = ranks;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, k_cache_select<DT, D>, c);
   note_launch();
-  return cudaGetLastError();
+  return e;
 }
 
 template <int DT>
@@ -528,9 +726,20 @@ cudaError_t run_select_d(const CacheDev& c, cudaStream_t st) {
 }  // namespace
 
 cudaError_t launch_cache_reserve(const ReserveDev& r, cudaStream_t st) {
-  k_cache_reserve<<<1, kReserveThreads, 0, st>>>(r);
+  const bool many = r.B > 64;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(many ? kReserveCluster : 1);
+  cfg.blockDim = dim3(many ? kReserveThreads : 256);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = cfg.gridDim.x;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, k_cache_reserve, r);
   note_launch();
-  return cudaGetLastError();
+  return e;
 }
 
 cudaError_t launch_cache_append(const CacheDev& c, cudaStream_t st) {
