@@ -125,14 +125,23 @@ __global__ void __launch_bounds__(kReserveThreads) k_cache_reserve(const Reserve
 constexpr float kTinyAmax = 0x1p-80f;
 
 // rint(127 x / amax), ties to even, as in exact arithmetic. inv = 127 / amax
-// and the product are each within 2^-24 of their values, so t is within 2e-5
-// of the quotient; only where that could decide the rounding is the quotient
-// formed in 64 bits (127 x is exact there, and a quotient that is not a tie
-// is further than 2^-53 from one).
+// and the product t are each within 2^-24 of their values, so t is within 2e-5
+// of the quotient, and only within that of a half h can the rounding be in
+// doubt. Ties are common (a bf16 amax that is a power of two makes every
+// eighth code one), so they are decided in fp32: the sign of 127 x - h amax,
+// both scaled by 2^-8 -- the product in two parts, the multiply-add with one
+// rounding; next to a half the difference has few bits left and is exact.
 constexpr float kRound = 12582912.f;  // 1.5 2^23: t + kRound is rounded to a whole number, its low byte the code
+constexpr float kNearHalf = 0.49998f;
 
-__device__ __noinline__ float quantize_exact(float x, float amax) {
-  return kRound + (float)rint((double)x * 127.0 / (double)amax);
+// kRound + the code, for t next to the half beside r.
+__device__ __forceinline__ float quantize_near_half(float x, float t, float r, float amax) {
+  const float f = t - r;
+  if (!(fabsf(f) > kNearHalf)) return r + kRound;
+  const float h = r + copysignf(0.5f, f);
+  const float p = x * (127.f / 256.f), p2 = fmaf(x, 127.f / 256.f, -p);
+  const float d = fmaf(-h * (1.f / 256.f), amax, p) + p2;
+  return (d > 0.f ? h + 0.5f : d < 0.f ? h - 0.5f : h) + kRound;
 }
 
 // Four codes of x as bytes; r: the codes as floats. inv = 0: all zero.
@@ -141,8 +150,9 @@ __device__ __forceinline__ uint32_t quantize4(const float4& x, float inv, float 
   float4 b = make_float4(t.x + kRound, t.y + kRound, t.z + kRound, t.w + kRound);
   r = make_float4(b.x - kRound, b.y - kRound, b.z - kRound, b.w - kRound);
   const float far = fmaxf(fmaxf(fabsf(t.x - r.x), fabsf(t.y - r.y)), fmaxf(fabsf(t.z - r.z), fabsf(t.w - r.w)));
-  if (far > 0.49998f) {
-    b = make_float4(quantize_exact(x.x, amax), quantize_exact(x.y, amax), quantize_exact(x.z, amax), quantize_exact(x.w, amax));
+  if (far > kNearHalf) {
+    b = make_float4(quantize_near_half(x.x, t.x, r.x, amax), quantize_near_half(x.y, t.y, r.y, amax),
+                    quantize_near_half(x.z, t.z, r.z, amax), quantize_near_half(x.w, t.w, r.w, amax));
     r = make_float4(b.x - kRound, b.y - kRound, b.z - kRound, b.w - kRound);
   }
   const uint32_t lo = __byte_perm(__float_as_uint(b.x), __float_as_uint(b.y), 0x0040);
@@ -374,7 +384,20 @@ cudaError_t run_append_d(const CacheDev& c, cudaStream_t st) {
 }
 
 // ---------------------------------------------------------------- select
-constexpr int kSelThreads = 256;
+constexpr int kSelThreads = 256, kSelWarps = kSelThreads / 32;
+constexpr int kSelStages = 3;  // 16 blocks' bounds each, for every warp
+
+// Shared memory of k_cache_select: rings, what comes with a stage, the query
+// operand, keys.
+template <int D>
+struct SelSmem {
+  static constexpr int kTile = 16 * kPitch<D>, kRing = kSelStages * 2 * kTile;
+  static constexpr int kMeta = kSelWarps * kRing;                 // [kSelWarps][kSelStages][16] amax
+  static constexpr int kQ = kMeta + kSelWarps * kSelStages * 64;  // [tiles of 8 heads][2][D / 16][32] words of q-, q+
+  static size_t bytes(const CacheDev& c) {
+    return kQ + (size_t)((c.rep + 7) / 8) * 2 * (D / 16) * 32 * 4 + (size_t)c.max_blocks * 8;
+  }
+};
 
 __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                        uint32_t b1) {
@@ -410,9 +433,10 @@ __device__ __forceinline__ uint32_t at_rank0(const T* p) {
 // the range of keys in which the last listed one lies, 256 bins at a time.
 template <int DT, int D>
 __global__ void __launch_bounds__(kSelThreads, 2) k_cache_select(const CacheDev c) {
-  extern __shared__ __align__(16) unsigned char sm[];
-  const int nht = (c.rep + 7) / 8;                                   // tiles of 8 heads
-  uint32_t* qf = reinterpret_cast<uint32_t*>(sm);                    // [nht][2][D / 16][32]: words of q-, q+
+  using Sm = SelSmem<D>;
+  extern __shared__ __align__(128) unsigned char sm[];
+  const int nht = (c.rep + 7) / 8;  // tiles of 8 heads
+  uint32_t* qf = reinterpret_cast<uint32_t*>(sm + Sm::kQ);
   unsigned long long* keys = reinterpret_cast<unsigned long long*>(qf + nht * 2 * (D / 16) * 32);
   __shared__ uint32_t red[32];
   __shared__ int hist[256];
@@ -423,7 +447,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) k_cache_select(const CacheDev 
   uint32_t rank, ranks;
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
-  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t = lane & 3;
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, t = lane & 3;
   const int64_t unit = blockIdx.x / ranks;
   int64_t u = unit;
   const int kv = (int)(u % c.n_kv);
@@ -442,6 +466,42 @@ __global__ void __launch_bounds__(kSelThreads, 2) k_cache_select(const CacheDev 
   } else {
     if (ranks > 1) cluster_arrive();  // waited for before the first block's memory is written
     if (tid == 0) s_n = 0;
+
+    // Tile i (blocks 16 i .. 16 i + 15) is warp i mod nw's. Lanes 0-15 hold the
+    // pages of its next tile, lanes 16-31 those of the one after.
+    const int nw = (int)ranks * kSelWarps, tiles = (here + 15) / 16;
+    const uint32_t ring_a = smem_addr(sm) + w * Sm::kRing, meta_a = smem_addr(sm + Sm::kMeta) + w * kSelStages * 64;
+    const auto look_up = [&](int tile) {
+      const int e = (tile + (lane >> 4) * nw) * 16 + (lane & 15);
+      return e < here ? cache_page(c, b, e) : -1;
+    };
+    const int first = (int)rank * kSelWarps + w;
+    int pages = look_up(first), pages_n = look_up(first + 2 * nw);
+    int sent = 0;
+    const auto issue = [&]() {
+      const int tile = first + sent * nw;
+      if (tile < tiles) {
+        const int st = sent % kSelStages, half = (sent & 1) * 16;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {  // 16 rows of 2 D / 16 chunks, a row's chunks side by side
+          const int id = i * 32 + lane, row = id / (D / 8), ch = id % (D / 8);
+          const int pg = max(__shfl_sync(0xffffffffu, pages, half + row), 0);
+          copy16(ring_a + st * 2 * Sm::kTile + (ch >= D / 16) * Sm::kTile + tile_at<D>(row, ch % (D / 16)),
+                 c.bounds + ((int64_t)pg * c.n_kv + kv) * 2 * D + ch * 16);
+        }
+        const int mine = max(__shfl_sync(0xffffffffu, pages, half + (lane & 15)), 0);
+        if (lane < 16) copy4(meta_a + st * 64 + lane * 4, c.amax + ((int64_t)mine * c.n_kv + kv) * 2);
+        ++sent;
+        if (!(sent & 1)) {
+          pages = pages_n;
+          pages_n = look_up(first + (sent + 2) * nw);
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int i = 0; i < kSelStages - 1; ++i) issue();
+
     // q in 8 bits, one amax for the group's heads
     const int64_t q0 = b * c.q_sb + (int64_t)kv * c.rep * c.q_sh + (int64_t)tok * c.q_sn;
     uint32_t top = 0;
@@ -450,7 +510,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) k_cache_select(const CacheDev 
     top = __reduce_max_sync(0xffffffffu, top);
     if (lane == 0) red[w] = top;
     __syncthreads();
-    for (int i = 0; i < kSelThreads / 32; ++i) top = max(top, red[i]);
+    for (int i = 0; i < kSelWarps; ++i) top = max(top, red[i]);
     const float amax = __uint_as_float(top);
     const float inv = amax >= kTinyAmax && amax < INFINITY ? __fdiv_rn(127.f, amax) : 0.f;
     for (int i = tid; i < nht * (D / 16) * 32; i += kSelThreads) {
@@ -459,8 +519,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) k_cache_select(const CacheDev 
       uint32_t neg = 0, pos = 0;
       if (head < c.rep && inv > 0.f) {
         float4 r;
-        const uint32_t v = quantize4(load4<DT>(row_ptr<DT>(c.q, q0 + (int64_t)head * c.q_sh), cache_word_channel<D>(wd, ln & 3)),
-                                     inv, amax, r);
+        const uint32_t v = quantize4(load4<DT>(row_ptr<DT>(c.q, q0 + (int64_t)head * c.q_sh), wd * 16 + (ln & 3) * 4), inv, amax, r);
         const uint32_t sign = (v >> 7 & 0x01010101u) * 255u;
         neg = v & sign;
         pos = v & ~sign;
@@ -471,71 +530,55 @@ __global__ void __launch_bounds__(kSelThreads, 2) k_cache_select(const CacheDev 
     __syncthreads();
     if (ranks > 1) cluster_wait();
 
-    // 32 blocks a warp at a time, as two tiles of 16
     const uint32_t keys0 = at_rank0(keys);
     unsigned long long my_lo = ~0ull, my_hi = 0;
     int my_forced = 0;
-    const int stride = (int)ranks * (kSelThreads / 32) * 32;
-    int e0 = ((int)rank * (kSelThreads / 32) + w) * 32;
-    int page = e0 + lane < here ? cache_page(c, b, e0 + lane) : -1;
-    for (; e0 < here; e0 += stride) {
-      const float am = __ldg(c.amax + ((int64_t)max(page, 0) * c.n_kv + kv) * 2);
-      uint32_t lo[2][2][D / 16], hi[2][2][D / 16];  // [tile][row g / g + 8]
+    int done = 0;
+    while (true) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kSelStages - 2) : "memory");
+      __syncwarp();  // the oldest stage is there for the whole warp, and the one before it free
+      issue();
+      if (done == sent) break;
+      const int st = done % kSelStages, e0 = (first + done * nw) * 16;
+      ++done;
+      const uint32_t at = ring_a + st * 2 * Sm::kTile;
+      const int mrow = lane & 15, mchunk = lane >> 4;
+      uint32_t x[2][D / 32][4];  // lo, hi: the A operand of every 32 channels
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int pg = max(__shfl_sync(0xffffffffu, page, h * 16 + e * 8 + g), 0);
-          const int8_t* p = c.bounds + ((int64_t)pg * c.n_kv + kv) * 2 * D;
-          cache_load_row<D>(p, t, lo[h][e]);
-          cache_load_row<D>(p + D, t, hi[h][e]);
-        }
-      const int now = page;
-      page = e0 + stride + lane < here ? cache_page(c, b, e0 + stride + lane) : -1;
-      int best[2][2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) best[h][0] = best[h][1] = INT32_MIN;
+      for (int k = 0; k < D / 32; ++k) {
+        ldmatrix4(x[0][k], at + tile_at<D>(mrow, 2 * k + mchunk));
+        ldmatrix4(x[1][k], at + Sm::kTile + tile_at<D>(mrow, 2 * k + mchunk));
+      }
+      int best0 = INT32_MIN, best1 = INT32_MIN;
       for (int ht = 0; ht < nht; ++ht) {
         int acc[2][4] = {};
-        const uint32_t* fn = qf + (ht * 2) * (D / 16) * 32 + lane;
-        const uint32_t* fp = fn + (D / 16) * 32;
+        const uint32_t* f = qf + (ht * 2) * (D / 16) * 32 + lane;
 #pragma unroll
-        for (int k = 0; k < D / 32; ++k) {
-          const uint32_t n0 = fn[2 * k * 32], n1 = fn[(2 * k + 1) * 32], p0 = fp[2 * k * 32], p1 = fp[(2 * k + 1) * 32];
+        for (int k = 0; k < D / 32; ++k)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            mma_s8(acc[h], lo[h][0][2 * k], lo[h][1][2 * k], lo[h][0][2 * k + 1], lo[h][1][2 * k + 1], n0, n1);
-            mma_s8(acc[h], hi[h][0][2 * k], hi[h][1][2 * k], hi[h][0][2 * k + 1], hi[h][1][2 * k + 1], p0, p1);
-          }
-        }
+          for (int h = 0; h < 2; ++h)
+            mma_s8(acc[h], x[h][k][0], x[h][k][1], x[h][k][2], x[h][k][3], f[(h * (D / 16) + 2 * k) * 32],
+                   f[(h * (D / 16) + 2 * k + 1) * 32]);
         const int head = ht * 8 + 2 * t;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (head < c.rep) { best[h][0] = max(best[h][0], acc[h][0]); best[h][1] = max(best[h][1], acc[h][2]); }
-          if (head + 1 < c.rep) { best[h][0] = max(best[h][0], acc[h][1]); best[h][1] = max(best[h][1], acc[h][3]); }
-        }
+        if (head < c.rep) { best0 = max(best0, acc[0][0] + acc[1][0]); best1 = max(best1, acc[0][2] + acc[1][2]); }
+        if (head + 1 < c.rep) { best0 = max(best0, acc[0][1] + acc[1][1]); best1 = max(best1, acc[0][3] + acc[1][3]); }
       }
-      // lane l takes block e0 + l: tile l / 16, row l % 16 -> the quad of row g = l % 8
-      int mine = 0;
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          int v = best[h][e];
-          v = max(v, __shfl_xor_sync(0xffffffffu, v, 1));
-          v = max(v, __shfl_xor_sync(0xffffffffu, v, 2));
-          v = __shfl_sync(0xffffffffu, v, (lane & 7) * 4);
-          if (lane >> 3 == h * 2 + e) mine = v;
-        }
+      best0 = max(best0, __shfl_xor_sync(0xffffffffu, best0, 1));
+      best1 = max(best1, __shfl_xor_sync(0xffffffffu, best1, 1));
+      best0 = max(best0, __shfl_xor_sync(0xffffffffu, best0, 2));
+      best1 = max(best1, __shfl_xor_sync(0xffffffffu, best1, 2));
+      // lane l < 16 takes block e0 + l, whose row is the quad g = l % 8's
+      const int v0 = __shfl_sync(0xffffffffu, best0, (lane & 7) * 4), v1 = __shfl_sync(0xffffffffu, best1, (lane & 7) * 4);
       const int blk = e0 + lane;
-      if (blk < here) {
+      if (lane < 16 && blk < here) {
         unsigned long long k = 0;
-        if (now >= 0) {
+        if (cache_page(c, b, blk) >= 0) {
           if (blk < c.sink || blk >= here - c.local) {
             k = ~0ull;
             ++my_forced;
           } else {
-            k = order_key((double)mine * (double)am);
+            const float am = *reinterpret_cast<const float*>(sm + Sm::kMeta + (w * kSelStages + st) * 64 + lane * 4);
+            k = order_key((double)(lane < 8 ? v0 : v1) * (double)am);
             my_lo = min(my_lo, k);
             my_hi = max(my_hi, k);
           }
@@ -543,6 +586,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) k_cache_select(const CacheDev 
         asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(keys0 + blk * 8), "l"(k) : "memory");
       }
     }
+    __syncwarp();
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
       my_lo = min(my_lo, __shfl_xor_sync(0xffffffffu, my_lo, o));
@@ -550,7 +594,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) k_cache_select(const CacheDev 
     }
     my_forced = __reduce_add_sync(0xffffffffu, my_forced);
     if (lane == 0) {
-      const int slot = (int)rank * (kSelThreads / 32) + w;
+      const int slot = (int)rank * kSelWarps + w;
       asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(at_rank0(&s_lo[slot])), "l"(my_lo) : "memory");
       asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(at_rank0(&s_hi[slot])), "l"(my_hi) : "memory");
       asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at_rank0(&s_forced[slot])), "r"(my_forced) : "memory");
@@ -572,7 +616,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) k_cache_select(const CacheDev 
   if (!few) {
     unsigned long long lo = ~0ull, hi = 0;
     rem = c.top;
-    for (int i = 0; i < (int)ranks * (kSelThreads / 32); ++i) {
+    for (int i = 0; i < (int)ranks * kSelWarps; ++i) {
       lo = min(lo, s_lo[i]);
       hi = max(hi, s_hi[i]);
       rem -= s_forced[i];
@@ -682,12 +726,12 @@ __global__ void __launch_bounds__(kSelThreads, 2) k_cache_select(const CacheDev 
   for (int i = total + tid; i < c.top; i += kSelThreads) out[i] = -1;
 }
 
-// Blocks of a cluster: enough of them to fill the GPU twice, none with less
-// than one round of its eight warps (256 blocks) to score.
+// Blocks of a cluster: one where the units alone give every SM one, else as
+// many as give two, with a round of the warps (128 blocks of tokens) for each.
 int select_ranks(const CacheDev& c) {
   const int64_t units = (int64_t)c.B * c.n * c.n_kv;
   int ranks = 1;
-  while (ranks < 8 && units * ranks < 2 * 148 && c.max_blocks > ranks * kSelThreads) ranks *= 2;
+  while (ranks < 8 && units * ranks < 148 && c.max_blocks > ranks * kSelWarps * 16) ranks *= 2;
   return ranks;
 }
 
@@ -696,7 +740,7 @@ cudaError_t run_select(const CacheDev& c, cudaStream_t st) {
   const int ranks = select_ranks(c);
   const int64_t grid = (int64_t)c.B * c.n * c.n_kv * ranks;
   if (grid > 0x7fffffff) return cudaErrorInvalidConfiguration;
-  const size_t smem = cache_select_smem(c);
+  const size_t smem = SelSmem<D>::bytes(c);
   if (smem > 40 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(k_cache_select<DT, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
@@ -747,7 +791,8 @@ cudaError_t launch_cache_append(const CacheDev& c, cudaStream_t st) {
 }
 
 size_t cache_select_smem(const CacheDev& c) {
-  return (size_t)((c.rep + 7) / 8) * 2 * (c.d / 16) * 32 * 4 + (size_t)c.max_blocks * 8;
+  return c.d == 32 ? SelSmem<32>::bytes(c) : c.d == 64 ? SelSmem<64>::bytes(c)
+         : c.d == 96 ? SelSmem<96>::bytes(c) : SelSmem<128>::bytes(c);
 }
 
 cudaError_t launch_cache_select(const CacheDev& c, cudaStream_t st) {

@@ -26,29 +26,34 @@ __device__ __forceinline__ int cache_page(const CacheDev& c, int b, int blk) {
   return (unsigned)page < (unsigned)c.num_pages ? page : -1;
 }
 
-// The code bytes of one key row that lane t (0..3) of a quad holds, as words
-// of four channels: with D = 64 a + r, word w of the first 4a covers channels
-// (w / 4) * 64 + 16 t + 4 (w % 4) .. + 3 (one 16-byte load for each 64
-// channels), the last two (r = 32) channels 64 a + 8 t + 4 (w - 4a) .. + 3.
-// The four lanes of a quad read whole 32-byte sectors, and the other operand
-// of the product only has to list its channels in the same order.
+// A staged tile: 16 key rows of D code bytes, as 16-byte chunks exchanged
+// within 128 bytes so that the eight rows of an 8x8 tile lie in eight banks
+// of 16 bytes (rows of 96 bytes are spaced as rows of 128).
 template <int D>
-__device__ __forceinline__ int cache_word_channel(int w, int t) {
-  constexpr int kFull = D / 64 * 4;
-  return w < kFull ? (w >> 2) * 64 + t * 16 + (w & 3) * 4 : D / 64 * 64 + t * 8 + (w - kFull) * 4;
+constexpr int kPitch = D == 96 ? 128 : D;
+template <int D>
+__device__ __forceinline__ int tile_at(int row, int chunk) {
+  constexpr int kRows = 128 / kPitch<D>;  // rows in 128 bytes
+  return row * kPitch<D> + ((chunk ^ (row / kRows & (kPitch<D> / 16 - 1))) << 4);
 }
 
-template <int D>
-__device__ __forceinline__ void cache_load_row(const int8_t* row, int t, uint32_t (&w)[D / 16]) {
-#pragma unroll
-  for (int i = 0; i < D / 64; ++i) {
-    const uint4 u = __ldg(reinterpret_cast<const uint4*>(row + i * 64 + t * 16));
-    w[4 * i] = u.x; w[4 * i + 1] = u.y; w[4 * i + 2] = u.z; w[4 * i + 3] = u.w;
-  }
-  if constexpr (D % 64 != 0) {
-    const uint2 u = __ldg(reinterpret_cast<const uint2*>(row + D / 64 * 64 + t * 8));
-    w[D / 16 - 2] = u.x; w[D / 16 - 1] = u.y;
-  }
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy8(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 
 }  // namespace ssa

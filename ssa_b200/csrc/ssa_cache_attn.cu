@@ -73,33 +73,6 @@ __device__ __forceinline__ void split_f16(float a, float b, uint32_t& hi, uint32
   lo = pack_f16(a - f.x, b - f.y);
 }
 
-// A staged tile: 16 key rows of D code bytes, as 16-byte chunks exchanged
-// within 128 bytes so that the eight rows of an 8x8 tile lie in eight banks
-// of 16 bytes (rows of 96 bytes are spaced as rows of 128).
-template <int D>
-constexpr int kPitch = D == 96 ? 128 : D;
-template <int D>
-__device__ __forceinline__ int tile_at(int row, int chunk) {
-  constexpr int kRows = 128 / kPitch<D>;  // rows in 128 bytes
-  return row * kPitch<D> + ((chunk ^ (row / kRows & (kPitch<D> / 16 - 1))) << 4);
-}
-
-__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void copy8(uint32_t dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
-
 // Shared memory of a block: for each warp a ring of staged tiles (keys and
 // values of 16 keys a stage), used for the warp's partial output afterwards;
 // what comes with each stage; the query operand.
