@@ -124,19 +124,19 @@ __global__ void __launch_bounds__(kReserveThreads) k_cache_reserve(const Reserve
 // step stay far inside the fp32 range.
 constexpr float kTinyAmax = 0x1p-80f;
 
-// rint(127 x / amax), ties to even, as in exact arithmetic. inv = 127 / amax
-// and the product t are each within 2^-24 of their values, so t is within 2e-5
-// of the quotient, and only within that of a half h can the rounding be in
-// doubt. Ties are common (a bf16 amax that is a power of two makes every
-// eighth code one), so they are decided in fp32: the sign of 127 x - h amax,
-// both scaled by 2^-8 -- the product in two parts, the multiply-add with one
-// rounding; next to a half the difference has few bits left and is exact.
-constexpr float kRound = 12582912.f;  // 1.5 2^23: t + kRound is rounded to a whole number, its low byte the code
+// rint(127 x / amax), ties to even, as in exact arithmetic. inv = 127 / amax is
+// within 2^-24 of its value and the multiply-adds round once, so x inv is
+// within 1e-5 of the quotient; only within that of a half h can the rounding
+// be in doubt. Ties are common (a bf16 amax that is a power of two makes every
+// eighth code one), so they are decided in fp32 too: by the sign of
+// 127 x - h amax, both scaled by 2^-8 -- the product in two parts, the
+// multiply-add with one rounding; next to a half the difference has few bits
+// left and is exact.
+constexpr float kRound = 12582912.f;  // 1.5 2^23: x + kRound is rounded to a whole number, its low byte the code
 constexpr float kNearHalf = 0.49998f;
 
-// kRound + the code, for t next to the half beside r.
-__device__ __forceinline__ float quantize_near_half(float x, float t, float r, float amax) {
-  const float f = t - r;
+// kRound + the code, where x inv = r + f.
+__device__ __forceinline__ float quantize_near_half(float x, float r, float f, float amax) {
   if (!(fabsf(f) > kNearHalf)) return r + kRound;
   const float h = r + copysignf(0.5f, f);
   const float p = x * (127.f / 256.f), p2 = fmaf(x, 127.f / 256.f, -p);
@@ -144,20 +144,52 @@ __device__ __forceinline__ float quantize_near_half(float x, float t, float r, f
   return (d > 0.f ? h + 0.5f : d < 0.f ? h - 0.5f : h) + kRound;
 }
 
-// Four codes of x as bytes; r: the codes as floats. inv = 0: all zero.
-__device__ __forceinline__ uint32_t quantize4(const float4& x, float inv, float amax, float4& r) {
-  const float4 t = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
-  float4 b = make_float4(t.x + kRound, t.y + kRound, t.z + kRound, t.w + kRound);
-  r = make_float4(b.x - kRound, b.y - kRound, b.z - kRound, b.w - kRound);
-  const float far = fmaxf(fmaxf(fabsf(t.x - r.x), fabsf(t.y - r.y)), fmaxf(fabsf(t.z - r.z), fabsf(t.w - r.w)));
-  if (far > kNearHalf) {
-    b = make_float4(quantize_near_half(x.x, t.x, r.x, amax), quantize_near_half(x.y, t.y, r.y, amax),
-                    quantize_near_half(x.z, t.z, r.z, amax), quantize_near_half(x.w, t.w, r.w, amax));
-    r = make_float4(b.x - kRound, b.y - kRound, b.z - kRound, b.w - kRound);
+__device__ __forceinline__ unsigned long long f2_add(unsigned long long a, unsigned long long b) {
+  unsigned long long d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ unsigned long long f2_mul(unsigned long long a, unsigned long long b) {
+  unsigned long long d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+// Four codes of x as bytes; r: the codes as floats, in pairs. inv = 0: all zero.
+__device__ __forceinline__ uint32_t quantize4(const float4& x, float inv, float amax, unsigned long long (&r)[2]) {
+  const unsigned long long i2 = f2_pack(inv, inv), up = f2_pack(kRound, kRound), down = f2_pack(-kRound, -kRound);
+  const unsigned long long neg = 0x8000000080000000ull;
+  const unsigned long long x0 = f2_pack(x.x, x.y), x1 = f2_pack(x.z, x.w);
+  unsigned long long b0 = f2_fma(x0, i2, up), b1 = f2_fma(x1, i2, up);
+  r[0] = f2_add(b0, down);
+  r[1] = f2_add(b1, down);
+  float fx, fy, fz, fw;
+  f2_unpack(f2_fma(x0, i2, r[0] ^ neg), fx, fy);
+  f2_unpack(f2_fma(x1, i2, r[1] ^ neg), fz, fw);
+  if (fmaxf(fmaxf(fabsf(fx), fabsf(fy)), fmaxf(fabsf(fz), fabsf(fw))) > kNearHalf) {
+    float rx, ry, rz, rw;
+    f2_unpack(r[0], rx, ry);
+    f2_unpack(r[1], rz, rw);
+    b0 = f2_pack(quantize_near_half(x.x, rx, fx, amax), quantize_near_half(x.y, ry, fy, amax));
+    b1 = f2_pack(quantize_near_half(x.z, rz, fz, amax), quantize_near_half(x.w, rw, fw, amax));
+    r[0] = f2_add(b0, down);
+    r[1] = f2_add(b1, down);
   }
-  const uint32_t lo = __byte_perm(__float_as_uint(b.x), __float_as_uint(b.y), 0x0040);
-  const uint32_t hi = __byte_perm(__float_as_uint(b.z), __float_as_uint(b.w), 0x0040);
+  float bx, by, bz, bw;
+  f2_unpack(b0, bx, by);
+  f2_unpack(b1, bz, bw);
+  const uint32_t lo = __byte_perm(__float_as_uint(bx), __float_as_uint(by), 0x0040);
+  const uint32_t hi = __byte_perm(__float_as_uint(bz), __float_as_uint(bw), 0x0040);
   return __byte_perm(lo, hi, 0x5410);
+}
+
+// What the codes stand for.
+__device__ __forceinline__ float4 scaled(const unsigned long long (&r)[2], float step) {
+  const unsigned long long s2 = f2_pack(step, step);
+  float4 v;
+  f2_unpack(f2_mul(r[0], s2), v.x, v.y);
+  f2_unpack(f2_mul(r[1], s2), v.z, v.w);
+  return v;
 }
 
 // Four consecutive elements as they lie in memory, and packed minima and
@@ -226,6 +258,20 @@ __device__ __forceinline__ void append_block(const CacheDev& c, int b, int kv, i
   const int page = p0 < len ? cache_page(c, b, blk) : -1;  // a block of padding is only cleared in the values
   // rows of the block: [0, old) from the tail, [old, end) from the input, the rest absent
   const int old = page < 0 ? 0 : max(0, min(BS, start - p0)), end = page < 0 ? 0 : min(BS, len - p0);
+  char* values = static_cast<char*>(s ? c.v_values : c.k_values);
+  if (values) values += (b * c.o_sb + kv * c.o_sh + (int64_t)(p0 - start) * c.o_sn + cv * 4) * kSize;
+  if (end == 0) {
+    if (values) {
+      V o;
+      o.zero();
+#pragma unroll
+      for (int p = 0; p < kPasses; ++p) {
+        const int row = p * kRg + r0;
+        if (p0 + row >= start && p0 + row - start < c.n) o.store(values + row * c.o_sn * kSize);
+      }
+    }
+    return;
+  }
   const int64_t sn = s ? c.v_sn : c.k_sn;
   const char* in = static_cast<const char*>(s ? c.v : c.k) +
                    ((s ? b * c.v_sb + kv * c.v_sh : b * c.k_sb + kv * c.k_sh) + (int64_t)(p0 - start) * sn + cv * 4) * kSize;
@@ -233,8 +279,10 @@ __device__ __forceinline__ void append_block(const CacheDev& c, int b, int kv, i
   const bool whole = old == 0 && end == BS;  // a complete block of new tokens: no row to leave out
   V x[kPasses];
   if (whole) {
+    const char* row = in + r0 * sn * kSize;
+    const int64_t stride = kRg * sn * kSize;
 #pragma unroll
-    for (int p = 0; p < kPasses; ++p) x[p].load_nc(in + (p * kRg + r0) * sn * kSize);
+    for (int p = 0; p < kPasses; ++p, row += stride) x[p].load_nc(row);
   } else {
 #pragma unroll
     for (int p = 0; p < kPasses; ++p) {
@@ -263,7 +311,7 @@ __device__ __forceinline__ void append_block(const CacheDev& c, int b, int kv, i
   const bool finite = amax > 0.f && amax < INFINITY;
   const float inv = finite ? __fdiv_rn(127.f, amax) : 0.f;
   const float step = __fdiv_rn(amax, 127.f);
-  if (tid == 0 && page >= 0) c.amax[((int64_t)page * c.n_kv + kv) * 2 + s] = amax;
+  if (tid == 0) c.amax[((int64_t)page * c.n_kv + kv) * 2 + s] = amax;
   if (!finite) {  // no codes: zeros, which stand for 0 or for NaN
 #pragma unroll
     for (int p = 0; p < kPasses; ++p) x[p].zero();
@@ -272,25 +320,23 @@ __device__ __forceinline__ void append_block(const CacheDev& c, int b, int kv, i
     // 0 * step is the value of every code: 0, or NaN of an amax that is infinite or NaN
   }
   int8_t* codes = (s ? c.v_codes : c.k_codes) + ((int64_t)page * c.n_kv + kv) * BS * D + cv * 4;
-  char* values = static_cast<char*>(s ? c.v_values : c.k_values);
   const bool open = p0 + BS > len;
-  if (values) values += (b * c.o_sb + kv * c.o_sh + (int64_t)(p0 - start) * c.o_sn + cv * 4) * kSize;
   if (whole) {
     if (values) {
       values += r0 * c.o_sn * kSize;
       const int64_t stride = kRg * c.o_sn * kSize;
 #pragma unroll
       for (int p = 0; p < kPasses; ++p, values += stride) {
-        float4 r;
+        unsigned long long r[2];
         *reinterpret_cast<uint32_t*>(codes + (p * kRg + r0) * D) = quantize4(x[p].f(), inv, amax, r);
         V o;
-        o.from(make_float4(r.x * step, r.y * step, r.z * step, r.w * step));
+        o.from(scaled(r, step));
         o.store(values);
       }
     } else {
 #pragma unroll
       for (int p = 0; p < kPasses; ++p) {
-        float4 r;
+        unsigned long long r[2];
         *reinterpret_cast<uint32_t*>(codes + (p * kRg + r0) * D) = quantize4(x[p].f(), inv, amax, r);
       }
     }
@@ -299,13 +345,13 @@ __device__ __forceinline__ void append_block(const CacheDev& c, int b, int kv, i
     for (int p = 0; p < kPasses; ++p) {
       const int row = p * kRg + r0;
       const bool have = row < end;
-      float4 r;
+      unsigned long long r[2];
       const uint32_t q = quantize4(x[p].f(), inv, amax, r);
       if (have) *reinterpret_cast<uint32_t*>(codes + row * D) = q;
       if (values && p0 + row >= start && p0 + row - start < c.n) {
         V o;
         o.zero();
-        if (have) o.from(make_float4(r.x * step, r.y * step, r.z * step, r.w * step));
+        if (have) o.from(scaled(r, step));
         o.store(values + row * c.o_sn * kSize);
       }
     }
@@ -321,7 +367,7 @@ __device__ __forceinline__ void append_block(const CacheDev& c, int b, int kv, i
     }
   }
   __syncthreads();  // red is free again
-  if (!open && s == 0 && page >= 0) {
+  if (!open && s == 0) {
     V* rl = reinterpret_cast<V*>(red);
     rl[tid] = lo;
     rl[kT + tid] = hi;
@@ -331,7 +377,7 @@ __device__ __forceinline__ void append_block(const CacheDev& c, int b, int kv, i
         lo.min_with(rl[i * kVec + tid]);
         hi.max_with(rl[kT + i * kVec + tid]);
       }
-      float4 r;
+      unsigned long long r[2];
       uint32_t* bd = reinterpret_cast<uint32_t*>(c.bounds + ((int64_t)page * c.n_kv + kv) * 2 * D) + tid;
       bd[0] = quantize4(lo.f(), inv, amax, r);
       bd[D / 4] = quantize4(hi.f(), inv, amax, r);
@@ -346,12 +392,12 @@ __device__ __forceinline__ void append_block(const CacheDev& c, int b, int kv, i
 template <int DT, int D, int BS>
 __global__ void __launch_bounds__(kAppendThreads<D, BS>, DT == kDtF32 ? 2 : 4) k_cache_append(const CacheDev c, const int nt) {
   __shared__ float4 red[(DT == kDtF32 ? 2 : 1) * kAppendThreads<D, BS>];
-  int64_t i = blockIdx.x;
-  const int j = (int)(i % nt);
-  i /= nt;
+  unsigned i = blockIdx.x;
+  const int j = (int)(i % (unsigned)nt);
+  i /= (unsigned)nt;
   const int s = (int)(i & 1);
   i >>= 1;
-  const int kv = (int)(i % c.n_kv), b = (int)(i / c.n_kv);
+  const int kv = (int)(i % (unsigned)c.n_kv), b = (int)(i / (unsigned)c.n_kv);
   int start, len;
   const int fresh = cache_step_tokens(c, b, start, len);
   len = start + fresh;
@@ -448,12 +494,12 @@ __global__ void __launch_bounds__(kSelThreads, 2) k_cache_select(const CacheDev 
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, t = lane & 3;
-  const int64_t unit = blockIdx.x / ranks;
-  int64_t u = unit;
-  const int kv = (int)(u % c.n_kv);
-  u /= c.n_kv;
-  const int tok = (int)(u % c.n), b = (int)(u / c.n);
-  int32_t* out = c.blocks_out + unit * c.top;
+  const unsigned unit = blockIdx.x / ranks;
+  unsigned u = unit;
+  const int kv = (int)(u % (unsigned)c.n_kv);
+  u /= (unsigned)c.n_kv;
+  const int tok = (int)(u % (unsigned)c.n), b = (int)(u / (unsigned)c.n);
+  int32_t* out = c.blocks_out + (int64_t)unit * c.top;
   int start, len;
   const int fresh = cache_step_tokens(c, b, start, len);
   const int here = tok < fresh ? (start + tok) / c.bs + 1 : 0;       // blocks that stand for election
@@ -518,7 +564,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) k_cache_select(const CacheDev 
       const int head = ht * 8 + (ln >> 2);
       uint32_t neg = 0, pos = 0;
       if (head < c.rep && inv > 0.f) {
-        float4 r;
+        unsigned long long r[2];
         const uint32_t v = quantize4(load4<DT>(row_ptr<DT>(c.q, q0 + (int64_t)head * c.q_sh), wd * 16 + (ln & 3) * 4), inv, amax, r);
         const uint32_t sign = (v >> 7 & 0x01010101u) * 255u;
         neg = v & sign;

@@ -97,33 +97,35 @@ struct Plan {
   int rows, tiles_max, list_groups;
 };
 
-__device__ __forceinline__ int64_t seq_work(const CacheDev& c, const Plan& pl, int b, int rows, int* tiles, int* groups) {
-  int start, len;
-  const int fresh = cache_step_tokens(c, b, start, len);
+__device__ __forceinline__ int seq_work(const CacheDev& c, const Plan& pl, int b, int rows, int* tiles, int* groups) {
   if (c.blocks) {
     *tiles = c.n * pl.tiles_max;
     *groups = pl.list_groups;
-    return (int64_t)*tiles * c.n_kv * *groups;
+  } else {
+    int start, len;
+    const int fresh = cache_step_tokens(c, b, start, len);
+    *tiles = (fresh * c.rep + rows - 1) / rows;
+    *groups = (len + kGroup - 1) / kGroup;
   }
-  *tiles = (int)(((int64_t)fresh * c.rep + rows - 1) / rows);
-  *groups = (len + kGroup - 1) / kGroup;
-  return (int64_t)*tiles * c.n_kv * *groups;
+  return *tiles * c.n_kv * *groups;
 }
 
-__device__ __forceinline__ int64_t block_sum64(int64_t v, int64_t* red) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  int64_t s = 0;
-  for (int i = 0; i < (int)blockDim.x / 32; ++i) s += red[i];
-  return s;
-}
-
-// Blocks that get a range: with less work than blocks the first `total`, one
-// group each, so that no range between two of a unit's is empty.
-__device__ __forceinline__ int ranges_of(int64_t total, int grid) { return total < grid ? (int)total : grid; }
+// Equal ranges of the work: block i of `nblk` takes [begin(i), begin(i + 1)),
+// one group more in the first `more`. With less work than blocks the first
+// `total` get one group each, so that no range between two of a unit's is empty.
+struct Ranges {
+  int nblk, each, more;
+  __device__ __forceinline__ Ranges(int total, int grid) {
+    nblk = total < grid ? total : grid;
+    each = nblk ? (int)((unsigned)total / (unsigned)nblk) : 0;
+    more = total - each * nblk;
+  }
+  __device__ __forceinline__ int begin(int i) const { return i * each + (i < more ? i : more); }
+  __device__ __forceinline__ int of(int x) const {  // the block whose range holds group x
+    const int first = more * (each + 1);
+    return x < first ? (int)((unsigned)x / (unsigned)(each + 1)) : more + (int)((unsigned)(x - first) / (unsigned)each);
+  }
+};
 
 struct Unit {
   int b, kv, tile, start, len, fresh, row0, nrows;  // row0: its first query row, of nrows valid ones
@@ -175,70 +177,75 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, 8 * NT)) k_cache_at
   extern __shared__ __align__(128) unsigned char sm[];
   uint2* qf = reinterpret_cast<uint2*>(sm + Sm::kQ);
   float* sml = reinterpret_cast<float*>(sm + Sm::kMl);
-  __shared__ int64_t red[kWarps];
-  __shared__ int64_t s_base;
-  __shared__ int s_b;
+  __shared__ int red[kWarps], red2[kWarps];
+  __shared__ int s_base, s_b;
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t = lane & 3;
   const int bs_shift = c.bs == 16 ? 4 : c.bs == 32 ? 5 : 6;
   asm volatile("griddepcontrol.launch_dependents;");  // k_cache_combine may take its place and wait
 
   // this block's range of the work, and the sequence it starts in
-  int64_t total;
+  int total;
   if (c.blocks) {
-    total = (int64_t)c.B * c.n * pl.tiles_max * c.n_kv * pl.list_groups;
+    const int per = c.n * pl.tiles_max * c.n_kv * pl.list_groups;
+    total = c.B * per;
+    if (tid == 0) {
+      const Ranges rg(total, gridDim.x);
+      const int at = rg.begin(min((int)blockIdx.x, rg.nblk));
+      s_b = (int)((unsigned)at / (unsigned)per);
+      s_base = s_b * per;
+    }
   } else {
-    int64_t sum = 0;
+    // up to 128 sequences: one scan gives the total and finds the sequence
     int tiles, groups;
-    for (int b = tid; b < c.B; b += kThreads) sum += seq_work(c, pl, b, ROWS, &tiles, &groups);
-    total = block_sum64(sum, red);
-  }
-  const int nblk = ranges_of(total, gridDim.x);
-  const int64_t lo = (int)blockIdx.x < nblk ? blockIdx.x * total / nblk : total;
-  const int64_t hi = (int)blockIdx.x < nblk ? (blockIdx.x + 1) * total / nblk : total;
-  if (tid == 0) { s_b = 0; s_base = 0; }
-  __syncthreads();
-  if (c.blocks) {
-    if (lo >= hi) return;
-    const int64_t per = total / c.B;
-    if (tid == 0) { s_b = (int)(lo / per); s_base = lo / per * per; }
-  } else {
-    int64_t before = 0;
+    const int mine0 = tid < c.B ? seq_work(c, pl, tid, ROWS, &tiles, &groups) : 0;
+    int sum = mine0;
+    for (int b = tid + kThreads; b < c.B; b += kThreads) sum += seq_work(c, pl, b, ROWS, &tiles, &groups);
+    sum = __reduce_add_sync(0xffffffffu, sum);
+    if (lane == 0) red[w] = sum;
+    __syncthreads();
+    total = 0;
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) total += red[i];
+    const Ranges rg(total, gridDim.x);
+    const int at = rg.begin(min((int)blockIdx.x, rg.nblk));
+    int before = 0;
     for (int b0 = 0; b0 < c.B; b0 += kThreads) {
-      int tiles, groups;
-      const int64_t mine = b0 + tid < c.B ? seq_work(c, pl, b0 + tid, ROWS, &tiles, &groups) : 0;
-      int64_t upto = mine;
+      const int mine = b0 == 0 ? mine0 : b0 + tid < c.B ? seq_work(c, pl, b0 + tid, ROWS, &tiles, &groups) : 0;
+      int upto = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
+        const int x = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += x;
       }
+      if (b0) __syncthreads();
+      if (lane == 31) red2[w] = upto;
       __syncthreads();
-      if (lane == 31) red[w] = upto;
-      __syncthreads();
-      int64_t all = 0;
+      int all = 0;
+#pragma unroll
       for (int i = 0; i < kWarps; ++i) {
-        if (i < w) upto += red[i];
-        all += red[i];
+        if (i < w) upto += red2[i];
+        all += red2[i];
       }
-      const int64_t from = before + upto - mine;
-      if (lo >= from && lo < from + mine) { s_b = b0 + tid; s_base = from; }
+      const int from = before + upto - mine;
+      if (at >= from && at < from + mine) { s_b = b0 + tid; s_base = from; }
       if (blockIdx.x == 0 && b0 + tid < c.B) c.prefix[b0 + tid] = from;
       before += all;
     }
     if (blockIdx.x == 0 && tid == 0) c.prefix[c.B] = total;
   }
   __syncthreads();
-  if (lo >= hi) return;
+  const Ranges rg(total, gridDim.x);
+  if ((int)blockIdx.x >= rg.nblk) return;
+  const int lo = rg.begin(blockIdx.x), hi = rg.begin(blockIdx.x + 1);
 
-  int b = s_b;
-  int64_t base = s_base;
-  for (int64_t at = lo; at < hi;) {
+  int b = s_b, base = s_base;
+  for (int at = lo; at < hi;) {
     int tiles, groups;
-    const int64_t mine = seq_work(c, pl, b, ROWS, &tiles, &groups);
+    const int mine = seq_work(c, pl, b, ROWS, &tiles, &groups);
     if (at >= base + mine) { base += mine; ++b; continue; }
-    const int u = (int)((at - base) / groups);
-    const int64_t ubeg = base + (int64_t)u * groups, uend = ubeg + groups;
-    const int g0 = (int)(at - ubeg), g1 = (int)((hi < uend ? hi : uend) - ubeg);
+    const int u = (int)((unsigned)(at - base) / (unsigned)groups);
+    const int ubeg = base + u * groups, uend = ubeg + groups;
+    const int g0 = at - ubeg, g1 = min(hi, uend) - ubeg;
     at = ubeg + g1;
     const Unit x = unit_of<ROWS>(c, pl, b, u, tiles);
 
@@ -525,51 +532,88 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, 8 * NT)) k_cache_at
 // is launched while k_cache_attn still runs and waits for it behind its set-up.
 template <int D, int NT, bool F32>
 __global__ void __launch_bounds__(kThreads) k_cache_combine(const CacheDev c, const Plan pl, const int ngrid,
-                                                            const int rows_used, const int64_t nrows) {
+                                                            const int rows_used, const int nrows) {
   constexpr int ROWS = 8 * NT, E = D / 32;
   const int lane = threadIdx.x & 31;
-  const int64_t id = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+  const unsigned id = blockIdx.x * kWarps + (threadIdx.x >> 5);
   // Every warp waits, so that this kernel's end implies the other's.
-  if (id >= nrows) {
+  if (id >= (unsigned)nrows) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     return;
   }
-  const int r = (int)(id % rows_used);
   const int per = pl.tiles_max * (c.blocks ? c.n : 1);  // row tiles a (sequence, kv head) can have
-  const int64_t unit = id / rows_used;
-  const int b = (int)(unit / ((int64_t)per * c.n_kv)), u = (int)(unit % ((int64_t)per * c.n_kv));
-  const int kv = u / per, tile = u % per;
+  const unsigned unit = id / (unsigned)rows_used, units_b = (unsigned)per * c.n_kv;
+  const int r = (int)(id - unit * rows_used);
+  const int b = (int)(unit / units_b), u = (int)(unit % units_b);
+  const int kv = (int)((unsigned)u / (unsigned)per), tile = u - kv * per;
   int tiles, groups;
-  const int64_t mine = seq_work(c, pl, b, ROWS, &tiles, &groups);
+  const int mine = seq_work(c, pl, b, ROWS, &tiles, &groups);
   const Unit x = unit_of<ROWS>(c, pl, b, u, per);
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (r >= (c.blocks ? c.rep - tile % pl.tiles_max * ROWS : c.n * c.rep - x.row0)) return;
   const int row = x.row0 + r, tok = row / c.rep, h = kv * c.rep + row - tok * c.rep;
   const int64_t at = x.b * c.o_sb + h * c.o_sh + tok * c.o_sn;
+  int total = mine * c.B, base = mine * b;
+  if (!c.blocks && c.B <= 128) {
+    // what the other kernel has found out too, while it still runs
+    total = base = 0;
+    for (int i = lane; i < c.B; i += 32) {
+      int a, e;
+      const int v = seq_work(c, pl, i, ROWS, &a, &e);
+      total += v;
+      base += i < b ? v : 0;
+    }
+    total = __reduce_add_sync(0xffffffffu, total);
+    base = __reduce_add_sync(0xffffffffu, base);
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (r >= (c.blocks ? c.rep - tile % pl.tiles_max * ROWS : c.n * c.rep - x.row0)) return;
   float m = kEmpty, l = 0.f, o[E];
 #pragma unroll
   for (int i = 0; i < E; ++i) o[i] = 0.f;
   if (tile < tiles && mine > 0 && r < x.nrows) {
-    const int64_t total = c.blocks ? mine * c.B : c.prefix[c.B], base = c.blocks ? mine * b : c.prefix[b];
-    const int64_t ubeg = base + ((int64_t)kv * tiles + tile) * groups, uend = ubeg + groups;
-    // block i holds [i total / nblk, (i + 1) total / nblk)
-    const int nblk = ranges_of(total, ngrid);
-    const int c0 = (int)(((ubeg + 1) * nblk - 1) / total), c1 = (int)((uend * nblk - 1) / total);
+    if (!c.blocks && c.B > 128) {
+      total = c.prefix[c.B];
+      base = c.prefix[b];
+    }
+    const int ubeg = base + (kv * tiles + tile) * groups;
+    const Ranges rg(total, ngrid);
+    const int c0 = rg.of(ubeg), c1 = rg.of(ubeg + groups - 1);
     if (c0 == c1) return;  // that block stored the row
     const auto slot = [&](int k) { return ((int64_t)k * 2 + (k == c0)) * ROWS + r; };
-    for (int k = c0 + lane; k <= c1; k += 32) m = fmaxf(m, c.part_ml[slot(k) * 2]);
+    // the first sums are under way while their weights are found
+    constexpr int kAhead = 4;
+    float first[kAhead][E];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const float* p = c.part_o + slot(min(c0 + j, c1)) * D + lane;
+#pragma unroll
+      for (int i = 0; i < E; ++i) first[j][i] = p[32 * i];
+    }
+    float2 ml = make_float2(kEmpty, 0.f);
+    if (c0 + lane <= c1) ml = *reinterpret_cast<const float2*>(c.part_ml + slot(c0 + lane) * 2);
+    m = ml.x;
+    for (int k = c0 + 32 + lane; k <= c1; k += 32) m = fmaxf(m, c.part_ml[slot(k) * 2]);
 #pragma unroll
     for (int q = 16; q; q >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, q));
     for (int k0 = c0; k0 <= c1; k0 += 32) {
-      float f = 0.f;
-      if (k0 + lane <= c1) {
-        const float2 ml = *reinterpret_cast<const float2*>(c.part_ml + slot(k0 + lane) * 2);
-        f = ex2(ml.x - m);
-        l = fmaf(f, ml.y, l);
+      if (k0 > c0) {
+        ml = make_float2(kEmpty, 0.f);
+        if (k0 + lane <= c1) ml = *reinterpret_cast<const float2*>(c.part_ml + slot(k0 + lane) * 2);
       }
+      const float f = ex2(ml.x - m);
+      l = fmaf(f, ml.y, l);
       const int cnt = min(32, c1 - k0 + 1);
+      int j = 0;
+      if (k0 == c0) {
+#pragma unroll
+        for (; j < kAhead; ++j) {
+          const float fj = __shfl_sync(0xffffffffu, f, j);
+          if (j < cnt)
+#pragma unroll
+            for (int i = 0; i < E; ++i) o[i] = fmaf(fj, first[j][i], o[i]);
+        }
+      }
 #pragma unroll 4
-      for (int j = 0; j < cnt; ++j) {
+      for (; j < cnt; ++j) {
         const float fj = __shfl_sync(0xffffffffu, f, j);
         const float* p = c.part_o + slot(k0 + j) * D + lane;
 #pragma unroll
@@ -617,7 +661,7 @@ cudaError_t run_attn(const CacheDev& c, const Plan& pl, cudaStream_t st) {
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   const int rows_used = (int)((c.blocks ? c.rep : (int64_t)c.n * c.rep) < ROWS ? (c.blocks ? c.rep : c.n * c.rep) : ROWS);
   const int64_t nrows = units * rows_used;
-  if ((nrows + kWarps - 1) / kWarps > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  if (nrows > 0x7fffffff - kWarps) return cudaErrorInvalidConfiguration;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((nrows + kWarps - 1) / kWarps));
   cfg.blockDim = dim3(kThreads);
@@ -627,7 +671,7 @@ cudaError_t run_attn(const CacheDev& c, const Plan& pl, cudaStream_t st) {
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, k_cache_combine<D, NT, F32>, c, pl, (int)c.grid, rows_used, nrows);
+  e = cudaLaunchKernelEx(&cfg, k_cache_combine<D, NT, F32>, c, pl, c.grid, rows_used, (int)nrows);
   note_launch();
   return e;
 }
@@ -651,12 +695,13 @@ size_t cache_attn_workspace_layout(CacheDev* c, void* ws) {
   const Plan p = plan_of(*c);
   const int64_t groups = p.list_groups ? p.list_groups : ((int64_t)c->max_blocks * c->bs + kGroup - 1) / kGroup;
   const int64_t most = units_of(*c, p) * groups;  // no use for more blocks than groups
+  if (most > 0x7fffffff) return 0;                // the kernels count groups in 32 bits
   const int64_t full = 148 * blocks_per_sm(c->d, p.rows);
   c->grid = (int)(most < full ? most : full);
-  const size_t o_pre = ((size_t)(c->B + 1) * 8 + 255) / 256 * 256;
+  const size_t o_pre = ((size_t)(c->B + 1) * 4 + 255) / 256 * 256;
   const size_t o_ml = o_pre + ((size_t)c->grid * 2 * p.rows * 2 * 4 + 255) / 256 * 256;
   char* base = static_cast<char*>(ws);
-  c->prefix = reinterpret_cast<int64_t*>(base);
+  c->prefix = reinterpret_cast<int32_t*>(base);
   c->part_ml = reinterpret_cast<float*>(base + o_pre);
   c->part_o = reinterpret_cast<float*>(base + o_ml);
   return o_ml + (size_t)c->grid * 2 * p.rows * c->d * 4;

@@ -595,6 +595,7 @@ int ssa_cache_attn(const ssa_cache_params* p, const void* q, const int8_t* k_cod
   ssa::CacheDev c = cache_dev(p);
   c.blocks = blocks;
   const size_t need = ssa::cache_attn_workspace_layout(&c, nullptr);
+  if (!need) return fail(SSA_ERR_UNSUPPORTED, "B * n_kv * n * H / n_kv * max_blocks * block_size is too large for one call");
   if (!workspace || workspace_bytes < need || !aligned(workspace, 16))
     return fail(SSA_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", need, workspace_bytes);
   ssa::cache_attn_workspace_layout(&c, workspace);

@@ -218,7 +218,7 @@ struct CacheDev {
   void* out;
   float* lse;
   // attention workspace
-  int64_t* prefix;        // [B + 1] work before each sequence
+  int32_t* prefix;        // [B + 1] work before each sequence, in all
   float* part_o;          // [2 * grid][rows][d] unnormalised outputs
   float* part_ml;         // [2 * grid][rows][2] their exponent offset and weight sum
   int grid;
@@ -238,7 +238,8 @@ cudaError_t launch_cache_reserve(const ReserveDev& r, cudaStream_t st);
 cudaError_t launch_cache_append(const CacheDev& c, cudaStream_t st);
 size_t cache_select_smem(const CacheDev& c);
 cudaError_t launch_cache_select(const CacheDev& c, cudaStream_t st);
-// Fills the workspace pointers of c (ws may be null) and c->grid; bytes needed.
+// Fills the workspace pointers of c (ws may be null) and c->grid; bytes needed
+// (0: more work than the kernels count).
 size_t cache_attn_workspace_layout(CacheDev* c, void* ws);
 cudaError_t launch_cache_attn(const CacheDev& c, cudaStream_t st);
 
