@@ -438,8 +438,8 @@ constexpr int kSelStages = 3;  // 16 blocks' bounds each, for every warp
 template <int D>
 struct SelSmem {
   static constexpr int kTile = 16 * kPitch<D>, kRing = kSelStages * 2 * kTile;
-  static constexpr int kMeta = kSelWarps * kRing;                 // [kSelWarps][kSelStages][16] amax
-  static constexpr int kQ = kMeta + kSelWarps * kSelStages * 64;  // [tiles of 8 heads][2][D / 16][32] words of q-, q+
+  static constexpr int kMeta = kSelWarps * kRing;                  // [kSelWarps][kSelStages]: [16] amax, [16] page
+  static constexpr int kQ = kMeta + kSelWarps * kSelStages * 128;  // [tiles of 8 heads][2][D / 16][32] words of q-, q+
   static size_t bytes(const CacheDev& c) {
     return kQ + (size_t)((c.rep + 7) / 8) * 2 * (D / 16) * 32 * 4 + (size_t)c.max_blocks * 8;
   }
@@ -513,10 +513,16 @@ __global__ void __launch_bounds__(kSelThreads, 2) k_cache_select(const CacheDev 
     if (ranks > 1) cluster_arrive();  // waited for before the first block's memory is written
     if (tid == 0) s_n = 0;
 
+    // q's amax: its first elements ahead of the bounds in the memory's queue
+    const int64_t q0 = b * c.q_sb + (int64_t)kv * c.rep * c.q_sh + (int64_t)tok * c.q_sn;
+    Vec4<DT> qv;
+    qv.zero();
+    if (tid < c.rep * (D / 4)) qv.load_nc(row_ptr<DT>(c.q, q0 + (int64_t)(tid / (D / 4)) * c.q_sh + tid % (D / 4) * 4));
+
     // Tile i (blocks 16 i .. 16 i + 15) is warp i mod nw's. Lanes 0-15 hold the
     // pages of its next tile, lanes 16-31 those of the one after.
     const int nw = (int)ranks * kSelWarps, tiles = (here + 15) / 16;
-    const uint32_t ring_a = smem_addr(sm) + w * Sm::kRing, meta_a = smem_addr(sm + Sm::kMeta) + w * kSelStages * 64;
+    const uint32_t ring_a = smem_addr(sm) + w * Sm::kRing, meta_a = smem_addr(sm + Sm::kMeta) + w * kSelStages * 128;
     const auto look_up = [&](int tile) {
       const int e = (tile + (lane >> 4) * nw) * 16 + (lane & 15);
       return e < here ? cache_page(c, b, e) : -1;
@@ -535,8 +541,11 @@ __global__ void __launch_bounds__(kSelThreads, 2) k_cache_select(const CacheDev 
           copy16(ring_a + st * 2 * Sm::kTile + (ch >= D / 16) * Sm::kTile + tile_at<D>(row, ch % (D / 16)),
                  c.bounds + ((int64_t)pg * c.n_kv + kv) * 2 * D + ch * 16);
         }
-        const int mine = max(__shfl_sync(0xffffffffu, pages, half + (lane & 15)), 0);
-        if (lane < 16) copy4(meta_a + st * 64 + lane * 4, c.amax + ((int64_t)mine * c.n_kv + kv) * 2);
+        const int mine = __shfl_sync(0xffffffffu, pages, half + (lane & 15));
+        if (lane < 16) {
+          copy4(meta_a + st * 128 + lane * 4, c.amax + ((int64_t)max(mine, 0) * c.n_kv + kv) * 2);
+          *reinterpret_cast<int*>(sm + Sm::kMeta + (w * kSelStages + st) * 128 + 64 + lane * 4) = mine;
+        }
         ++sent;
         if (!(sent & 1)) {
           pages = pages_n;
@@ -549,9 +558,8 @@ __global__ void __launch_bounds__(kSelThreads, 2) k_cache_select(const CacheDev 
     for (int i = 0; i < kSelStages - 1; ++i) issue();
 
     // q in 8 bits, one amax for the group's heads
-    const int64_t q0 = b * c.q_sb + (int64_t)kv * c.rep * c.q_sh + (int64_t)tok * c.q_sn;
-    uint32_t top = 0;
-    for (int i = tid; i < c.rep * (D / 4); i += kSelThreads)
+    uint32_t top = abs_top(qv.f());
+    for (int i = tid + kSelThreads; i < c.rep * (D / 4); i += kSelThreads)
       top = max(top, abs_top(load4<DT>(row_ptr<DT>(c.q, q0 + (int64_t)(i / (D / 4)) * c.q_sh), i % (D / 4) * 4)));
     top = __reduce_max_sync(0xffffffffu, top);
     if (lane == 0) red[w] = top;
@@ -618,13 +626,13 @@ __global__ void __launch_bounds__(kSelThreads, 2) k_cache_select(const CacheDev 
       const int blk = e0 + lane;
       if (lane < 16 && blk < here) {
         unsigned long long k = 0;
-        if (cache_page(c, b, blk) >= 0) {
+        const unsigned char* meta = sm + Sm::kMeta + (w * kSelStages + st) * 128 + lane * 4;
+        if (*reinterpret_cast<const int*>(meta + 64) >= 0) {
           if (blk < c.sink || blk >= here - c.local) {
             k = ~0ull;
             ++my_forced;
           } else {
-            const float am = *reinterpret_cast<const float*>(sm + Sm::kMeta + (w * kSelStages + st) * 64 + lane * 4);
-            k = order_key((double)(lane < 8 ? v0 : v1) * (double)am);
+            k = order_key((double)(lane < 8 ? v0 : v1) * (double)*reinterpret_cast<const float*>(meta));
             my_lo = min(my_lo, k);
             my_hi = max(my_hi, k);
           }

@@ -84,11 +84,34 @@ struct Smem {
   static constexpr int kWarp = kRing > kOut ? kRing : kOut;
   static constexpr int kMeta = kWarps * kWarp;                           // [kWarps][kStages] {amax k, v, first key, -}
   static constexpr int kMl = kMeta + kWarps * kStages * 16;              // [kWarps][8 NT] {offset, sum}
-  static constexpr int kQ = kMl + kWarps * 8 * NT * 8;                   // [F32 ? 2 : 1][NT][D / 16][32] uint2
+  static constexpr int kScale = kMl + kWarps * 8 * NT * 8;               // [8 NT] score factor of a row
+  static constexpr int kQ = kScale + 8 * NT * 4;                         // [F32 ? 2 : 1][NT][D / 16][32] uint2
   static constexpr int kBytes = kQ + (F32 ? 2 : 1) * NT * (D / 16) * 32 * 8;
 };
 // Blocks that share an SM (registers for 16 and 32 rows, the rings for 8).
 constexpr int blocks_per_sm(int d, int rows) { return rows == 32 ? 2 : rows == 16 || d >= 96 ? 3 : 4; }
+
+// Four elements as they lie in memory: widened where they are used, so that
+// a load does not wait where it is issued.
+template <bool F32>
+struct Raw4 {
+  uint4 u;
+  __device__ __forceinline__ void zero() { u = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ void load(const void* row, int i) {
+    if constexpr (F32) u = __ldg(reinterpret_cast<const uint4*>(static_cast<const float*>(row) + i));
+    else {
+      const uint2 v = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(row) + i));
+      u.x = v.x;
+      u.y = v.y;
+    }
+  }
+  __device__ __forceinline__ float4 f() const {
+    if constexpr (F32) return make_float4(__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w));
+    else
+      return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
+                         __uint_as_float(u.y & 0xffff0000u));
+  }
+};
 
 // Units and work of the call. Without a list a unit is (sequence, kv head,
 // tile of query rows) and its work the sequence's groups of 64 keys; with one
@@ -177,6 +200,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, 8 * NT)) k_cache_at
   extern __shared__ __align__(128) unsigned char sm[];
   uint2* qf = reinterpret_cast<uint2*>(sm + Sm::kQ);
   float* sml = reinterpret_cast<float*>(sm + Sm::kMl);
+  float* srow = reinterpret_cast<float*>(sm + Sm::kScale);
   __shared__ int red[kWarps], red2[kWarps];
   __shared__ int s_base, s_b;
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t = lane & 3;
@@ -253,6 +277,18 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, 8 * NT)) k_cache_at
     const int lim_max = x.nrows <= 0 ? 0 : c.causal ? x.start + (x.row0 + x.nrows - 1) / c.rep + 1 : x.len;
     const int lim_min = c.causal ? x.start + x.row0 / c.rep + 1 : x.len;
 
+    // Warp i < NT fetches the i-th 8 query rows, ahead of the codes in the memory's queue.
+    Raw4<F32> qv[W16];
+    if (w < NT && w * 8 + g < x.nrows) {
+      const int row = x.row0 + w * 8 + g, tok = row / c.rep, h = x.kv * c.rep + row - tok * c.rep;
+      const void* qr = row_ptr<kDt>(c.q, x.b * c.q_sb + h * c.q_sh + tok * c.q_sn);
+#pragma unroll
+      for (int i = 0; i < W16; ++i) qv[i].load(qr, i * 16 + t * 4);
+    } else {
+#pragma unroll
+      for (int i = 0; i < W16; ++i) qv[i].zero();
+    }
+
     // The warp's 16 keys of each group, in order, through its ring. Lane l
     // holds the page of group s0 + l, and of group s0 + 32 + l (loaded ahead).
     unsigned char* ring = sm + w * Sm::kWarp;
@@ -310,22 +346,13 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, 8 * NT)) k_cache_at
     for (int i = 0; i < kStages - 1; ++i) issue();
 
     // Q as the products' 8-wide operand: rows scaled into fp16's range by a power of two
-    float sfac[NT][2];
-    int lim[NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int r = nt * 8 + g;
-      const bool have = r < x.nrows;
-      const int row = x.row0 + (have ? r : 0), tok = row / c.rep, h = x.kv * c.rep + row - tok * c.rep;
-      const void* qr = row_ptr<kDt>(c.q, x.b * c.q_sb + h * c.q_sh + tok * c.q_sn);
-      float4 v[W16];
+    if (w < NT) {
       uint32_t top = 0;
 #pragma unroll
       for (int i = 0; i < W16; ++i) {
-        v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (have) v[i] = load4<kDt>(qr, i * 16 + t * 4);
-        top = max(top, max(max(__float_as_uint(v[i].x) & 0x7fffffffu, __float_as_uint(v[i].y) & 0x7fffffffu),
-                           max(__float_as_uint(v[i].z) & 0x7fffffffu, __float_as_uint(v[i].w) & 0x7fffffffu)));
+        const float4 v = qv[i].f();
+        top = max(top, max(max(__float_as_uint(v.x) & 0x7fffffffu, __float_as_uint(v.y) & 0x7fffffffu),
+                           max(__float_as_uint(v.z) & 0x7fffffffu, __float_as_uint(v.w) & 0x7fffffffu)));
       }
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
@@ -335,23 +362,27 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, 8 * NT)) k_cache_at
       const float up = __uint_as_float((uint32_t)(e + 127) << 23), down = __uint_as_float((uint32_t)(127 - e) << 23);
 #pragma unroll
       for (int i = 0; i < W16; ++i) {
-        if (i % kWarps != w) continue;
+        const float4 v = qv[i].f();
         uint2 hi2, lo2;
-        split_f16(v[i].x * up, v[i].y * up, hi2.x, lo2.x);
-        split_f16(v[i].z * up, v[i].w * up, hi2.y, lo2.y);
-        qf[(nt * W16 + i) * 32 + lane] = hi2;
-        if constexpr (F32) qf[((NT + nt) * W16 + i) * 32 + lane] = lo2;
+        split_f16(v.x * up, v.y * up, hi2.x, lo2.x);
+        split_f16(v.z * up, v.w * up, hi2.y, lo2.y);
+        qf[(w * W16 + i) * 32 + lane] = hi2;
+        if constexpr (F32) qf[((NT + w) * W16 + i) * 32 + lane] = lo2;
       }
-      const float mine_s = c.scale * 1.4426950408889634f * down;
+      if (t == 0) srow[w * 8 + g] = c.scale * 1.4426950408889634f * down;
+    }
+    __syncthreads();
+    float sfac[NT][2];
+    int lim[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        sfac[nt][k] = __shfl_sync(0xffffffffu, mine_s, (2 * t + k) * 4);
         const int rr = nt * 8 + 2 * t + k;
+        sfac[nt][k] = srow[rr];
         lim[nt][k] = INT32_MAX;  // rows behind the last one: computed, never stored
         if (rr < x.nrows) lim[nt][k] = c.causal ? x.start + (x.row0 + rr) / c.rep + 1 : x.len;
       }
-    }
-    __syncthreads();
 
     float acc[W16][NT][4], mref[NT][2], lsum[NT][2];
 #pragma unroll
