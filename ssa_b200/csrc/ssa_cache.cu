@@ -53,6 +53,7 @@ __global__ void __launch_bounds__(kReserveThreads) k_cache_reserve(const Reserve
   __shared__ int s_given, s_refused;
   const int rank = blockIdx.x, ranks = gridDim.x, threads = blockDim.x;
   const int lane = threadIdx.x & 31;
+  grid_wait();
   const int failed = r.state[1];
   const int count = max(0, min(r.state[0], r.num_pages));
   if (threadIdx.x == 0) s_given = s_refused = 0;
@@ -201,7 +202,6 @@ struct Vec4<kDtF32> {
   float4 v;
   __device__ __forceinline__ void zero() { v = make_float4(0.f, 0.f, 0.f, 0.f); }
   __device__ __forceinline__ void load(const void* p) { v = *static_cast<const float4*>(p); }
-  __device__ __forceinline__ void load_nc(const void* p) { v = __ldg(static_cast<const float4*>(p)); }
   __device__ __forceinline__ void store(void* p) const { *static_cast<float4*>(p) = v; }
   __device__ __forceinline__ float4 f() const { return v; }
   static __device__ __forceinline__ float mn(float a, float b) { float r; asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
@@ -215,7 +215,6 @@ struct Vec4<kDtBF16> {
   uint2 v;
   __device__ __forceinline__ void zero() { v = make_uint2(0u, 0u); }
   __device__ __forceinline__ void load(const void* p) { v = *static_cast<const uint2*>(p); }
-  __device__ __forceinline__ void load_nc(const void* p) { v = __ldg(static_cast<const uint2*>(p)); }
   __device__ __forceinline__ void store(void* p) const { *static_cast<uint2*>(p) = v; }
   __device__ __forceinline__ float4 f() const {
     return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16),
@@ -282,13 +281,13 @@ __device__ __forceinline__ void append_block(const CacheDev& c, int b, int kv, i
     const char* row = in + r0 * sn * kSize;
     const int64_t stride = kRg * sn * kSize;
 #pragma unroll
-    for (int p = 0; p < kPasses; ++p, row += stride) x[p].load_nc(row);
+    for (int p = 0; p < kPasses; ++p, row += stride) x[p].load(row);
   } else {
 #pragma unroll
     for (int p = 0; p < kPasses; ++p) {
       const int row = p * kRg + r0;
       x[p].zero();
-      if (row >= old && row < end) x[p].load_nc(in + row * sn * kSize);
+      if (row >= old && row < end) x[p].load(in + row * sn * kSize);
       if (row < old) x[p].load(tail + (int64_t)row * D * kSize);
     }
   }
@@ -361,7 +360,7 @@ __device__ __forceinline__ void append_block(const CacheDev& c, int b, int kv, i
     for (int p = 0; p < kPasses; ++p) {
       const int row = p * kRg + r0;
       if (row >= old && row < end) {
-        if (!finite) x[p].load_nc(in + row * sn * kSize);
+        if (!finite) x[p].load(in + row * sn * kSize);
         x[p].store(tail + (int64_t)row * D * kSize);
       }
     }
@@ -398,6 +397,7 @@ __global__ void __launch_bounds__(kAppendThreads<D, BS>, DT == kDtF32 ? 2 : 4) k
   const int s = (int)(i & 1);
   i >>= 1;
   const int kv = (int)(i % (unsigned)c.n_kv), b = (int)(i / (unsigned)c.n_kv);
+  grid_wait();
   int start, len;
   const int fresh = cache_step_tokens(c, b, start, len);
   len = start + fresh;
@@ -413,9 +413,10 @@ cudaError_t run_append(const CacheDev& c, cudaStream_t st) {
   const int nt = (c.n + BS - 2) / BS + 1;
   const int64_t grid = (int64_t)c.B * c.n_kv * 2 * nt;
   if (grid > 0x7fffffff) return cudaErrorInvalidConfiguration;
-  k_cache_append<DT, D, BS><<<(unsigned)grid, kAppendThreads<D, BS>, 0, st>>>(c, nt);
+  CacheLaunch l((unsigned)grid, kAppendThreads<D, BS>, 0, st);
+  const cudaError_t e = cudaLaunchKernelEx(&l.cfg, k_cache_append<DT, D, BS>, c, nt);
   note_launch();
-  return cudaGetLastError();
+  return e;
 }
 
 template <int DT, int D>
@@ -500,6 +501,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) k_cache_select(const CacheDev 
   u /= (unsigned)c.n_kv;
   const int tok = (int)(u % (unsigned)c.n), b = (int)(u / (unsigned)c.n);
   int32_t* out = c.blocks_out + (int64_t)unit * c.top;
+  grid_wait();
   int start, len;
   const int fresh = cache_step_tokens(c, b, start, len);
   const int here = tok < fresh ? (start + tok) / c.bs + 1 : 0;       // blocks that stand for election
@@ -517,39 +519,46 @@ __global__ void __launch_bounds__(kSelThreads, 2) k_cache_select(const CacheDev 
     const int64_t q0 = b * c.q_sb + (int64_t)kv * c.rep * c.q_sh + (int64_t)tok * c.q_sn;
     Vec4<DT> qv;
     qv.zero();
-    if (tid < c.rep * (D / 4)) qv.load_nc(row_ptr<DT>(c.q, q0 + (int64_t)(tid / (D / 4)) * c.q_sh + tid % (D / 4) * 4));
+    if (tid < c.rep * (D / 4)) qv.load(row_ptr<DT>(c.q, q0 + (int64_t)(tid / (D / 4)) * c.q_sh + tid % (D / 4) * 4));
 
     // Tile i (blocks 16 i .. 16 i + 15) is warp i mod nw's. Lanes 0-15 hold the
-    // pages of its next tile, lanes 16-31 those of the one after.
+    // pages of its next tile, lanes 16-31 those of the one after; the table's
+    // entries of the two behind them are on their way.
     const int nw = (int)ranks * kSelWarps, tiles = (here + 15) / 16;
-    const uint32_t ring_a = smem_addr(sm) + w * Sm::kRing, meta_a = smem_addr(sm + Sm::kMeta) + w * kSelStages * 128;
+    const uint32_t ring_a = smem_addr(sm) + w * Sm::kRing;
+    unsigned char* meta = sm + Sm::kMeta + w * kSelStages * 128 + (lane & 15) * 4;
     const auto look_up = [&](int tile) {
       const int e = (tile + (lane >> 4) * nw) * 16 + (lane & 15);
-      return e < here ? cache_page(c, b, e) : -1;
+      return e < here ? cache_entry(c, b, e) : -1;
     };
     const int first = (int)rank * kSelWarps + w;
-    int pages = look_up(first), pages_n = look_up(first + 2 * nw);
-    int sent = 0;
+    int pages = look_up(first), entries = look_up(first + 2 * nw);
+    pages = cache_checked(c, pages);
+    // 16 rows of 2 D / 16 chunks, a row's chunks side by side: copy i of a lane
+    // is chunk (32 i + lane) mod (D / 8) of row (32 i + lane) / (D / 8)
+    const int8_t* kv_bounds = c.bounds + (int64_t)kv * 2 * D;
+    const unsigned page_bytes = (unsigned)c.n_kv * 2 * D;
+    int sent = 0, sent_stage = 0;
     const auto issue = [&]() {
-      const int tile = first + sent * nw;
-      if (tile < tiles) {
-        const int st = sent % kSelStages, half = (sent & 1) * 16;
+      if (first + sent * nw < tiles) {
+        const int half = (sent & 1) * 16;
+        const uint32_t to = ring_a + sent_stage * 2 * Sm::kTile;
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) {  // 16 rows of 2 D / 16 chunks, a row's chunks side by side
+        for (int i = 0; i < D / 16; ++i) {
           const int id = i * 32 + lane, row = id / (D / 8), ch = id % (D / 8);
-          const int pg = max(__shfl_sync(0xffffffffu, pages, half + row), 0);
-          copy16(ring_a + st * 2 * Sm::kTile + (ch >= D / 16) * Sm::kTile + tile_at<D>(row, ch % (D / 16)),
-                 c.bounds + ((int64_t)pg * c.n_kv + kv) * 2 * D + ch * 16);
+          const unsigned pg = (unsigned)max(__shfl_sync(0xffffffffu, pages, half + row), 0);
+          copy16(to + (ch >= D / 16) * Sm::kTile + tile_at<D>(row, ch % (D / 16)), kv_bounds + (uint64_t)pg * page_bytes + ch * 16);
         }
-        const int mine = __shfl_sync(0xffffffffu, pages, half + (lane & 15));
+        const int pg = __shfl_sync(0xffffffffu, pages, half + (lane & 15));
         if (lane < 16) {
-          copy4(meta_a + st * 128 + lane * 4, c.amax + ((int64_t)max(mine, 0) * c.n_kv + kv) * 2);
-          *reinterpret_cast<int*>(sm + Sm::kMeta + (w * kSelStages + st) * 128 + 64 + lane * 4) = mine;
+          copy4(smem_addr(meta + sent_stage * 128), c.amax + ((int64_t)max(pg, 0) * c.n_kv + kv) * 2);
+          *reinterpret_cast<int*>(meta + sent_stage * 128 + 64) = pg;
         }
         ++sent;
+        sent_stage = sent_stage == kSelStages - 1 ? 0 : sent_stage + 1;
         if (!(sent & 1)) {
-          pages = pages_n;
-          pages_n = look_up(first + (sent + 2) * nw);
+          pages = cache_checked(c, entries);
+          entries = look_up(first + (sent + 2) * nw);
         }
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
@@ -559,8 +568,10 @@ __global__ void __launch_bounds__(kSelThreads, 2) k_cache_select(const CacheDev 
 
     // q in 8 bits, one amax for the group's heads
     uint32_t top = abs_top(qv.f());
-    for (int i = tid + kSelThreads; i < c.rep * (D / 4); i += kSelThreads)
-      top = max(top, abs_top(load4<DT>(row_ptr<DT>(c.q, q0 + (int64_t)(i / (D / 4)) * c.q_sh), i % (D / 4) * 4)));
+    for (int i = tid + kSelThreads; i < c.rep * (D / 4); i += kSelThreads) {
+      qv.load(row_ptr<DT>(c.q, q0 + (int64_t)(i / (D / 4)) * c.q_sh + i % (D / 4) * 4));
+      top = max(top, abs_top(qv.f()));
+    }
     top = __reduce_max_sync(0xffffffffu, top);
     if (lane == 0) red[w] = top;
     __syncthreads();
@@ -573,7 +584,8 @@ __global__ void __launch_bounds__(kSelThreads, 2) k_cache_select(const CacheDev 
       uint32_t neg = 0, pos = 0;
       if (head < c.rep && inv > 0.f) {
         unsigned long long r[2];
-        const uint32_t v = quantize4(load4<DT>(row_ptr<DT>(c.q, q0 + (int64_t)head * c.q_sh), wd * 16 + (ln & 3) * 4), inv, amax, r);
+        qv.load(row_ptr<DT>(c.q, q0 + (int64_t)head * c.q_sh + wd * 16 + (ln & 3) * 4));
+        const uint32_t v = quantize4(qv.f(), inv, amax, r);
         const uint32_t sign = (v >> 7 & 0x01010101u) * 255u;
         neg = v & sign;
         pos = v & ~sign;
@@ -587,35 +599,44 @@ __global__ void __launch_bounds__(kSelThreads, 2) k_cache_select(const CacheDev 
     const uint32_t keys0 = at_rank0(keys);
     unsigned long long my_lo = ~0ull, my_hi = 0;
     int my_forced = 0;
-    int done = 0;
+    uint32_t q1[2][D / 16];  // the query operand of up to 8 heads stays in registers
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) q1[h][k] = qf[(h * (D / 16) + k) * 32 + lane];
+    int done = 0, stage = 0;
     while (true) {
       asm volatile("cp.async.wait_group %0;" ::"n"(kSelStages - 2) : "memory");
       __syncwarp();  // the oldest stage is there for the whole warp, and the one before it free
       issue();
       if (done == sent) break;
-      const int st = done % kSelStages, e0 = (first + done * nw) * 16;
-      ++done;
-      const uint32_t at = ring_a + st * 2 * Sm::kTile;
-      const int mrow = lane & 15, mchunk = lane >> 4;
+      const uint32_t at = ring_a + stage * 2 * Sm::kTile;
       uint32_t x[2][D / 32][4];  // lo, hi: the A operand of every 32 channels
 #pragma unroll
       for (int k = 0; k < D / 32; ++k) {
-        ldmatrix4(x[0][k], at + tile_at<D>(mrow, 2 * k + mchunk));
-        ldmatrix4(x[1][k], at + Sm::kTile + tile_at<D>(mrow, 2 * k + mchunk));
+        ldmatrix4(x[0][k], at + tile_at<D>(lane & 15, 2 * k + (lane >> 4)));
+        ldmatrix4(x[1][k], at + Sm::kTile + tile_at<D>(lane & 15, 2 * k + (lane >> 4)));
       }
       int best0 = INT32_MIN, best1 = INT32_MIN;
-      for (int ht = 0; ht < nht; ++ht) {
+      const auto heads = [&](int ht, const uint32_t (&q)[2][D / 16]) {
         int acc[2][4] = {};
-        const uint32_t* f = qf + (ht * 2) * (D / 16) * 32 + lane;
 #pragma unroll
         for (int k = 0; k < D / 32; ++k)
 #pragma unroll
           for (int h = 0; h < 2; ++h)
-            mma_s8(acc[h], x[h][k][0], x[h][k][1], x[h][k][2], x[h][k][3], f[(h * (D / 16) + 2 * k) * 32],
-                   f[(h * (D / 16) + 2 * k + 1) * 32]);
+            mma_s8(acc[h], x[h][k][0], x[h][k][1], x[h][k][2], x[h][k][3], q[h][2 * k], q[h][2 * k + 1]);
         const int head = ht * 8 + 2 * t;
         if (head < c.rep) { best0 = max(best0, acc[0][0] + acc[1][0]); best1 = max(best1, acc[0][2] + acc[1][2]); }
         if (head + 1 < c.rep) { best0 = max(best0, acc[0][1] + acc[1][1]); best1 = max(best1, acc[0][3] + acc[1][3]); }
+      };
+      heads(0, q1);
+      for (int ht = 1; ht < nht; ++ht) {
+        uint32_t q[2][D / 16];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) q[h][k] = qf[((ht * 2 + h) * (D / 16) + k) * 32 + lane];
+        heads(ht, q);
       }
       best0 = max(best0, __shfl_xor_sync(0xffffffffu, best0, 1));
       best1 = max(best1, __shfl_xor_sync(0xffffffffu, best1, 1));
@@ -623,22 +644,23 @@ __global__ void __launch_bounds__(kSelThreads, 2) k_cache_select(const CacheDev 
       best1 = max(best1, __shfl_xor_sync(0xffffffffu, best1, 2));
       // lane l < 16 takes block e0 + l, whose row is the quad g = l % 8's
       const int v0 = __shfl_sync(0xffffffffu, best0, (lane & 7) * 4), v1 = __shfl_sync(0xffffffffu, best1, (lane & 7) * 4);
-      const int blk = e0 + lane;
+      const int blk = (first + done * nw) * 16 + lane;
       if (lane < 16 && blk < here) {
         unsigned long long k = 0;
-        const unsigned char* meta = sm + Sm::kMeta + (w * kSelStages + st) * 128 + lane * 4;
-        if (*reinterpret_cast<const int*>(meta + 64) >= 0) {
+        if (*reinterpret_cast<const int*>(meta + stage * 128 + 64) >= 0) {
           if (blk < c.sink || blk >= here - c.local) {
             k = ~0ull;
             ++my_forced;
           } else {
-            k = order_key((double)(lane < 8 ? v0 : v1) * (double)*reinterpret_cast<const float*>(meta));
+            k = order_key((double)(lane < 8 ? v0 : v1) * (double)*reinterpret_cast<const float*>(meta + stage * 128));
             my_lo = min(my_lo, k);
             my_hi = max(my_hi, k);
           }
         }
         asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(keys0 + blk * 8), "l"(k) : "memory");
       }
+      ++done;
+      stage = stage == kSelStages - 1 ? 0 : stage + 1;
     }
     __syncwarp();
 #pragma unroll
@@ -799,18 +821,8 @@ cudaError_t run_select(const CacheDev& c, cudaStream_t st) {
     const cudaError_t e = cudaFuncSetAttribute(k_cache_select<DT, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
   }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)grid);
-  cfg.blockDim = dim3(kSelThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = ranks;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, k_cache_select<DT, D>, c);
+  CacheLaunch l((unsigned)grid, kSelThreads, smem, st, ranks);
+  const cudaError_t e = cudaLaunchKernelEx(&l.cfg, k_cache_select<DT, D>, c);
   note_launch();
   return e;
 }
@@ -825,17 +837,8 @@ cudaError_t run_select_d(const CacheDev& c, cudaStream_t st) {
 
 cudaError_t launch_cache_reserve(const ReserveDev& r, cudaStream_t st) {
   const bool many = r.B > 64;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(many ? kReserveCluster : 1);
-  cfg.blockDim = dim3(many ? kReserveThreads : 256);
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = cfg.gridDim.x;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, k_cache_reserve, r);
+  CacheLaunch l(many ? kReserveCluster : 1, many ? kReserveThreads : 256, 0, st, many ? kReserveCluster : 1);
+  const cudaError_t e = cudaLaunchKernelEx(&l.cfg, k_cache_reserve, r);
   note_launch();
   return e;
 }

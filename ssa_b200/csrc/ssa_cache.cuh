@@ -7,10 +7,39 @@
 
 namespace ssa {
 
+// Every kernel here is launched while the one before it in the stream may
+// still run, and waits for its end -- with it everything that one waited for
+// -- before it reads anything; then it lets the next one come up. Loads are
+// plain ones: a read-only load might be moved above the wait.
+__device__ __forceinline__ void grid_wait() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+// Launch attributes of these kernels: programmatic dependency on the launch
+// before, and a cluster size.
+struct CacheLaunch {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at[2];
+  CacheLaunch(unsigned grid, unsigned threads, size_t smem, cudaStream_t st, unsigned cluster = 1) {
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = cluster;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+  }
+};
+
 // Tokens of sequence b's current step (q rows / appended tokens that count).
 __device__ __forceinline__ int cache_step_tokens(const CacheDev& c, int b, int& start, int& len) {
-  start = __ldg(c.start + b);
-  len = __ldg(c.lens + b);
+  start = c.start[b];
+  len = c.lens[b];
   const int64_t cap = (int64_t)c.max_blocks * c.bs;
   if (start < 0 || len < 0) { start = 0; len = 0; }
   if (len > cap) len = (int)cap;
@@ -22,8 +51,17 @@ __device__ __forceinline__ int cache_step_tokens(const CacheDev& c, int b, int& 
 // page numbers outside the pool are left out instead of being dereferenced.
 __device__ __forceinline__ int cache_page(const CacheDev& c, int b, int blk) {
   if (blk < 0 || blk >= c.max_blocks) return -1;
-  const int page = __ldg(c.table + (int64_t)b * c.max_blocks + blk);
+  const int page = c.table[(int64_t)b * c.max_blocks + blk];
   return (unsigned)page < (unsigned)c.num_pages ? page : -1;
+}
+
+// The same in two steps, for a look-up ahead: the table's entry, and the
+// check, made only where the entry is used (it waits for the load).
+__device__ __forceinline__ int cache_entry(const CacheDev& c, int b, int blk) {
+  return blk >= 0 && blk < c.max_blocks ? c.table[(int64_t)b * c.max_blocks + blk] : -1;
+}
+__device__ __forceinline__ int cache_checked(const CacheDev& c, int entry) {
+  return (unsigned)entry < (unsigned)c.num_pages ? entry : -1;
 }
 
 // A staged tile: 16 key rows of D code bytes, as 16-byte chunks exchanged

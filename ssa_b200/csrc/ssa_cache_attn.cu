@@ -98,9 +98,9 @@ struct Raw4 {
   uint4 u;
   __device__ __forceinline__ void zero() { u = make_uint4(0, 0, 0, 0); }
   __device__ __forceinline__ void load(const void* row, int i) {
-    if constexpr (F32) u = __ldg(reinterpret_cast<const uint4*>(static_cast<const float*>(row) + i));
+    if constexpr (F32) u = *reinterpret_cast<const uint4*>(static_cast<const float*>(row) + i);
     else {
-      const uint2 v = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(row) + i));
+      const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(row) + i);
       u.x = v.x;
       u.y = v.y;
     }
@@ -147,6 +147,52 @@ struct Ranges {
   __device__ __forceinline__ int of(int x) const {  // the block whose range holds group x
     const int first = more * (each + 1);
     return x < first ? (int)((unsigned)x / (unsigned)(each + 1)) : more + (int)((unsigned)(x - first) / (unsigned)each);
+  }
+};
+
+// This thread block's range, and the sequence it begins in: up to as many
+// sequences as threads take one scan of their work. Block 0 leaves the work
+// before each sequence, and all of it, in `prefix`.
+struct RangeSmem {
+  int sum[32], scan[32], b, base;
+};
+struct BlockRange {
+  int lo, hi, b, base;
+  template <class Work>
+  __device__ __forceinline__ BlockRange(int B, int32_t* prefix, RangeSmem& s, const Work& work) {
+    const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, threads = blockDim.x, nw = threads >> 5;
+    const int mine0 = tid < B ? work(tid) : 0;
+    int sum = mine0;
+    for (int i = tid + threads; i < B; i += threads) sum += work(i);
+    sum = __reduce_add_sync(0xffffffffu, sum);
+    if (lane == 0) s.sum[w] = sum;
+    __syncthreads();
+    const int total = __reduce_add_sync(0xffffffffu, lane < nw ? s.sum[lane] : 0);
+    const Ranges rg(total, gridDim.x);
+    lo = rg.begin(min((int)blockIdx.x, rg.nblk));
+    hi = (int)blockIdx.x < rg.nblk ? rg.begin(blockIdx.x + 1) : lo;
+    int before = 0;
+    for (int b0 = 0; b0 < B; b0 += threads) {
+      const int mine = b0 == 0 ? mine0 : b0 + tid < B ? work(b0 + tid) : 0;
+      int upto = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += x;
+      }
+      if (b0) __syncthreads();
+      if (lane == 31) s.scan[w] = upto;
+      __syncthreads();
+      const int x = lane < nw ? s.scan[lane] : 0;
+      const int from = before + upto - mine + __reduce_add_sync(0xffffffffu, lane < w ? x : 0);
+      if (lo >= from && lo < from + mine) { s.b = b0 + tid; s.base = from; }
+      if (prefix && blockIdx.x == 0 && b0 + tid < B) prefix[b0 + tid] = from;
+      before += __reduce_add_sync(0xffffffffu, x);
+    }
+    if (prefix && blockIdx.x == 0 && tid == 0) prefix[B] = total;
+    __syncthreads();
+    b = s.b;
+    base = s.base;
   }
 };
 
@@ -201,68 +247,18 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, 8 * NT)) k_cache_at
   uint2* qf = reinterpret_cast<uint2*>(sm + Sm::kQ);
   float* sml = reinterpret_cast<float*>(sm + Sm::kMl);
   float* srow = reinterpret_cast<float*>(sm + Sm::kScale);
-  __shared__ int red[kWarps], red2[kWarps];
-  __shared__ int s_base, s_b;
+  __shared__ RangeSmem rs;
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t = lane & 3;
   const int bs_shift = c.bs == 16 ? 4 : c.bs == 32 ? 5 : 6;
-  asm volatile("griddepcontrol.launch_dependents;");  // k_cache_combine may take its place and wait
-
-  // this block's range of the work, and the sequence it starts in
-  int total;
-  if (c.blocks) {
-    const int per = c.n * pl.tiles_max * c.n_kv * pl.list_groups;
-    total = c.B * per;
-    if (tid == 0) {
-      const Ranges rg(total, gridDim.x);
-      const int at = rg.begin(min((int)blockIdx.x, rg.nblk));
-      s_b = (int)((unsigned)at / (unsigned)per);
-      s_base = s_b * per;
-    }
-  } else {
-    // up to 128 sequences: one scan gives the total and finds the sequence
+  grid_wait();  // k_cache_combine may take its place behind it
+  const BlockRange br(c.B, c.prefix, rs, [&](int i) {
     int tiles, groups;
-    const int mine0 = tid < c.B ? seq_work(c, pl, tid, ROWS, &tiles, &groups) : 0;
-    int sum = mine0;
-    for (int b = tid + kThreads; b < c.B; b += kThreads) sum += seq_work(c, pl, b, ROWS, &tiles, &groups);
-    sum = __reduce_add_sync(0xffffffffu, sum);
-    if (lane == 0) red[w] = sum;
-    __syncthreads();
-    total = 0;
-#pragma unroll
-    for (int i = 0; i < kWarps; ++i) total += red[i];
-    const Ranges rg(total, gridDim.x);
-    const int at = rg.begin(min((int)blockIdx.x, rg.nblk));
-    int before = 0;
-    for (int b0 = 0; b0 < c.B; b0 += kThreads) {
-      const int mine = b0 == 0 ? mine0 : b0 + tid < c.B ? seq_work(c, pl, b0 + tid, ROWS, &tiles, &groups) : 0;
-      int upto = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int x = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += x;
-      }
-      if (b0) __syncthreads();
-      if (lane == 31) red2[w] = upto;
-      __syncthreads();
-      int all = 0;
-#pragma unroll
-      for (int i = 0; i < kWarps; ++i) {
-        if (i < w) upto += red2[i];
-        all += red2[i];
-      }
-      const int from = before + upto - mine;
-      if (at >= from && at < from + mine) { s_b = b0 + tid; s_base = from; }
-      if (blockIdx.x == 0 && b0 + tid < c.B) c.prefix[b0 + tid] = from;
-      before += all;
-    }
-    if (blockIdx.x == 0 && tid == 0) c.prefix[c.B] = total;
-  }
-  __syncthreads();
-  const Ranges rg(total, gridDim.x);
-  if ((int)blockIdx.x >= rg.nblk) return;
-  const int lo = rg.begin(blockIdx.x), hi = rg.begin(blockIdx.x + 1);
+    return seq_work(c, pl, i, ROWS, &tiles, &groups);
+  });
+  const int lo = br.lo, hi = br.hi;
+  if (lo >= hi) return;
 
-  int b = s_b, base = s_base;
+  int b = br.b, base = br.base;
   for (int at = lo; at < hi;) {
     int tiles, groups;
     const int mine = seq_work(c, pl, b, ROWS, &tiles, &groups);
@@ -293,30 +289,31 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, 8 * NT)) k_cache_at
     // holds the page of group s0 + l, and of group s0 + 32 + l (loaded ahead).
     unsigned char* ring = sm + w * Sm::kWarp;
     const uint32_t ring_a = smem_addr(ring), meta_a = smem_addr(sm + Sm::kMeta + w * kStages * 16);
-    int page, kb, off, page_n, kb_n, off_n;
-    const auto look_up = [&](int s0, int& pg, int& first, int& o) {
-      pg = -1;
+    int page, kb, off, entry_n, kb_n, off_n;
+    const auto look_up = [&](int s0, int& entry, int& first, int& o) {
+      entry = -1;
       if (s0 + lane < g1) {
         const int64_t key = (int64_t)(s0 + lane) * kGroup + w * 16;
-        const int entry = (int)(key >> bs_shift);
+        const int e = (int)(key >> bs_shift);
         o = (int)key & (c.bs - 1);
-        const int blk = !x.list ? entry : entry < c.top ? __ldg(x.list + entry) : -1;
+        const int blk = !x.list ? e : e < c.top ? x.list[e] : -1;
         if (blk >= 0 && blk < c.max_blocks) {
           first = blk * c.bs + o;
-          if (first < lim_max) pg = cache_page(c, x.b, blk);
+          if (first < lim_max) entry = cache_entry(c, x.b, blk);
         }
       }
     };
     int s0 = g0;
     look_up(s0, page, kb, off);
-    look_up(s0 + 32, page_n, kb_n, off_n);
+    look_up(s0 + 32, entry_n, kb_n, off_n);
+    page = cache_checked(c, page);
     uint32_t todo = __ballot_sync(0xffffffffu, page >= 0);
     int issued = 0, used = 0;
     const auto issue = [&]() {
       while (!todo && s0 + 32 < g1) {
         s0 += 32;
-        page = page_n; kb = kb_n; off = off_n;
-        look_up(s0 + 32, page_n, kb_n, off_n);
+        page = cache_checked(c, entry_n); kb = kb_n; off = off_n;
+        look_up(s0 + 32, entry_n, kb_n, off_n);
         todo = __ballot_sync(0xffffffffu, page >= 0);
       }
       if (todo) {
@@ -567,9 +564,11 @@ __global__ void __launch_bounds__(kThreads) k_cache_combine(const CacheDev c, co
   constexpr int ROWS = 8 * NT, E = D / 32;
   const int lane = threadIdx.x & 31;
   const unsigned id = blockIdx.x * kWarps + (threadIdx.x >> 5);
-  // Every warp waits, so that this kernel's end implies the other's.
+  // k_cache_attn lets this kernel come up only after its own wait, so lengths
+  // may be read before this one's. Every warp waits: this kernel's end then
+  // implies the other's.
   if (id >= (unsigned)nrows) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    grid_wait();
     return;
   }
   const int per = pl.tiles_max * (c.blocks ? c.n : 1);  // row tiles a (sequence, kv head) can have
@@ -595,7 +594,7 @@ __global__ void __launch_bounds__(kThreads) k_cache_combine(const CacheDev c, co
     total = __reduce_add_sync(0xffffffffu, total);
     base = __reduce_add_sync(0xffffffffu, base);
   }
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  grid_wait();
   if (r >= (c.blocks ? c.rep - tile % pl.tiles_max * ROWS : c.n * c.rep - x.row0)) return;
   float m = kEmpty, l = 0.f, o[E];
 #pragma unroll
@@ -687,22 +686,15 @@ cudaError_t run_attn(const CacheDev& c, const Plan& pl, cudaStream_t st) {
   if (e != cudaSuccess) return e;
   const int64_t units = units_of(c, pl);
   if (units > 0x7fffffff) return cudaErrorInvalidConfiguration;
-  k_cache_attn<D, NT, F32><<<c.grid, kThreads, smem, st>>>(c, pl);
-  note_launch();
-  if ((e = cudaGetLastError()) != cudaSuccess) return e;
   const int rows_used = (int)((c.blocks ? c.rep : (int64_t)c.n * c.rep) < ROWS ? (c.blocks ? c.rep : c.n * c.rep) : ROWS);
   const int64_t nrows = units * rows_used;
   if (nrows > 0x7fffffff - kWarps) return cudaErrorInvalidConfiguration;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((nrows + kWarps - 1) / kWarps));
-  cfg.blockDim = dim3(kThreads);
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, k_cache_combine<D, NT, F32>, c, pl, c.grid, rows_used, (int)nrows);
+  CacheLaunch main(c.grid, kThreads, smem, st);
+  e = cudaLaunchKernelEx(&main.cfg, k_cache_attn<D, NT, F32>, c, pl);
+  note_launch();
+  if (e != cudaSuccess) return e;
+  CacheLaunch join((unsigned)((nrows + kWarps - 1) / kWarps), kThreads, 0, st);
+  e = cudaLaunchKernelEx(&join.cfg, k_cache_combine<D, NT, F32>, c, pl, c.grid, rows_used, (int)nrows);
   note_launch();
   return e;
 }
