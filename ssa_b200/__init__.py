@@ -20,10 +20,11 @@ from .attention import (  # noqa: F401
     measure_cross_layer_overlap,
     CachedGraphSparseTransformer,
 )
+from .cache import BlockCache  # noqa: F401  (serving; no counterpart in the reference)
 
 __all__ = [
     "SSAConfig", "SubquadraticRegimeTracker", "WindowGraphBuilder", "GlobalGraphBuilder",
     "LSHGraphBuilder", "merge_neighbors", "sparse_gather_attention", "SparseAttention",
     "SparseTransformerLayer", "SparseTransformer", "neighbor_overlap",
-    "measure_cross_layer_overlap", "CachedGraphSparseTransformer",
+    "measure_cross_layer_overlap", "CachedGraphSparseTransformer", "BlockCache",
 ]

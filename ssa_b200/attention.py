@@ -26,6 +26,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import ops
+from .cache import BlockCache
 
 
 # ---------------------------------------------------------------------------
@@ -434,6 +435,49 @@ class SparseAttention(nn.Module):
         return out_proj, stats
 
 
+    # -- serving (no counterpart in the reference) ----------------------------
+    def cached_blocks(self, block_size: int) -> Tuple[int, int]:
+        """Blocks every step attends whatever their bound: the leading ones up to
+        the last global token (sink), and those the window reaches back to from
+        the token's own (local)."""
+        idx = self.config.global_token_indices
+        G = self.config.num_global_tokens if idx is None else max(idx, default=-1) + 1
+        return -(-max(G, 0) // block_size), 1 + -(-self.config.window_size // block_size)
+
+    @torch.no_grad()
+    def prefill(self, x: torch.Tensor, cache: BlockCache, layer: int = 0) -> torch.Tensor:
+        """`forward` of a prompt x (B, N, d_model) over its sparse graph, storing
+        its keys and values as the step's tokens: call `cache.reserve(N)` before
+        (once for all layers). Returns (B, N, d_model)."""
+        B, N, _ = x.shape
+        q = self._split_q(self.Wq(x))
+        k = self._split_kv_grouped(self.Wk(x))
+        v = self._split_kv_grouped(self.Wv(x))
+        cache.append(k, v, layer)
+        nb, valid = self._graph(q, k, N, self.config.causal, False)
+        out = ops.gather_attention(q, k, v, nb, valid, self.scale, self.config.fp32_attn_weights)
+        return self.Wo(out.transpose(1, 2).reshape(B, N, self.H * self.d_head))
+
+    @torch.no_grad()
+    def step(self, x: torch.Tensor, cache: BlockCache, layer: int = 0) -> torch.Tensor:
+        """Attention of the step's tokens x (B, n, d_model) over the cached
+        sequence up to each token: every block, or with `cache.top_blocks` the
+        global tokens' and the window's blocks and those of the highest bound of
+        q.k up to that number. Call `cache.reserve(n)` before (once for all
+        layers). Rows behind a sequence's new tokens come from zero attention."""
+        if not self.config.causal:
+            raise ValueError("SparseAttention.step needs config.causal=True: a token cannot attend what is not there yet")
+        B, n, _ = x.shape
+        q = self._split_q(self.Wq(x))
+        cache.append(self._split_kv_grouped(self.Wk(x)), self._split_kv_grouped(self.Wv(x)), layer)
+        blocks = None
+        if cache.top_blocks is not None:
+            sink, local = self.cached_blocks(cache.block_size)
+            blocks = cache.select(q, layer, sink=sink, local=local)
+        out = cache.attend(q, self.scale, layer, blocks)
+        return self.Wo(out.transpose(1, 2).reshape(B, n, self.H * self.d_head))
+
+
 # ---------------------------------------------------------------------------
 # Transformer stacks (sparse_attention.py:1517-1550, :1688-1792)
 # ---------------------------------------------------------------------------
@@ -453,6 +497,13 @@ class SparseTransformerLayer(nn.Module):
         a, stats = self.attn(self.norm1(x), return_stats=return_stats)
         return x + a + self.ff(self.norm2(x + a)), stats
 
+    @torch.no_grad()
+    def step(self, x, cache: BlockCache, layer: int = 0, prompt: bool = False):
+        """The block over the step's tokens (SparseAttention.step, or for a
+        whole prompt SparseAttention.prefill)."""
+        a = (self.attn.prefill if prompt else self.attn.step)(self.norm1(x), cache, layer)
+        return x + a + self.ff(self.norm2(x + a))
+
 
 class SparseTransformer(nn.Module):
     def __init__(self, config: SSAConfig, num_layers: int = 6, vocab_size: int = 0):
@@ -469,6 +520,35 @@ class SparseTransformer(nn.Module):
             x, stats = layer(x, return_stats=return_stats)
             stats_list.append(stats)
         return self.norm(x), stats_list
+
+    def new_cache(self, batch: int, max_tokens: int, *, block_size: int = 64, num_blocks: Optional[int] = None,
+                  top_blocks: Optional[int] = None) -> BlockCache:
+        """A BlockCache for this model's layers, heads, dtype and device."""
+        attn, w = self.layers[0].attn, self.norm.weight
+        return BlockCache(batch, attn.n_kv, attn.d_head, max_tokens, num_layers=len(self.layers), block_size=block_size,
+                          num_blocks=num_blocks, top_blocks=top_blocks, dtype=w.dtype, device=w.device)
+
+    @torch.no_grad()
+    def prefill(self, x, cache: BlockCache) -> torch.Tensor:
+        """`forward` of the prompts x ((B, N) ids or (B, N, d_model)) of an empty
+        cache, over the sparse graph, filling the cache. Returns (B, N, d_model)."""
+        return self._cached(x, cache, x.shape[1], True)
+
+    @torch.no_grad()
+    def step(self, x, cache: BlockCache, new_lens: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """The model over the next tokens of every sequence, x (B, n) ids or
+        (B, n, d_model), reading and extending `cache`. new_lens (B,) int32: how
+        many of a row's n tokens are real (the others' outputs mean nothing).
+        Returns (B, n, d_model)."""
+        return self._cached(x, cache, x.shape[1] if new_lens is None else new_lens, False)
+
+    def _cached(self, x, cache, new_lens, prompt):
+        if self.embed is not None:
+            x = self.embed(x)
+        cache.reserve(new_lens)
+        for i, layer in enumerate(self.layers):
+            x = layer.step(x, cache, i, prompt)
+        return self.norm(x)
 
 
 def neighbor_overlap(neighbors_a: torch.Tensor, neighbors_b: torch.Tensor,

@@ -99,3 +99,25 @@ def test_reserve_reference():
     assert (start, lens, state) == ([0, 16, 5], [17, 17, 16], [0, 0])
     assert table == [[3, 2], [9, 1], [9, 9]]
     assert R.reserve([0, 0, 16], [17, 16, 0], [[9] * 2] * 3, [1, 2], [1, 0], 16)[1:3] == ([0, 0, 16], [1, 2])
+
+
+def test_block_cache_refusals():
+    from ssa_b200 import BlockCache
+    for bad, err in ((dict(batch=0), ValueError), (dict(block_size=24), NotImplementedError), (dict(head_dim=48), NotImplementedError),
+                     (dict(dtype=torch.float16), NotImplementedError), (dict(top_blocks=0), ValueError), (dict(device="cpu"), RuntimeError)):
+        kw = {**dict(batch=1, num_kv_heads=1, head_dim=64, max_tokens=64), **bad}
+        with pytest.raises(err):
+            BlockCache(**kw)
+
+
+def test_cached_blocks():
+    import warnings
+    from ssa_b200 import SSAConfig, SparseAttention
+    with warnings.catch_warnings():
+        warnings.simplefilter("ignore")
+        for kw, want in ((dict(num_global_tokens=2, window_size=8), (1, 2)), (dict(num_global_tokens=0, window_size=0), (0, 1)),
+                         (dict(num_global_tokens=33, window_size=16), (3, 2)),
+                         (dict(global_token_indices=[0, 40], window_size=17), (3, 3)),
+                         (dict(global_token_indices=[], window_size=1), (0, 2))):
+            attn = SparseAttention(SSAConfig(d_model=64, num_heads=2, num_neighbors=64, **kw))
+            assert attn.cached_blocks(16) == want, kw
