@@ -26,9 +26,9 @@ OBJ_DIR = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "libssa_b200.so")
 TORCH_LIB = os.path.join(PKG, "_ssa_torch.so")
 SOURCES = ["ssa_graph.cu", "ssa_select_tc.cu", "ssa_hash_tc.cu", "ssa_select_rows.cu", "ssa_attn.cu", "ssa_cache.cu",
-           "ssa_cache_attn.cu", "ssa_capi.cu"]
+           "ssa_cache_attn.cu", "ssa_cache_prompt.cu", "ssa_capi.cu"]
 HEADERS = ["ssa_common.cuh", "ssa_internal.h", "ssa_select_common.cuh", "ssa_tcgen05.cuh",
-           "ssa_cache.cuh"]
+           "ssa_cache.cuh", "ssa_cache_attn.cuh"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
          "--expt-relaxed-constexpr"]

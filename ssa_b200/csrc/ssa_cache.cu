@@ -145,17 +145,6 @@ __device__ __forceinline__ float quantize_near_half(float x, float r, float f, f
   return (d > 0.f ? h + 0.5f : d < 0.f ? h - 0.5f : h) + kRound;
 }
 
-__device__ __forceinline__ unsigned long long f2_add(unsigned long long a, unsigned long long b) {
-  unsigned long long d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ unsigned long long f2_mul(unsigned long long a, unsigned long long b) {
-  unsigned long long d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-
 // Four codes of x as bytes; r: the codes as floats, in pairs. inv = 0: all zero.
 __device__ __forceinline__ uint32_t quantize4(const float4& x, float inv, float amax, unsigned long long (&r)[2]) {
   const unsigned long long i2 = f2_pack(inv, inv), up = f2_pack(kRound, kRound), down = f2_pack(-kRound, -kRound);

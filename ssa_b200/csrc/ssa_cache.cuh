@@ -36,6 +36,17 @@ struct CacheLaunch {
   }
 };
 
+__device__ __forceinline__ unsigned long long f2_add(unsigned long long a, unsigned long long b) {
+  unsigned long long d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ unsigned long long f2_mul(unsigned long long a, unsigned long long b) {
+  unsigned long long d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
 // Tokens of sequence b's current step (q rows / appended tokens that count).
 __device__ __forceinline__ int cache_step_tokens(const CacheDev& c, int b, int& start, int& len) {
   start = c.start[b];

@@ -19,26 +19,13 @@
 // units and cut into one equal range for each thread block, so ragged batches
 // balance; a unit that spans several blocks leaves its partial sums in the
 // workspace and k_cache_combine joins them in range order.
-#include <cuda_fp16.h>
-#include <math.h>
-
-#include "ssa_cache.cuh"
+#include "ssa_cache_attn.cuh"
 
 namespace ssa {
 
 namespace {
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
-constexpr int kGroup = 64;       // keys a block takes at a time: 16 for each warp
-constexpr float kEmpty = -1e30f; // offset of a row that has seen no key
-constexpr float kHead = 13.f;    // weights run up to 2^13, and 2^15 before the offset moves
-constexpr float kSlack = 2.f;
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -50,19 +37,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
-}
-
-// Codes (biased by 128) in bytes SEL picks -> two fp16: 0x6400 | u is 1024 + u.
-template <int SEL>
-__device__ __forceinline__ uint32_t codes_f16(uint32_t biased) {
-  const uint32_t h = __byte_perm(biased, 0x64646464u, SEL);
-  const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&h), __half2half2(__ushort_as_half(0x6480)));
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
-
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-  const __half2 v = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
 }
 
 // High part and remainder of a pair.
@@ -88,156 +62,6 @@ struct Smem {
   static constexpr int kQ = kScale + 8 * NT * 4;                         // [F32 ? 2 : 1][NT][D / 16][32] uint2
   static constexpr int kBytes = kQ + (F32 ? 2 : 1) * NT * (D / 16) * 32 * 8;
 };
-// Blocks that share an SM (registers for 16 and 32 rows, the rings for 8).
-constexpr int blocks_per_sm(int d, int rows) { return rows == 32 ? 2 : rows == 16 || d >= 96 ? 3 : 4; }
-
-// Four elements as they lie in memory: widened where they are used, so that
-// a load does not wait where it is issued.
-template <bool F32>
-struct Raw4 {
-  uint4 u;
-  __device__ __forceinline__ void zero() { u = make_uint4(0, 0, 0, 0); }
-  __device__ __forceinline__ void load(const void* row, int i) {
-    if constexpr (F32) u = *reinterpret_cast<const uint4*>(static_cast<const float*>(row) + i);
-    else {
-      const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(row) + i);
-      u.x = v.x;
-      u.y = v.y;
-    }
-  }
-  __device__ __forceinline__ float4 f() const {
-    if constexpr (F32) return make_float4(__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w));
-    else
-      return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
-                         __uint_as_float(u.y & 0xffff0000u));
-  }
-};
-
-// Units and work of the call. Without a list a unit is (sequence, kv head,
-// tile of query rows) and its work the sequence's groups of 64 keys; with one
-// it is (sequence, token, kv head, tile of heads) and its work the list's.
-struct Plan {
-  int rows, tiles_max, list_groups;
-};
-
-__device__ __forceinline__ int seq_work(const CacheDev& c, const Plan& pl, int b, int rows, int* tiles, int* groups) {
-  if (c.blocks) {
-    *tiles = c.n * pl.tiles_max;
-    *groups = pl.list_groups;
-  } else {
-    int start, len;
-    const int fresh = cache_step_tokens(c, b, start, len);
-    *tiles = (fresh * c.rep + rows - 1) / rows;
-    *groups = (len + kGroup - 1) / kGroup;
-  }
-  return *tiles * c.n_kv * *groups;
-}
-
-// Equal ranges of the work: block i of `nblk` takes [begin(i), begin(i + 1)),
-// one group more in the first `more`. With less work than blocks the first
-// `total` get one group each, so that no range between two of a unit's is empty.
-struct Ranges {
-  int nblk, each, more;
-  __device__ __forceinline__ Ranges(int total, int grid) {
-    nblk = total < grid ? total : grid;
-    each = nblk ? (int)((unsigned)total / (unsigned)nblk) : 0;
-    more = total - each * nblk;
-  }
-  __device__ __forceinline__ int begin(int i) const { return i * each + (i < more ? i : more); }
-  __device__ __forceinline__ int of(int x) const {  // the block whose range holds group x
-    const int first = more * (each + 1);
-    return x < first ? (int)((unsigned)x / (unsigned)(each + 1)) : more + (int)((unsigned)(x - first) / (unsigned)each);
-  }
-};
-
-// This thread block's range, and the sequence it begins in: up to as many
-// sequences as threads take one scan of their work. Block 0 leaves the work
-// before each sequence, and all of it, in `prefix`.
-struct RangeSmem {
-  int sum[32], scan[32], b, base;
-};
-struct BlockRange {
-  int lo, hi, b, base;
-  template <class Work>
-  __device__ __forceinline__ BlockRange(int B, int32_t* prefix, RangeSmem& s, const Work& work) {
-    const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, threads = blockDim.x, nw = threads >> 5;
-    const int mine0 = tid < B ? work(tid) : 0;
-    int sum = mine0;
-    for (int i = tid + threads; i < B; i += threads) sum += work(i);
-    sum = __reduce_add_sync(0xffffffffu, sum);
-    if (lane == 0) s.sum[w] = sum;
-    __syncthreads();
-    const int total = __reduce_add_sync(0xffffffffu, lane < nw ? s.sum[lane] : 0);
-    const Ranges rg(total, gridDim.x);
-    lo = rg.begin(min((int)blockIdx.x, rg.nblk));
-    hi = (int)blockIdx.x < rg.nblk ? rg.begin(blockIdx.x + 1) : lo;
-    int before = 0;
-    for (int b0 = 0; b0 < B; b0 += threads) {
-      const int mine = b0 == 0 ? mine0 : b0 + tid < B ? work(b0 + tid) : 0;
-      int upto = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int x = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += x;
-      }
-      if (b0) __syncthreads();
-      if (lane == 31) s.scan[w] = upto;
-      __syncthreads();
-      const int x = lane < nw ? s.scan[lane] : 0;
-      const int from = before + upto - mine + __reduce_add_sync(0xffffffffu, lane < w ? x : 0);
-      if (lo >= from && lo < from + mine) { s.b = b0 + tid; s.base = from; }
-      if (prefix && blockIdx.x == 0 && b0 + tid < B) prefix[b0 + tid] = from;
-      before += __reduce_add_sync(0xffffffffu, x);
-    }
-    if (prefix && blockIdx.x == 0 && tid == 0) prefix[B] = total;
-    __syncthreads();
-    b = s.b;
-    base = s.base;
-  }
-};
-
-struct Unit {
-  int b, kv, tile, start, len, fresh, row0, nrows;  // row0: its first query row, of nrows valid ones
-  const int32_t* list;
-};
-
-template <int ROWS>
-__device__ __forceinline__ Unit unit_of(const CacheDev& c, const Plan& pl, int b, int u, int tiles) {
-  Unit x;
-  x.b = b;
-  x.fresh = cache_step_tokens(c, b, x.start, x.len);
-  x.kv = u / tiles;
-  x.tile = u - x.kv * tiles;
-  x.list = nullptr;
-  if (c.blocks) {
-    const int tok = x.tile / pl.tiles_max, ht = x.tile - tok * pl.tiles_max;
-    x.row0 = tok * c.rep + ht * ROWS;
-    x.nrows = tok < x.fresh ? min(ROWS, c.rep - ht * ROWS) : 0;
-    x.list = c.blocks + (((int64_t)b * c.n + tok) * c.n_kv + x.kv) * c.top;
-  } else {
-    x.row0 = x.tile * ROWS;
-    x.nrows = min(ROWS, x.fresh * c.rep - x.row0);
-  }
-  return x;
-}
-
-// A unit's final rows (or zeros): row r of the tile is token (row0 + r) / rep
-// and the group's head (row0 + r) % rep.
-template <bool F32>
-__device__ __forceinline__ void store_out(const CacheDev& c, const Unit& x, int r, int ch, float4 o) {
-  const int row = x.row0 + r, tok = row / c.rep, h = x.kv * c.rep + row - tok * c.rep;
-  const int64_t at = x.b * c.o_sb + h * c.o_sh + tok * c.o_sn + ch;
-  if constexpr (F32) *reinterpret_cast<float4*>(static_cast<float*>(c.out) + at) = o;
-  else
-    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(c.out) + at) =
-        make_uint2(f32_to_bf16_bits(o.x) | (uint32_t)f32_to_bf16_bits(o.y) << 16,
-                   f32_to_bf16_bits(o.z) | (uint32_t)f32_to_bf16_bits(o.w) << 16);
-}
-__device__ __forceinline__ void store_lse(const CacheDev& c, const Unit& x, int r, float m, float l) {
-  const int row = x.row0 + r, tok = row / c.rep, h = x.kv * c.rep + row - tok * c.rep;
-  c.lse[((int64_t)x.b * c.H + h) * c.n + tok] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
-}
-
 template <int D, int NT, bool F32>
 __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, 8 * NT)) k_cache_attn(const CacheDev c, const Plan pl) {
   using Sm = Smem<D, NT, F32>;
@@ -251,7 +75,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, 8 * NT)) k_cache_at
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t = lane & 3;
   const int bs_shift = c.bs == 16 ? 4 : c.bs == 32 ? 5 : 6;
   grid_wait();  // k_cache_combine may take its place behind it
-  const BlockRange br(c.B, c.prefix, rs, [&](int i) {
+  const BlockRange br(c.B, c.prefix, least_groups(ROWS), rs, [&](int i) {
     int tiles, groups;
     return seq_work(c, pl, i, ROWS, &tiles, &groups);
   });
@@ -431,7 +255,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, 8 * NT)) k_cache_at
 
       // weights 2^(s' + log2(step_v) - m + 13)
       const float vs = va > 0.f ? va : 1.f;  // a page of zeros: any step does
-      const float lv = F32 ? log2f(vs) : __log2f(vs), iv = 1.f / vs;
+      const float lv = (F32 ? log2f(vs) : __log2f(vs)) + (va != va ? va : 0.f), iv = 1.f / vs;
       const bool edge = kbj + 16 > lim_min;
       bool move = false;
 #pragma unroll
@@ -605,12 +429,12 @@ __global__ void __launch_bounds__(kThreads) k_cache_combine(const CacheDev c, co
       base = c.prefix[b];
     }
     const int ubeg = base + (kv * tiles + tile) * groups;
-    const Ranges rg(total, ngrid);
+    const Ranges rg(total, ngrid, least_groups(ROWS));
     const int c0 = rg.of(ubeg), c1 = rg.of(ubeg + groups - 1);
     if (c0 == c1) return;  // that block stored the row
     const auto slot = [&](int k) { return ((int64_t)k * 2 + (k == c0)) * ROWS + r; };
     // the first sums are under way while their weights are found
-    constexpr int kAhead = 4;
+    constexpr int kAhead = 8;
     float first[kAhead][E];
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
@@ -642,7 +466,7 @@ __global__ void __launch_bounds__(kThreads) k_cache_combine(const CacheDev c, co
             for (int i = 0; i < E; ++i) o[i] = fmaf(fj, first[j][i], o[i]);
         }
       }
-#pragma unroll 4
+#pragma unroll 8
       for (; j < cnt; ++j) {
         const float fj = __shfl_sync(0xffffffffu, f, j);
         const float* p = c.part_o + slot(k0 + j) * D + lane;
@@ -660,9 +484,11 @@ __global__ void __launch_bounds__(kThreads) k_cache_combine(const CacheDev c, co
   if (lane == 0 && c.lse) store_lse(c, x, r, m, l);
 }
 
-// Rows of a tile: 8, 16 or 32 (the rows a group has, as far as they go).
+// Rows of a tile: 8, 16 or 32 (the rows a group has, as far as they go), or
+// 128 on the 5th-generation tensor cores.
 int tile_rows(const CacheDev& c) {
   const int64_t rows = c.blocks ? c.rep : (int64_t)c.n * c.rep;
+  if (rows >= kPromptMin && !c.blocks && c.dtype == kDtBF16) return kPromptRows;
   return rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
 }
 
@@ -679,29 +505,38 @@ int64_t units_of(const CacheDev& c, const Plan& p) {
 }
 
 template <int D, int NT, bool F32>
-cudaError_t run_attn(const CacheDev& c, const Plan& pl, cudaStream_t st) {
+cudaError_t run_combine(const CacheDev& c, const Plan& pl, cudaStream_t st) {
   constexpr int ROWS = 8 * NT;
-  constexpr size_t smem = Smem<D, NT, F32>::kBytes;
-  cudaError_t e = cudaFuncSetAttribute(k_cache_attn<D, NT, F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e != cudaSuccess) return e;
   const int64_t units = units_of(c, pl);
   if (units > 0x7fffffff) return cudaErrorInvalidConfiguration;
   const int rows_used = (int)((c.blocks ? c.rep : (int64_t)c.n * c.rep) < ROWS ? (c.blocks ? c.rep : c.n * c.rep) : ROWS);
   const int64_t nrows = units * rows_used;
   if (nrows > 0x7fffffff - kWarps) return cudaErrorInvalidConfiguration;
+  CacheLaunch join((unsigned)((nrows + kWarps - 1) / kWarps), kThreads, 0, st);
+  const cudaError_t e = cudaLaunchKernelEx(&join.cfg, k_cache_combine<D, NT, F32>, c, pl, c.grid, rows_used, (int)nrows);
+  note_launch();
+  return e;
+}
+
+template <int D, int NT, bool F32>
+cudaError_t run_attn(const CacheDev& c, const Plan& pl, cudaStream_t st) {
+  constexpr size_t smem = Smem<D, NT, F32>::kBytes;
+  cudaError_t e = cudaFuncSetAttribute(k_cache_attn<D, NT, F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return e;
   CacheLaunch main(c.grid, kThreads, smem, st);
   e = cudaLaunchKernelEx(&main.cfg, k_cache_attn<D, NT, F32>, c, pl);
   note_launch();
-  if (e != cudaSuccess) return e;
-  CacheLaunch join((unsigned)((nrows + kWarps - 1) / kWarps), kThreads, 0, st);
-  e = cudaLaunchKernelEx(&join.cfg, k_cache_combine<D, NT, F32>, c, pl, c.grid, rows_used, (int)nrows);
-  note_launch();
-  return e;
+  return e != cudaSuccess ? e : run_combine<D, NT, F32>(c, pl, st);
 }
 
 template <int D, bool F32>
 cudaError_t run_attn_rows(const CacheDev& c, cudaStream_t st) {
   const Plan pl = plan_of(c);
+  if constexpr (!F32)
+    if (pl.rows == kPromptRows) {
+      const cudaError_t e = launch_cache_prompt(c, pl, st);
+      return e != cudaSuccess ? e : run_combine<D, kPromptRows / 8, false>(c, pl, st);
+    }
   return pl.rows == 8 ? run_attn<D, 1, F32>(c, pl, st) : pl.rows == 16 ? run_attn<D, 2, F32>(c, pl, st)
                                                                        : run_attn<D, 4, F32>(c, pl, st);
 }

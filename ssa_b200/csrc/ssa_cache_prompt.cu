@@ -1,0 +1,462 @@
+// ssa_cache_prompt.cu -- attention over the 8-bit block cache for many query
+// rows (a prompt's chunk, drafts of a multi-query model), on the
+// 5th-generation tensor cores.
+//
+// The mathematics is k_cache_attn's (ssa_cache_attn.cu); with 64 rows and more
+// a kv head the products bound it, and turning codes into fp16 once for every
+// 32 rows. Here 128 rows share the conversion:
+//   warps 4-7 load the codes of 64 keys a block of steps ahead, convert them
+//             to fp16 and store K and V as swizzled 128-byte rows (two stages);
+//   warp 8    issues S = Q K^T (128 x 64 x d, fp32 in TMEM) for the next keys,
+//             then O += P V (128 x d x 64) with P in TMEM and V key-major, as
+//             it lies;
+//   warps 0-3 own a row a thread: read S, mask, move the row's offset when a
+//             score outgrows it, and write P = 2^(s - m) as fp16 to TMEM.
+// Two thread blocks share an SM, so one's products run under the other's
+// exponentials: 64 keys take a block 512 cycles of tensor pipe, as many of the
+// exponential unit, and about 500 of issue.
+#include "ssa_cache_attn.cuh"
+#include "ssa_tcgen05.cuh"
+
+namespace ssa {
+
+using namespace tc;
+
+int read_cache_error(int clear) { return tc_read_error(clear); }
+
+namespace {
+
+constexpr int kSoftWarps = 4, kConvWarps = 4, kThreads = (kSoftWarps + kConvWarps + 1) * 32;
+constexpr int kConvThreads = kConvWarps * 32;
+// Registers: the launch's 96 a thread (9 warps, two blocks an SM) are dealt out
+// as 72 to the 128 converting threads and 120 to the 128 with a row:
+// 128 * 72 + 128 * 120 + 32 * 96 = 288 * 96.
+constexpr uint32_t kTmemCols = 256, kColP = 64, kColO = 128;  // S at 0
+constexpr uint32_t kWaitLimit = 1u << 24;
+
+template <int D>
+struct PromptSmem {
+  static constexpr int kAtoms = (D + 63) / 64;                         // 64 channels: rows of 128 bytes
+  static constexpr int kQ = 0;                                         // [kAtoms][128 rows][128 bytes]
+  static constexpr int kTile = kAtoms * 64 * 128;                      // [kAtoms][64 keys][128 bytes]
+  static constexpr int kKV = kAtoms * kPromptRows * 128;               // [2 stages][K, V] tiles
+  static constexpr int kMeta = kKV + 4 * kTile;                        // [2 stages][4] {step_k, log2 step_v, 1 / step_v, -}
+  static constexpr int kBars = kMeta + 2 * 4 * 16;
+  static constexpr int kBytes = kBars + 128 + 1024;                    // the base is rounded up to 1024
+};
+
+// fp16 A and B, fp32 sums, M x N; B key-major or (transposed) channel-major.
+constexpr uint32_t idesc_f16(int m, int n, bool b_transposed) {
+  return (1u << 4) | (b_transposed ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+
+// V's operand: the product's N (channels) runs along the 128-byte rows, its K
+// (keys) down them: 64-channel atoms `atom` bytes apart, groups of 8 keys 1024.
+__device__ __forceinline__ uint64_t desc_channels_inner(uint32_t saddr, uint32_t atom) {
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(atom >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) |
+         ((uint64_t)1u << 46) | ((uint64_t)2u << 61);
+}
+
+// D (+)= A B with A in TMEM.
+__device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(b), "r"(idesc), "r"(acc));
+}
+
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
+      "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]),
+      "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// The units of a thread block's range, one after the other (every warp walks
+// them for itself).
+struct Segments {
+  int at, hi, b, base;
+  __device__ __forceinline__ Segments(const BlockRange& r) : at(r.lo), hi(r.hi), b(r.b), base(r.base) {}
+  __device__ __forceinline__ bool next(const CacheDev& c, const Plan& pl, Unit& x, int& g0, int& g1, int& groups) {
+    while (at < hi) {
+      int tiles;
+      const int mine = seq_work(c, pl, b, kPromptRows, &tiles, &groups);
+      if (at >= base + mine) { base += mine; ++b; continue; }
+      const int u = (int)((unsigned)(at - base) / (unsigned)groups), ubeg = base + u * groups, uend = ubeg + groups;
+      g0 = at - ubeg;
+      g1 = min(hi, uend) - ubeg;
+      at = ubeg + g1;
+      x = unit_of<kPromptRows>(c, pl, b, u, tiles);
+      return true;
+    }
+    return false;
+  }
+};
+
+// Keys a row of the tile sees: at most `lim_max`; groups of 64 a segment has to visit.
+__device__ __forceinline__ int lim_max_of(const CacheDev& c, const Unit& x) {
+  return c.causal ? x.start + (x.row0 + x.nrows - 1) / c.rep + 1 : x.len;
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, const Plan pl) {
+  using Sm = PromptSmem<D>;
+  extern __shared__ __align__(16) unsigned char raw[];
+  unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+  float4* meta = reinterpret_cast<float4*>(sm + Sm::kMeta);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + Sm::kBars);
+  uint64_t *kfull = bars, *vfull = bars + 2, *kvempty = bars + 4, *sfull = bars + 6, *sempty = bars + 7, *pfull = bars + 8,
+           *odone = bars + 9, *qfull = bars + 10, *mma_done = bars + 11;
+  __shared__ RangeSmem rs;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_flag_s;
+  volatile int* abort_flag = &abort_flag_s;
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+  grid_wait();
+  const BlockRange br(c.B, c.prefix, least_groups(kPromptRows), rs, [&](int i) {
+    int tiles, groups;
+    return seq_work(c, pl, i, kPromptRows, &tiles, &groups);
+  });
+  if (br.lo >= br.hi) return;
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(kfull + i, kConvWarps);
+      mbar_init(vfull + i, kConvWarps);
+      mbar_init(kvempty + i, 1);
+    }
+    mbar_init(sfull, 1);
+    mbar_init(sempty, kSoftWarps);
+    mbar_init(pfull, kSoftWarps);
+    mbar_init(odone, 1);
+    mbar_init(qfull, kSoftWarps);
+    mbar_init(mma_done, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (w == kSoftWarps + kConvWarps) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(kTmemCols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  Segments seg(br);
+  Unit x;
+  int g0, g1, groups;
+  int it = 0;  // blocks of 64 keys so far, the same count in every role
+
+  if (w >= kSoftWarps && w < kSoftWarps + kConvWarps) {
+    // ------------------------------------------------------------ codes to fp16
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    const int ct = tid - kSoftWarps * 32;
+    const int bs_shift = c.bs == 16 ? 4 : c.bs == 32 ? 5 : 6;
+    constexpr int kLoads = D / 32;  // 16-byte pieces of a tile's codes a thread has
+    bool ok = true;
+    while (ok && seg.next(c, pl, x, g0, g1, groups)) {
+      const int lim_max = lim_max_of(c, x);
+      const int ge = min(g1, (lim_max + 63) / 64);
+      // lane l: the table's entry for keys 16 (l % 4) .. of a block
+      const auto entry = [&](int gr) {
+        const int key = gr * 64 + (lane & 3) * 16;
+        return gr < ge && key < lim_max ? cache_entry(c, x.b, key >> bs_shift) : -1;
+      };
+      const auto load = [&](const int8_t* codes, int gr, int pages, uint4 (&r)[kLoads]) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+          const int id = i * kConvThreads + ct, row = id / (D / 16), part = id % (D / 16), sub = row >> 4;
+          const int64_t pg = max(__shfl_sync(0xffffffffu, pages, sub), 0);
+          const int off = (gr * 64 + sub * 16) & (c.bs - 1);
+          r[i] = *reinterpret_cast<const uint4*>(codes + (((pg * c.n_kv + x.kv) * c.bs + off + (row & 15)) * D + part * 16));
+        }
+      };
+      const auto store = [&](unsigned char* tile, const uint4 (&r)[kLoads]) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+          const int id = i * kConvThreads + ct, row = id / (D / 16), part = id % (D / 16);
+          const uint32_t w4[4] = {r[i].x ^ 0x80808080u, r[i].y ^ 0x80808080u, r[i].z ^ 0x80808080u, r[i].w ^ 0x80808080u};
+          uint4 h[2];
+          h[0] = make_uint4(codes_f16<0x4140>(w4[0]), codes_f16<0x4342>(w4[0]), codes_f16<0x4140>(w4[1]), codes_f16<0x4342>(w4[1]));
+          h[1] = make_uint4(codes_f16<0x4140>(w4[2]), codes_f16<0x4342>(w4[2]), codes_f16<0x4140>(w4[3]), codes_f16<0x4342>(w4[3]));
+          unsigned char* at = tile + (part >> 2) * (64 * 128) + row * 128;
+          // chunks 2 part, 2 part + 1 of the row; every other group of four lanes the second one first, for the banks
+          const int first = (part >> 2) & 1, c0 = (part & 3) * 2;
+          *reinterpret_cast<uint4*>(at + (((c0 + first) ^ (row & 7)) << 4)) = first ? h[1] : h[0];
+          *reinterpret_cast<uint4*>(at + (((c0 + 1 - first) ^ (row & 7)) << 4)) = first ? h[0] : h[1];
+        }
+      };
+      int pages = cache_checked(c, entry(g0)), ahead = entry(g0 + 1);
+      uint4 kr[kLoads], vr[kLoads];
+      float2 am = make_float2(0.f, 0.f);
+      const auto load_amax = [&](int pg) {
+        return w == kSoftWarps && lane < 4 && pg >= 0
+                   ? *(reinterpret_cast<const float2*>(c.amax) + (int64_t)pg * c.n_kv + x.kv) : make_float2(0.f, 0.f);
+      };
+      if (g0 < ge) {
+        load(c.k_codes, g0, pages, kr);
+        am = load_amax(pages);
+        load(c.v_codes, g0, pages, vr);
+      }
+      for (int gr = g0; gr < ge; ++gr, ++it) {
+        const int st = it & 1;
+        unsigned char* tile = sm + Sm::kKV + st * 2 * Sm::kTile;
+        if (!(ok = mbar_wait_warp(kvempty + st, ((it >> 1) & 1) ^ 1, abort_flag, 31, kWaitLimit))) break;
+        if (w == kSoftWarps && lane < 4) {
+          const float va = am.y * (1.f / 127.f), vs = va > 0.f ? va : 1.f;
+          // keys without a page: scores of minus infinity; a page of NaN: scores of NaN
+          meta[st * 4 + lane] = pages >= 0 ? make_float4(am.x * (1.f / 127.f), __log2f(vs) + (va != va ? va : 0.f), 1.f / vs, 0.f)
+                                           : make_float4(0.f, -INFINITY, 0.f, 0.f);
+        }
+        pages = cache_checked(c, ahead);
+        ahead = entry(gr + 2);
+        store(tile, kr);
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(kfull + st);
+        if (gr + 1 < ge) {
+          load(c.k_codes, gr + 1, pages, kr);
+          am = load_amax(pages);
+        }
+        store(tile + Sm::kTile, vr);
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(vfull + st);
+        if (gr + 1 < ge) load(c.v_codes, gr + 1, pages, vr);
+      }
+    }
+  } else if (w == kSoftWarps + kConvWarps) {
+    // ------------------------------------------------------------ products
+    if (lane == 0) {
+      const uint32_t qa = smem_u32(sm + Sm::kQ), kva = smem_u32(sm + Sm::kKV);
+      constexpr uint32_t kDescS = idesc_f16(kPromptRows, 64, false), kDescO = idesc_f16(kPromptRows, D, true);
+      bool ok = true;
+      int segs = 0;
+      const auto scores = [&](int i) {
+        const int st = i & 1;
+        if (!mbar_wait(kfull + st, (i >> 1) & 1, abort_flag, 32, kWaitLimit)) return false;
+        if (i && !mbar_wait(sempty, (i - 1) & 1, abort_flag, 33, kWaitLimit)) return false;
+        tc_fence_after();
+        const uint32_t ka = kva + st * 2 * Sm::kTile;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk)
+          umma_bf16(tmem, umma_desc(qa + (kk >> 2) * (kPromptRows * 128) + (kk & 3) * 32),
+                    umma_desc(ka + (kk >> 2) * (64 * 128) + (kk & 3) * 32), kDescS, kk > 0);
+        umma_commit(sfull);
+        return true;
+      };
+      while (ok && seg.next(c, pl, x, g0, g1, groups)) {
+        const int nb = min(g1, (lim_max_of(c, x) + 63) / 64) - g0;
+        if (nb <= 0) continue;
+        ok = mbar_wait(qfull, segs++ & 1, abort_flag, 34, kWaitLimit) && scores(it);
+        for (int j = 0; ok && j < nb; ++j, ++it) {
+          const int st = it & 1;
+          if (j + 1 < nb && !(ok = scores(it + 1))) break;
+          ok = mbar_wait(vfull + st, (it >> 1) & 1, abort_flag, 35, kWaitLimit) && mbar_wait(pfull, it & 1, abort_flag, 36, kWaitLimit);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t va = kva + (st * 2 + 1) * Sm::kTile;
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            umma_ts(tmem + kColO, tmem + kColP + kk * 8, desc_channels_inner(va + kk * 16 * 128, 64 * 128), kDescO, (j | kk) > 0);
+          umma_commit(kvempty + st);
+          umma_commit(odone);
+        }
+      }
+      // Products still in flight (also after a wait that ran out) end before TMEM is freed.
+      umma_commit(mma_done);
+      mbar_drain(mma_done, 0);
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------ a row a thread
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 120;");
+    const int r = tid;
+    const uint32_t trow = tmem + ((uint32_t)(w * 32) << 16);
+    bool ok = true;
+    while (ok && seg.next(c, pl, x, g0, g1, groups)) {
+      const bool have = r < x.nrows;
+      const int nb = min(g1, (lim_max_of(c, x) + 63) / 64) - g0;
+      const int lim_min = c.causal ? x.start + x.row0 / c.rep + 1 : x.len;
+      const int row = x.row0 + (have ? r : 0), tok = row / c.rep, h = x.kv * c.rep + row - tok * c.rep;
+      const int lim = !have ? INT32_MAX : c.causal ? x.start + tok + 1 : x.len;
+      float m = kEmpty, l = 0.f;
+      if (nb > 0) {
+        // Q, scaled into fp16's range by a power of two; the scale's sign goes with it
+        const uint16_t* qr = static_cast<const uint16_t*>(c.q) + x.b * c.q_sb + h * c.q_sh + tok * c.q_sn;
+        const auto piece = [&](int i) {
+          return have ? *reinterpret_cast<const uint2*>(qr + i * 4) : make_uint2(0u, 0u);
+        };
+        uint32_t top = 0;  // |q| as integers; the row is read twice rather than kept
+#pragma unroll 8
+        for (int i = 0; i < D / 4; ++i) {
+          const uint2 u = piece(i);
+          top = max(top, max(max((u.x << 16) & 0x7fffffffu, u.x & 0x7fff0000u), max((u.y << 16) & 0x7fffffffu, u.y & 0x7fff0000u)));
+        }
+        int e = 9 - ((int)(top >> 23) - 127);
+        e = top >= 0x7f800000u ? 0 : min(e, 100);
+        const float up0 = __uint_as_float((uint32_t)(e + 127) << 23), down = __uint_as_float((uint32_t)(127 - e) << 23);
+        const float up = c.scale < 0.f ? -up0 : up0;
+        const float sfac = fabsf(c.scale) * 1.4426950408889634f * down;
+#pragma unroll 4
+        for (int i = 0; i < D / 8; ++i) {
+          uint32_t o[4];
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const uint2 u = piece(2 * i + k);
+            o[2 * k] = pack_f16(__uint_as_float(u.x << 16) * up, __uint_as_float(u.x & 0xffff0000u) * up);
+            o[2 * k + 1] = pack_f16(__uint_as_float(u.y << 16) * up, __uint_as_float(u.y & 0xffff0000u) * up);
+          }
+          *reinterpret_cast<uint4*>(sm + Sm::kQ + (i >> 3) * (kPromptRows * 128) + r * 128 + (((i & 7) ^ (r & 7)) << 4)) =
+              make_uint4(o[0], o[1], o[2], o[3]);
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(qfull);
+
+        for (int j = 0; j < nb; ++j, ++it) {
+          const int st = it & 1, key0 = (g0 + j) * 64;
+          if (!(ok = mbar_wait_warp(kfull + st, (it >> 1) & 1, abort_flag, 37, kWaitLimit))) break;  // the steps
+          float4 mt[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) mt[k] = meta[st * 4 + k];
+          if (!(ok = mbar_wait_warp(sfull, it & 1, abort_flag, 38, kWaitLimit))) break;
+          tc_fence_after();
+          float s[64];
+          tmem_ld32(trow, s);
+          tmem_ld32(trow + 32, s + 32);
+          tmem_wait_ld();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(sempty);
+
+          float mx = -INFINITY;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float f = mt[k].x * sfac;
+            const unsigned long long f2 = f2_pack(f, f), a2 = f2_pack(mt[k].y, mt[k].y);
+#pragma unroll
+            for (int i = 0; i < 16; i += 2)
+              f2_unpack(f2_fma(f2_pack(s[k * 16 + i], s[k * 16 + i + 1]), f2, a2), s[k * 16 + i], s[k * 16 + i + 1]);
+          }
+          if (key0 + 64 > lim_min) {
+#pragma unroll
+            for (int i = 0; i < 64; ++i)
+              if (key0 + i >= lim) s[i] = -INFINITY;
+          }
+#pragma unroll
+          for (int i = 0; i < 64; ++i) mx = fmaxf(mx, s[i]);
+          const bool move = mx > m + (kHead + kSlack);
+          float f = 1.f;
+          if (__any_sync(0xffffffffu, move)) {
+            const float mn = fmaxf(m, mx - kHead);
+            f = ex2(m - mn);
+            m = mn;
+            l *= f;
+          }
+          // weights, fp16; the sum before the rounding
+          uint32_t p[32];
+          const float nm = -m;
+          const unsigned long long n2 = f2_pack(nm, nm);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+              float a, e2;
+              f2_unpack(f2_add(f2_pack(s[k * 16 + i], s[k * 16 + i + 1]), n2), a, e2);
+              a = ex2(a);
+              e2 = ex2(e2);
+              sum0 += a;
+              sum1 += e2;
+              p[k * 8 + i / 2] = pack_f16(a, e2);
+            }
+            l = fmaf(sum0 + sum1, mt[k].z, l);
+          }
+          if (j > 0) {
+            // the product before has read P and added to O
+            if (!(ok = mbar_wait_warp(odone, (it - 1) & 1, abort_flag, 39, kWaitLimit))) break;
+            tc_fence_after();
+            if (__any_sync(0xffffffffu, f != 1.f)) {
+#pragma unroll 1
+              for (int ch = 0; ch < D; ch += 32) {
+                float o[32];
+                uint32_t u[32];
+                tmem_ld32(trow + kColO + ch, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) u[i] = __float_as_uint(o[i] * f);
+                tmem_st32(trow + kColO + ch, u);
+              }
+            }
+          }
+          tmem_st32(trow + kColP, p);
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(pfull);
+        }
+        if (ok) {
+          ok = mbar_wait_warp(odone, (it - 1) & 1, abort_flag, 40, kWaitLimit);
+          tc_fence_after();
+        }
+      }
+      if (!ok) break;
+      const bool full = g0 == 0 && g1 == groups;
+      const int64_t slot = ((int64_t)blockIdx.x * 2 + (g0 == 0)) * kPromptRows + r;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll 1
+      for (int ch = 0; ch < D; ch += 32) {
+        float o[32];
+        if (nb > 0) {
+          tmem_ld32(trow + kColO + ch, o);
+          tmem_wait_ld();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0.f;
+        }
+        if (!have) continue;
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+          if (full) store_out<false>(c, x, r, ch + i, make_float4(o[i] * inv, o[i + 1] * inv, o[i + 2] * inv, o[i + 3] * inv));
+          else *reinterpret_cast<float4*>(c.part_o + slot * D + ch + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+        }
+      }
+      tc_fence_before();
+      if (have) {
+        if (!full) *reinterpret_cast<float2*>(c.part_ml + slot * 2) = make_float2(m, l);
+        else if (c.lse) store_lse(c, x, r, m, l);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (w == kSoftWarps + kConvWarps)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
+}
+
+template <int D>
+cudaError_t run_prompt(const CacheDev& c, const Plan& pl, cudaStream_t st) {
+  constexpr size_t smem = PromptSmem<D>::kBytes;
+  const cudaError_t e = cudaFuncSetAttribute(k_cache_prompt<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return e;
+  CacheLaunch l((unsigned)c.grid, kThreads, smem, st);
+  const cudaError_t e2 = cudaLaunchKernelEx(&l.cfg, k_cache_prompt<D>, c, pl);
+  note_launch();
+  return e2;
+}
+
+}  // namespace
+
+cudaError_t launch_cache_prompt(const CacheDev& c, const Plan& pl, cudaStream_t st) {
+  return c.d == 32 ? run_prompt<32>(c, pl, st) : c.d == 64 ? run_prompt<64>(c, pl, st)
+         : c.d == 96 ? run_prompt<96>(c, pl, st) : run_prompt<128>(c, pl, st);
+}
+
+}  // namespace ssa

@@ -114,6 +114,7 @@ size_t hash_tc_planes_bytes(const GraphDev& g);
 cudaError_t launch_hash_planes(const GraphDev& g, cudaStream_t st);
 cudaError_t launch_hash_tc(const GraphDev& g, bool keys, cudaStream_t st);
 int read_hash_tc_error(int clear);
+int read_cache_error(int clear);
 // Fused QKV projection + hash (self-attention, bf16): out[rows][n_out] =
 // x[rows][dm] w[n_out][dm]^T, with the graph's hash state written into its
 // workspace (g.q / g.k are views of out).

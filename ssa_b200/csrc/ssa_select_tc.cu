@@ -601,8 +601,9 @@ cudaError_t launch_select_tc(const GraphDev& g, int mode, cudaStream_t st) {
 int read_device_error(int clear) {
   const int a = tc_read_error(clear);
   const int b = read_hash_tc_error(clear);
-  if (a < 0 || b < 0) return -1;
-  return a ? a : b;
+  const int c = read_cache_error(clear);
+  if (a < 0 || b < 0 || c < 0) return -1;
+  return a ? a : b ? b : c;
 }
 
 }  // namespace ssa

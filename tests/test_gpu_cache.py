@@ -282,6 +282,11 @@ ATTENDS = [  # dtype, H, n_kv, d, bs, n, lens after the step
     (BF, 8, 8, 32, 16, 70, [300, 70, 75]),
     (BF, 16, 2, 128, 64, 19, [200, 1, 64]),
     (F32, 12, 4, 128, 32, 11, [64, 100]),
+    # 64 rows a kv head and more: the many-row kernel
+    (BF, 6, 2, 96, 32, 40, [200, 41, 0]),
+    (BF, 32, 1, 128, 16, 5, [1000, 5, 64]),
+    (BF, 4, 2, 64, 64, 300, [1100, 300, 17]),
+    (BF, 2, 1, 32, 32, 33, [65, 2000]),
 ]
 
 
@@ -380,14 +385,14 @@ def test_attention_skips_blocks_without_a_page(case, cuda):
     _check_attention(pool, q, out, lse, 0.2)
 
 
-@pytest.mark.parametrize("dtype,d", [(BF, 128), (F32, 64)])
-def test_attention_sharp_and_far_scores(dtype, d, cuda):
+@pytest.mark.parametrize("dtype,d,rep", [(BF, 128, 4), (F32, 64, 4), (BF, 64, 72)])
+def test_attention_sharp_and_far_scores(dtype, d, rep, cuda):
     """Scores that grow along the cache (the running offset moves all the way),
     a single dominating key, and pages of very different steps, one of zeros."""
     n_kv, bs, L = 1, 16, 400
     g = torch.Generator().manual_seed(9)
     k, v = _kv(g, 1, L, n_kv, d, dtype, cuda), _kv(g, 1, L, n_kv, d, dtype, cuda)
-    q = _kv(g, 1, 1, 4, d, dtype, cuda)
+    q = _kv(g, 1, 1, rep, d, dtype, cuda)
     ramp = torch.linspace(-40, 40, L, device=cuda).view(1, 1, L, 1)
     k1 = (q[:, :1, :1] * ramp / (q[:, :1, :1].float() ** 2).sum() * d ** 0.5).to(dtype)
     steps = (2.0 ** torch.randint(-30, 30, (L // bs,), generator=g).double()).float().repeat_interleave(bs).to(cuda)
@@ -402,19 +407,21 @@ def test_attention_sharp_and_far_scores(dtype, d, cuda):
         _check_attention(pool, q, out, lse, d ** -0.5)
 
 
-def test_attention_keeps_nan_and_infinity_where_they_are(cuda):
-    """A sequence with a NaN page or an infinite q gives NaN; the others, and
-    stale pages behind a length, do not see it."""
+@pytest.mark.parametrize("rep", [2, 64])
+@pytest.mark.parametrize("bad,value", [("k", math.nan), ("k", math.inf), ("v", math.nan), ("v", -math.inf)])
+def test_attention_keeps_nan_and_infinity_where_they_are(bad, value, rep, cuda):
+    """A sequence with a page of NaN or infinity or an infinite q gives NaN; the
+    others, and stale pages behind a length, do not see it."""
     n_kv, d, bs = 1, 64, 16
     g = torch.Generator().manual_seed(2)
     pool = Pool(cuda, 3, n_kv, d, bs, 4, BF)
     k, v = _kv(g, 3, 40, n_kv, d, BF, cuda), _kv(g, 3, 40, n_kv, d, BF, cuda)
-    k[1, 0, 20, 3] = math.nan
+    (k if bad == "k" else v)[1, 0, 20, 3] = value
     pool.advance([40, 40, 40])
     pool.append(k, v)
     pool.amax[pool.table[:, 3].long()] = math.nan  # behind every length
     pool.start = pool.lens - 1
-    q = _kv(g, 3, 1, 2, d, BF, cuda)
+    q = _kv(g, 3, 1, rep, d, BF, cuda)
     q[2, 1, 0, 5] = math.inf
     out, lse = pool.attend(q, 0.125, want_lse=True)
     assert torch.isnan(out[1]).all() and torch.isnan(out[2, 1]).all()
