@@ -283,37 +283,45 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
       const bool have = r < x.nrows;
       const int nb = min(g1, (lim_max_of(c, x) + 63) / 64) - g0;
       const int lim_min = c.causal ? x.start + x.row0 / c.rep + 1 : x.len;
-      const int row = x.row0 + (have ? r : 0), tok = row / c.rep, h = x.kv * c.rep + row - tok * c.rep;
+      const int row = x.row0 + (have ? r : 0), tok = row / c.rep, hd = x.kv * c.rep + row - tok * c.rep;
       const int lim = !have ? INT32_MAX : c.causal ? x.start + tok + 1 : x.len;
+      // this thread's row in q and out (rows behind the last one: the first, never stored)
+      const int64_t q_at = x.b * c.q_sb + hd * c.q_sh + tok * c.q_sn, o_at = x.b * c.o_sb + hd * c.o_sh + tok * c.o_sn;
       float m = kEmpty, l = 0.f;
       if (nb > 0) {
-        // Q, scaled into fp16's range by a power of two; the scale's sign goes with it
-        const uint16_t* qr = static_cast<const uint16_t*>(c.q) + x.b * c.q_sb + h * c.q_sh + tok * c.q_sn;
-        const auto piece = [&](int i) {
-          return have ? *reinterpret_cast<const uint2*>(qr + i * 4) : make_uint2(0u, 0u);
-        };
-        uint32_t top = 0;  // |q| as integers; the row is read twice rather than kept
+        // Q: rows into their swizzled places as they come, 8 bytes a lane, then
+        // each thread turns its own into fp16 where it lies, scaled by a power of
+        // two; the scale's sign goes with it.
+        const char* q0 = static_cast<const char*>(c.q) + lane * 8;
+        const uint32_t qs = smem_u32(sm + Sm::kQ) + (lane >> 4) * (kPromptRows * 128) + (lane & 1) * 8;
 #pragma unroll 8
-        for (int i = 0; i < D / 4; ++i) {
-          const uint2 u = piece(i);
-          top = max(top, max(max((u.x << 16) & 0x7fffffffu, u.x & 0x7fff0000u), max((u.y << 16) & 0x7fffffffu, u.y & 0x7fff0000u)));
+        for (int i = 0; i < 32; ++i) {
+          const int64_t at = __shfl_sync(0xffffffffu, q_at, i);
+          const int rr = w * 32 + i;
+          if (lane < D / 4) copy8(qs + rr * 128 + ((((lane >> 1) & 7) ^ (rr & 7)) << 4), q0 + at * 2);
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        __syncwarp();
+        unsigned char* mine = sm + Sm::kQ + r * 128;
+        const auto piece = [&](int i) {
+          return reinterpret_cast<uint4*>(mine + (i >> 3) * (kPromptRows * 128) + (((i & 7) ^ (r & 7)) << 4));
+        };
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          const uint4 u = *piece(i);
+          top = max(top, max(max(max((u.x << 16) & 0x7fffffffu, u.x & 0x7fff0000u), max((u.y << 16) & 0x7fffffffu, u.y & 0x7fff0000u)),
+                             max(max((u.z << 16) & 0x7fffffffu, u.z & 0x7fff0000u), max((u.w << 16) & 0x7fffffffu, u.w & 0x7fff0000u))));
         }
         int e = 9 - ((int)(top >> 23) - 127);
         e = top >= 0x7f800000u ? 0 : min(e, 100);
-        const float up0 = __uint_as_float((uint32_t)(e + 127) << 23), down = __uint_as_float((uint32_t)(127 - e) << 23);
-        const float up = c.scale < 0.f ? -up0 : up0;
-        const float sfac = fabsf(c.scale) * 1.4426950408889634f * down;
+        const float up0 = __uint_as_float((uint32_t)(e + 127) << 23), up = c.scale < 0.f ? -up0 : up0;
+        const float sfac = fabsf(c.scale) * 1.4426950408889634f * __uint_as_float((uint32_t)(127 - e) << 23);
+        const auto half2 = [&](uint32_t u) { return pack_f16(__uint_as_float(u << 16) * up, __uint_as_float(u & 0xffff0000u) * up); };
 #pragma unroll 4
         for (int i = 0; i < D / 8; ++i) {
-          uint32_t o[4];
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const uint2 u = piece(2 * i + k);
-            o[2 * k] = pack_f16(__uint_as_float(u.x << 16) * up, __uint_as_float(u.x & 0xffff0000u) * up);
-            o[2 * k + 1] = pack_f16(__uint_as_float(u.y << 16) * up, __uint_as_float(u.y & 0xffff0000u) * up);
-          }
-          *reinterpret_cast<uint4*>(sm + Sm::kQ + (i >> 3) * (kPromptRows * 128) + r * 128 + (((i & 7) ^ (r & 7)) << 4)) =
-              make_uint4(o[0], o[1], o[2], o[3]);
+          const uint4 u = *piece(i);
+          *piece(i) = make_uint4(half2(u.x), half2(u.y), half2(u.z), half2(u.w));
         }
         fence_async_smem();
         __syncwarp();
@@ -408,7 +416,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
       }
       if (!ok) break;
       const bool full = g0 == 0 && g1 == groups;
-      const int64_t slot = ((int64_t)blockIdx.x * 2 + (g0 == 0)) * kPromptRows + r;
+      const int64_t slot = ((int64_t)blockIdx.x * 2 + (g0 == 0)) * kPromptRows;
       const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll 1
       for (int ch = 0; ch < D; ch += 32) {
@@ -421,15 +429,22 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
           for (int i = 0; i < 32; ++i) o[i] = 0.f;
         }
         if (!have) continue;
+        if (full) {
+          uint16_t* to = static_cast<uint16_t*>(c.out) + o_at + ch;
 #pragma unroll
-        for (int i = 0; i < 32; i += 4) {
-          if (full) store_out<false>(c, x, r, ch + i, make_float4(o[i] * inv, o[i + 1] * inv, o[i + 2] * inv, o[i + 3] * inv));
-          else *reinterpret_cast<float4*>(c.part_o + slot * D + ch + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          for (int i = 0; i < 32; i += 4)
+            *reinterpret_cast<uint2*>(to + i) =
+                make_uint2(f32_to_bf16_bits(o[i] * inv) | (uint32_t)f32_to_bf16_bits(o[i + 1] * inv) << 16,
+                           f32_to_bf16_bits(o[i + 2] * inv) | (uint32_t)f32_to_bf16_bits(o[i + 3] * inv) << 16);
+        } else {
+          float* to = c.part_o + (slot + r) * D + ch;
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(to + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
         }
       }
       tc_fence_before();
       if (have) {
-        if (!full) *reinterpret_cast<float2*>(c.part_ml + slot * 2) = make_float2(m, l);
+        if (!full) *reinterpret_cast<float2*>(c.part_ml + (slot + r) * 2) = make_float2(m, l);
         else if (c.lse) store_lse(c, x, r, m, l);
       }
     }
