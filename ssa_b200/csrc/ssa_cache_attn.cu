@@ -379,15 +379,21 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, 8 * NT)) k_cache_at
   }
 }
 
-// One warp for each query row: joins the partial sums of a unit that several
-// blocks worked on, in range order, and writes zeros to rows without work. It
-// is launched while k_cache_attn still runs and waits for it behind its set-up.
-template <int D, int NT, bool F32>
+// Joins the partial sums of a query row that several blocks worked on, and
+// writes zeros to rows without work. PARTS warps share a row's sums, each in
+// range order and then one after the other: one where there are many rows,
+// four where few rows have many sums (one sequence of 16384 tokens, two kv
+// heads: 74 sums a row). The kernel is launched while the other still runs
+// and waits for it behind its set-up.
+template <int D, int NT, bool F32, int PARTS>
 __global__ void __launch_bounds__(kThreads) k_cache_combine(const CacheDev c, const Plan pl, const int ngrid,
                                                             const int rows_used, const int nrows) {
   constexpr int ROWS = 8 * NT, E = D / 32;
-  const int lane = threadIdx.x & 31;
-  const unsigned id = blockIdx.x * kWarps + (threadIdx.x >> 5);
+  constexpr int kDt = F32 ? kDtF32 : kDtBF16;
+  __shared__ float s_ml[PARTS][2], s_o[PARTS][D];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int part = PARTS == 1 ? 0 : w;
+  const unsigned id = PARTS == 1 ? blockIdx.x * kWarps + w : blockIdx.x;
   // k_cache_attn lets this kernel come up only after its own wait, so lengths
   // may be read before this one's. Every warp waits: this kernel's end then
   // implies the other's.
@@ -432,42 +438,48 @@ __global__ void __launch_bounds__(kThreads) k_cache_combine(const CacheDev c, co
     const Ranges rg(total, ngrid, least_groups(ROWS));
     const int c0 = rg.of(ubeg), c1 = rg.of(ubeg + groups - 1);
     if (c0 == c1) return;  // that block stored the row
-    const auto slot = [&](int k) { return ((int64_t)k * 2 + (k == c0)) * ROWS + r; };
+    // sums part, part + PARTS, ... of the row's
+    const int cnt = (c1 - c0 + PARTS - part) / PARTS;
+    const auto slot = [&](int i) {
+      const int k = c0 + part + i * PARTS;
+      return ((int64_t)k * 2 + (k == c0)) * ROWS + r;
+    };
     // the first sums are under way while their weights are found
     constexpr int kAhead = 8;
     float first[kAhead][E];
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
-      const float* p = c.part_o + slot(min(c0 + j, c1)) * D + lane;
+    for (int j = 0; j < kAhead; ++j)
+      if (j < cnt) {
+        const float* p = c.part_o + slot(j) * D + lane;
 #pragma unroll
-      for (int i = 0; i < E; ++i) first[j][i] = p[32 * i];
-    }
+        for (int i = 0; i < E; ++i) first[j][i] = p[32 * i];
+      }
     float2 ml = make_float2(kEmpty, 0.f);
-    if (c0 + lane <= c1) ml = *reinterpret_cast<const float2*>(c.part_ml + slot(c0 + lane) * 2);
+    if (lane < cnt) ml = *reinterpret_cast<const float2*>(c.part_ml + slot(lane) * 2);
     m = ml.x;
-    for (int k = c0 + 32 + lane; k <= c1; k += 32) m = fmaxf(m, c.part_ml[slot(k) * 2]);
+    for (int k = 32 + lane; k < cnt; k += 32) m = fmaxf(m, c.part_ml[slot(k) * 2]);
 #pragma unroll
     for (int q = 16; q; q >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, q));
-    for (int k0 = c0; k0 <= c1; k0 += 32) {
-      if (k0 > c0) {
+    for (int k0 = 0; k0 < cnt; k0 += 32) {
+      if (k0) {
         ml = make_float2(kEmpty, 0.f);
-        if (k0 + lane <= c1) ml = *reinterpret_cast<const float2*>(c.part_ml + slot(k0 + lane) * 2);
+        if (k0 + lane < cnt) ml = *reinterpret_cast<const float2*>(c.part_ml + slot(k0 + lane) * 2);
       }
       const float f = ex2(ml.x - m);
       l = fmaf(f, ml.y, l);
-      const int cnt = min(32, c1 - k0 + 1);
+      const int here = min(32, cnt - k0);
       int j = 0;
-      if (k0 == c0) {
+      if (k0 == 0) {
 #pragma unroll
         for (; j < kAhead; ++j) {
           const float fj = __shfl_sync(0xffffffffu, f, j);
-          if (j < cnt)
+          if (j < here)
 #pragma unroll
             for (int i = 0; i < E; ++i) o[i] = fmaf(fj, first[j][i], o[i]);
         }
       }
 #pragma unroll 8
-      for (; j < cnt; ++j) {
+      for (; j < here; ++j) {
         const float fj = __shfl_sync(0xffffffffu, f, j);
         const float* p = c.part_o + slot(k0 + j) * D + lane;
 #pragma unroll
@@ -476,11 +488,33 @@ __global__ void __launch_bounds__(kThreads) k_cache_combine(const CacheDev c, co
     }
 #pragma unroll
     for (int q = 16; q; q >>= 1) l += __shfl_xor_sync(0xffffffffu, l, q);
+    if constexpr (PARTS > 1) {  // the whole block has one row: everyone is here
+      if (lane == 0) {
+        s_ml[part][0] = m;
+        s_ml[part][1] = l;
+      }
+#pragma unroll
+      for (int i = 0; i < E; ++i) s_o[part][lane + 32 * i] = o[i];
+      __syncthreads();
+      if (part) return;
+#pragma unroll
+      for (int k = 1; k < PARTS; ++k) m = fmaxf(m, s_ml[k][0]);
+      l = 0.f;
+#pragma unroll
+      for (int i = 0; i < E; ++i) o[i] = 0.f;
+#pragma unroll
+      for (int k = 0; k < PARTS; ++k) {
+        const float f = ex2(s_ml[k][0] - m);
+        l = fmaf(f, s_ml[k][1], l);
+#pragma unroll
+        for (int i = 0; i < E; ++i) o[i] = fmaf(f, s_o[k][lane + 32 * i], o[i]);
+      }
+    }
   }
+  if (part) return;
   const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-  for (int i = 0; i < E; ++i)
-    store1<F32 ? kDtF32 : kDtBF16>(row_ptr_mut<F32 ? kDtF32 : kDtBF16>(c.out, at), lane + 32 * i, o[i] * inv);
+  for (int i = 0; i < E; ++i) store1<kDt>(row_ptr_mut<kDt>(c.out, at), lane + 32 * i, o[i] * inv);
   if (lane == 0 && c.lse) store_lse(c, x, r, m, l);
 }
 
@@ -488,7 +522,9 @@ __global__ void __launch_bounds__(kThreads) k_cache_combine(const CacheDev c, co
 // 128 on the 5th-generation tensor cores.
 int tile_rows(const CacheDev& c) {
   const int64_t rows = c.blocks ? c.rep : (int64_t)c.n * c.rep;
-  if (rows >= kPromptMin && !c.blocks && c.dtype == kDtBF16) return kPromptRows;
+  if (rows >= kPromptMin && !c.blocks && c.dtype == kDtBF16 &&
+      rows * c.B * c.n_kv * c.max_blocks * c.bs >= kPromptWork)
+    return kPromptRows;
   return rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
 }
 
@@ -512,8 +548,11 @@ cudaError_t run_combine(const CacheDev& c, const Plan& pl, cudaStream_t st) {
   const int rows_used = (int)((c.blocks ? c.rep : (int64_t)c.n * c.rep) < ROWS ? (c.blocks ? c.rep : c.n * c.rep) : ROWS);
   const int64_t nrows = units * rows_used;
   if (nrows > 0x7fffffff - kWarps) return cudaErrorInvalidConfiguration;
-  CacheLaunch join((unsigned)((nrows + kWarps - 1) / kWarps), kThreads, 0, st);
-  const cudaError_t e = cudaLaunchKernelEx(&join.cfg, k_cache_combine<D, NT, F32>, c, pl, c.grid, rows_used, (int)nrows);
+  // a block a row where a unit may be in many ranges and the rows leave the SMs room
+  const bool wide = c.grid > 8 * units && nrows <= 148 * 16;
+  CacheLaunch join((unsigned)(wide ? nrows : (nrows + kWarps - 1) / kWarps), kThreads, 0, st);
+  const cudaError_t e = wide ? cudaLaunchKernelEx(&join.cfg, k_cache_combine<D, NT, F32, kWarps>, c, pl, c.grid, rows_used, (int)nrows)
+                             : cudaLaunchKernelEx(&join.cfg, k_cache_combine<D, NT, F32, 1>, c, pl, c.grid, rows_used, (int)nrows);
   note_launch();
   return e;
 }

@@ -33,9 +33,18 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// Rows of a tile for the kernel that takes many (ssa_cache_prompt.cu), and the
-// rows a kv head has to have for it.
-constexpr int kPromptRows = 128, kPromptMin = 64;
+// Rows of a tile for the kernel that takes many (ssa_cache_prompt.cu). It is
+// taken from 96 rows a kv head where rows x keys, by the table's width, come
+// to 2^24. Measured against the 32-row tiles (us; two kv heads, d 128 / 64):
+//   rows  sequences x keys   32-row tiles   128-row tiles
+//     64    32 x 8192          67 / 49         71 / 50
+//    128     1 x 16384         35 / 28         44 / 36
+//    128     8 x 8192          40 / 30         41 / 31
+//    128    32 x 8192         108 / 77         80 / 56
+//    512     1 x 16384         55 / 40         51 / 38
+//    512    32 x 8192         402 / 279       223 / 155
+constexpr int kPromptRows = 128, kPromptMin = 96;
+constexpr int64_t kPromptWork = 1 << 24;
 // Groups of 64 keys that are worth a thread block and its share of the join.
 constexpr int least_groups(int rows) { return rows == kPromptRows ? 4 : 1; }
 

@@ -282,18 +282,27 @@ ATTENDS = [  # dtype, H, n_kv, d, bs, n, lens after the step
     (BF, 8, 8, 32, 16, 70, [300, 70, 75]),
     (BF, 16, 2, 128, 64, 19, [200, 1, 64]),
     (F32, 12, 4, 128, 32, 11, [64, 100]),
-    # 64 rows a kv head and more: the many-row kernel
+    # the many-row kernel (96 rows a kv head and a wide table)
     (BF, 6, 2, 96, 32, 40, [200, 41, 0]),
     (BF, 32, 1, 128, 16, 5, [1000, 5, 64]),
     (BF, 4, 2, 64, 64, 300, [1100, 300, 17]),
-    (BF, 2, 1, 32, 32, 33, [65, 2000]),
+    (BF, 3, 1, 32, 32, 33, [65, 2000]),
+    (BF, 16, 1, 128, 64, 6, [640, 3000, 6, 0]),
 ]
+MANY_ROWS = len(ATTENDS) - 5  # cases from here on
+
+
+def _widen(pool, blocks):
+    """The table with more columns, without pages."""
+    pool.table = torch.nn.functional.pad(pool.table, (0, blocks - pool.table.shape[1]), value=-1).contiguous()
 
 
 def _filled(case, cuda, seed=0, spread=1.0):
     dtype, H, n_kv, d, bs, n, lens = ATTENDS[case]
     g = torch.Generator().manual_seed(100 + case + seed)
     pool = Pool(cuda, len(lens), n_kv, d, bs, -(-max(lens) // bs) + 1, dtype, seed=case)
+    if case >= MANY_ROWS:
+        _widen(pool, -(-2 ** 24 // (len(lens) * n * H * bs)))
     k, v = _kv(g, len(lens), max(lens), n_kv, d, dtype, cuda), _kv(g, len(lens), max(lens), n_kv, d, dtype, cuda)
     k = k * spread
     pool.advance(lens)
@@ -367,7 +376,7 @@ def test_attention_over_listed_blocks(case, cuda):
     pool, q = _filled(case, cuda)
     B, H, n, d = q.shape
     g = torch.Generator().manual_seed(case)
-    mb, scale = pool.table.shape[1], d ** -0.5
+    mb, scale = -(-max(ATTENDS[case][6]) // pool.bs) + 1, d ** -0.5
     for top in (1, 3, 7):
         blocks = torch.stack([torch.randperm(mb + 6, generator=g)[:min(top, mb)] - 3 for _ in range(B * n * pool.n_kv)])
         blocks = torch.nn.functional.pad(blocks, (0, top - blocks.shape[1]), value=-1).view(B, n, pool.n_kv, top)
@@ -376,16 +385,16 @@ def test_attention_over_listed_blocks(case, cuda):
         _check_attention(pool, q, out, lse, scale, blocks=blocks)
 
 
-@pytest.mark.parametrize("case", [0, 1, 4, 9])
+@pytest.mark.parametrize("case", [0, 1, 4, 9, 12, 15])
 def test_attention_skips_blocks_without_a_page(case, cuda):
     pool, q = _filled(case, cuda)
     pool.table[:, 0] = -1
-    pool.table[-1, -1] = pool.P
+    pool.table[-1, 1] = pool.P
     out, lse = pool.attend(q, 0.2, want_lse=True)
     _check_attention(pool, q, out, lse, 0.2)
 
 
-@pytest.mark.parametrize("dtype,d,rep", [(BF, 128, 4), (F32, 64, 4), (BF, 64, 72)])
+@pytest.mark.parametrize("dtype,d,rep", [(BF, 128, 4), (F32, 64, 4), (BF, 64, 100)])
 def test_attention_sharp_and_far_scores(dtype, d, rep, cuda):
     """Scores that grow along the cache (the running offset moves all the way),
     a single dominating key, and pages of very different steps, one of zeros."""
@@ -400,6 +409,8 @@ def test_attention_sharp_and_far_scores(dtype, d, rep, cuda):
     v2[:, :, bs:2 * bs] = 0
     for kk, vv in ((k1, v), (k1.flip(2), v), (k, v2), (k * 30, v), (k * 0, v)):
         pool = Pool(cuda, 1, n_kv, d, bs, L // bs, dtype)
+        if rep >= 96:
+            _widen(pool, -(-2 ** 24 // (rep * bs)))
         pool.advance([L])
         pool.append(kk.contiguous(), vv)
         pool.start = torch.tensor([L - 1], dtype=torch.int32, device=cuda)
@@ -407,7 +418,7 @@ def test_attention_sharp_and_far_scores(dtype, d, rep, cuda):
         _check_attention(pool, q, out, lse, d ** -0.5)
 
 
-@pytest.mark.parametrize("rep", [2, 64])
+@pytest.mark.parametrize("rep", [2, 128])
 @pytest.mark.parametrize("bad,value", [("k", math.nan), ("k", math.inf), ("v", math.nan), ("v", -math.inf)])
 def test_attention_keeps_nan_and_infinity_where_they_are(bad, value, rep, cuda):
     """A sequence with a page of NaN or infinity or an infinite q gives NaN; the
@@ -420,6 +431,8 @@ def test_attention_keeps_nan_and_infinity_where_they_are(bad, value, rep, cuda):
     pool.advance([40, 40, 40])
     pool.append(k, v)
     pool.amax[pool.table[:, 3].long()] = math.nan  # behind every length
+    if rep >= 96:
+        _widen(pool, -(-2 ** 24 // (3 * rep * bs)))
     pool.start = pool.lens - 1
     q = _kv(g, 3, 1, rep, d, BF, cuda)
     q[2, 1, 0, 5] = math.inf
@@ -497,6 +510,38 @@ def test_captured_decode_step(cuda):
     for a, b in zip(two[0].state(), p.state()):
         assert torch.equal(a, b)
     assert _lib.load().ssa_device_error(1) == 0
+
+
+def test_attention_many_sums_a_row(cuda):
+    """Few units over the whole GPU: a row's partial sums come from tens of
+    thread blocks, by one warp a row and by four."""
+    for H, n_kv, n, d, dtype in ((2, 1, 1, 64, BF), (4, 2, 1, 128, F32), (8, 1, 90, 64, BF), (32, 1, 64, 32, BF)):
+        g = torch.Generator().manual_seed(8)
+        L = 9000
+        pool = Pool(cuda, 1, n_kv, d, 64, -(-L // 64), dtype)
+        pool.advance([L])
+        pool.append(_kv(g, 1, L, n_kv, d, dtype, cuda), _kv(g, 1, L, n_kv, d, dtype, cuda))
+        pool.start = pool.lens - n
+        q = _kv(g, 1, n, H, d, dtype, cuda)
+        out, lse = pool.attend(q, d ** -0.5, want_lse=True)
+        assert torch.equal(out, pool.attend(q, d ** -0.5))
+        few = [0, n - 1] if n > 1 else [0]  # two tokens' rows are enough to compare
+        sub = Pool.__new__(Pool)
+        sub.__dict__.update(pool.__dict__)
+        for t in few:
+            sub.start, sub.lens = pool.start + t, pool.start + t + 1
+            _check_attention(sub, q[:, :, t:t + 1], out[:, :, t:t + 1], lse[:, :, t:t + 1], d ** -0.5)
+
+
+def test_many_row_kernel_repeats(cuda):
+    """Back to back calls of the many-row kernel, whose warps hand blocks of
+    keys to one another: the same bits every time, and no wait that ran out."""
+    pool, q = _filled(len(ATTENDS) - 1, cuda)
+    want = pool.attend(q, 0.1)
+    differ = torch.zeros((), device=cuda)
+    for _ in range(300):
+        differ += (pool.attend(q, 0.1) != want).any()
+    assert float(differ) == 0 and _lib.load().ssa_device_error(1) == 0
 
 
 def test_other_stream(cuda):
