@@ -806,12 +806,10 @@ cudaError_t run_select(const CacheDev& c, cudaStream_t st) {
   const int64_t grid = (int64_t)c.B * c.n * c.n_kv * ranks;
   if (grid > 0x7fffffff) return cudaErrorInvalidConfiguration;
   const size_t smem = SelSmem<D>::bytes(c);
-  if (smem > 40 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(k_cache_select<DT, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return e;
-  }
+  cudaError_t e = allow_smem<k_cache_select<DT, D>>(kSelSmemMax);
+  if (e != cudaSuccess) return e;
   CacheLaunch l((unsigned)grid, kSelThreads, smem, st, ranks);
-  const cudaError_t e = cudaLaunchKernelEx(&l.cfg, k_cache_select<DT, D>, c);
+  e = cudaLaunchKernelEx(&l.cfg, k_cache_select<DT, D>, c);
   note_launch();
   return e;
 }

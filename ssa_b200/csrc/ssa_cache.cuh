@@ -2,6 +2,8 @@
 // code paths its kernels share (ssa_cache.cu, ssa_cache_attn.cu).
 #pragma once
 
+#include <atomic>
+
 #include "ssa_common.cuh"
 #include "ssa_internal.h"
 
@@ -45,6 +47,21 @@ __device__ __forceinline__ unsigned long long f2_mul(unsigned long long a, unsig
   unsigned long long d;
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
+}
+
+// Lets kernel K use `bytes` of dynamic shared memory, once on each device (the
+// call takes a third of a launch's time).
+template <auto K>
+inline cudaError_t allow_smem(size_t bytes) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+  if (bit && (done.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+  e = cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
 }
 
 // Tokens of sequence b's current step (q rows / appended tokens that count).

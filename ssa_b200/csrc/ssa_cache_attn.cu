@@ -560,7 +560,7 @@ cudaError_t run_combine(const CacheDev& c, const Plan& pl, cudaStream_t st) {
 template <int D, int NT, bool F32>
 cudaError_t run_attn(const CacheDev& c, const Plan& pl, cudaStream_t st) {
   constexpr size_t smem = Smem<D, NT, F32>::kBytes;
-  cudaError_t e = cudaFuncSetAttribute(k_cache_attn<D, NT, F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  cudaError_t e = allow_smem<k_cache_attn<D, NT, F32>>(smem);
   if (e != cudaSuccess) return e;
   CacheLaunch main(c.grid, kThreads, smem, st);
   e = cudaLaunchKernelEx(&main.cfg, k_cache_attn<D, NT, F32>, c, pl);

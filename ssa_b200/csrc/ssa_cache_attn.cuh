@@ -35,14 +35,15 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
 
 // Rows of a tile for the kernel that takes many (ssa_cache_prompt.cu). It is
 // taken from 96 rows a kv head where rows x keys, by the table's width, come
-// to 2^24. Measured against the 32-row tiles (us; two kv heads, d 128 / 64):
+// to 2^24. Measured (us; two kv heads, d 128 / 64):
 //   rows  sequences x keys   32-row tiles   128-row tiles
-//     64    32 x 8192          67 / 49         71 / 50
-//    128     1 x 16384         35 / 28         44 / 36
-//    128     8 x 8192          40 / 30         41 / 31
-//    128    32 x 8192         108 / 77         80 / 56
-//    512     1 x 16384         55 / 40         51 / 38
-//    512    32 x 8192         402 / 279       223 / 155
+//     64    32 x 8192          64 / 46         69 / 49
+//    128     1 x 16384         29 / 22         35 / 23
+//    128     8 x 8192          40 / 30         41 / 30     2^24
+//    128    32 x 8192         107 / 77         79 / 55
+//    512     1 x 16384         55 / 40         44 / 31     2^24
+//    512    32 x 8192         403 / 279       223 / 156
+//   2048    32 x 8192        1533 / 1066      735 / 521
 constexpr int kPromptRows = 128, kPromptMin = 96;
 constexpr int64_t kPromptWork = 1 << 24;
 // Groups of 64 keys that are worth a thread block and its share of the join.

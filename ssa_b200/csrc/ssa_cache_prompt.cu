@@ -459,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
 template <int D>
 cudaError_t run_prompt(const CacheDev& c, const Plan& pl, cudaStream_t st) {
   constexpr size_t smem = PromptSmem<D>::kBytes;
-  const cudaError_t e = cudaFuncSetAttribute(k_cache_prompt<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  const cudaError_t e = allow_smem<k_cache_prompt<D>>(smem);
   if (e != cudaSuccess) return e;
   CacheLaunch l((unsigned)c.grid, kThreads, smem, st);
   const cudaError_t e2 = cudaLaunchKernelEx(&l.cfg, k_cache_prompt<D>, c, pl);

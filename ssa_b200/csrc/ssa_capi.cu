@@ -563,7 +563,7 @@ int ssa_cache_select(const ssa_cache_params* p, const void* q, const int8_t* bou
   if (p->sink < 0 || p->local < 1 || p->top < 1 || p->sink > p->top - p->local)
     return fail(SSA_ERR_INVALID, "top=%d must be at least sink (%d >= 0) + local (%d >= 1)", p->top, p->sink, p->local);
   ssa::CacheDev c = cache_dev(p);
-  if (ssa::cache_select_smem(c) > 222 * 1024)
+  if (ssa::cache_select_smem(c) > ssa::kSelSmemMax)
     return fail(SSA_ERR_UNSUPPORTED, "too many blocks in a table (%d) for the selection's on-chip scores", p->max_blocks);
   c.q = q; c.bounds = const_cast<int8_t*>(bounds); c.amax = const_cast<float*>(amax);
   c.table = table; c.start = start; c.lens = lens; c.blocks_out = blocks_out;

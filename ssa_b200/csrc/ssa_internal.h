@@ -238,6 +238,7 @@ struct ReserveDev {
 cudaError_t launch_cache_reserve(const ReserveDev& r, cudaStream_t st);
 cudaError_t launch_cache_append(const CacheDev& c, cudaStream_t st);
 size_t cache_select_smem(const CacheDev& c);
+constexpr size_t kSelSmemMax = 222 * 1024;  // what the selection may need
 cudaError_t launch_cache_select(const CacheDev& c, cudaStream_t st);
 // Fills the workspace pointers of c (ws may be null) and c->grid; bytes needed
 // (0: more work than the kernels count).

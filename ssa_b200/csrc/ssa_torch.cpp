@@ -7,6 +7,7 @@
 // layer, so the way from Python to the launch counts: through ctypes one such
 // call took 14 to 24 us, through this module 5 to 12.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -95,6 +96,15 @@ Lens lens_of(const Tensor& table, const Tensor& start, const Tensor& lens, int64
           static_cast<int32_t*>(buffer("lens", lens, at::kInt, {B}, like))};
 }
 
+// Uninitialised tensors on t's device, without the dispatcher's way there.
+Tensor fresh(const Tensor& t, at::ScalarType type, at::IntArrayRef shape) {
+  return at::detail::empty_cuda(shape, type, t.device(), c10::nullopt);
+}
+// (B, heads, n, d) as a view of (B, n, heads, d): the layout a projection reads.
+Tensor fresh_heads(const Tensor& t, int64_t B, int64_t heads, int64_t n, int64_t d) {
+  return at::detail::empty_strided_cuda({B, heads, n, d}, {n * heads * d, d, heads * d, 1}, t.scalar_type(), t.device());
+}
+
 void* stream_of(const Tensor& t) { return at::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
 
 std::tuple<Tensor, Tensor, Tensor> cache_reserve(const Tensor& lens, const Tensor& new_lens, const Tensor& table,
@@ -108,10 +118,9 @@ std::tuple<Tensor, Tensor, Tensor> cache_reserve(const Tensor& lens, const Tenso
   if (out) {
     std::tie(start, after, st) = *out;
   } else {
-    const Tensor both = at::empty({2, B}, lens.options());
-    start = both.select(0, 0);
-    after = both.select(0, 1);
-    st = at::empty({2}, lens.options());
+    start = fresh(lens, at::kInt, {B});
+    after = fresh(lens, at::kInt, {B});
+    st = fresh(lens, at::kInt, {2});
   }
   const auto p = [&](const char* name, const Tensor& t, at::IntArrayRef shape) {
     return static_cast<int32_t*>(buffer(name, t, at::kInt, shape, lens));
@@ -157,9 +166,8 @@ optional<std::tuple<Tensor, Tensor>> cache_append(const Tensor& k_in, const Tens
   Tensor kv, vv;
   ssa_cache_params p = {};
   if (want_values) {
-    const Tensor both = at::empty({2, B, n, n_kv, d}, k.options());
-    kv = both.select(0, 0).transpose(1, 2);
-    vv = both.select(0, 1).transpose(1, 2);
+    kv = fresh_heads(k, B, n_kv, n, d);
+    vv = fresh_heads(k, B, n_kv, n, d);
     p.o_sb = n * n_kv * d; p.o_sh = d; p.o_sn = n_kv * d;
   }
   if (B && n) {
@@ -188,7 +196,7 @@ Tensor cache_select(const Tensor& q_in, const Tensor& bounds, const Tensor& amax
   auto* pa = static_cast<float*>(buffer("amax", amax, at::kFloat, {P, n_kv, 2}, q));
   const Lens ln = lens_of(table, start, lens, B, q);
   const c10::cuda::OptionalCUDAGuard guard(q.device());
-  const Tensor out = at::empty({B, n, n_kv, i32(top, "top")}, q.options().dtype(at::kInt));
+  const Tensor out = fresh(q, at::kInt, {B, n, n_kv, i32(top, "top")});
   if (B && n) {
     ssa_cache_params p = {};
     p.B = i32(B, "B"); p.H = i32(H, "H"); p.n_kv = i32(n_kv, "n_kv"); p.n = i32(n, "n"); p.d = i32(d, "d");
@@ -226,9 +234,9 @@ std::tuple<Tensor, optional<Tensor>> cache_attention(const Tensor& q_in, const T
     pl = static_cast<int32_t*>(buffer("blocks", *blocks, at::kInt, {B, n, n_kv, blocks->size(3)}, q));
   }
   const c10::cuda::OptionalCUDAGuard guard(q.device());
-  const Tensor out = at::empty({B, n, H, d}, q.options()).transpose(1, 2);
+  const Tensor out = fresh_heads(q, B, H, n, d);
   optional<Tensor> lse;
-  if (want_lse) lse = at::empty({B, H, n}, q.options().dtype(at::kFloat));
+  if (want_lse) lse = fresh(q, at::kFloat, {B, H, n});
   if (B && n) {
     p.B = i32(B, "B"); p.H = i32(H, "H"); p.n_kv = i32(n_kv, "n_kv"); p.n = i32(n, "n"); p.d = i32(d, "d");
     p.block_size = i32(bs, "block_size"); p.max_blocks = i32(table.size(1), "max_blocks"); p.num_pages = i32(P, "num_pages");
@@ -236,7 +244,7 @@ std::tuple<Tensor, optional<Tensor>> cache_attention(const Tensor& q_in, const T
     p.q_sb = q.stride(0); p.q_sh = q.stride(1); p.q_sn = q.stride(2);
     p.o_sb = n * H * d; p.o_sh = d; p.o_sn = H * d;
     const size_t bytes = ssa_cache_attn_workspace_size(&p, pl != nullptr);
-    const Tensor ws = at::empty({(int64_t)(bytes ? bytes : 1)}, q.options().dtype(at::kByte));
+    const Tensor ws = fresh(q, at::kByte, {(int64_t)(bytes ? bytes : 1)});
     check(ssa_cache_attn(&p, q.data_ptr(), pk, pv, pa, ln.table, ln.start, ln.lens, pl, out.data_ptr(),
                          want_lse ? lse->data_ptr<float>() : nullptr, ws.data_ptr(), bytes, stream_of(q)),
           "ssa_cache_attn");
