@@ -233,7 +233,13 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
   } else if (w == kSoftWarps + kConvWarps) {
     // ------------------------------------------------------------ products
     if (lane == 0) {
-      const uint32_t qa = smem_u32(sm + Sm::kQ), kva = smem_u32(sm + Sm::kKV);
+      // One thread issues everything, an instruction every nine cycles or so:
+      // descriptors are made once, and only their address field moves (16-byte
+      // units). Made in place they took the thread longer than the products.
+      const uint64_t q_desc = umma_desc(smem_u32(sm + Sm::kQ));
+      const uint64_t k_desc = umma_desc(smem_u32(sm + Sm::kKV));
+      const uint64_t v_desc = desc_channels_inner(smem_u32(sm + Sm::kKV + Sm::kTile), 64 * 128);
+      constexpr uint32_t kStage = 2 * Sm::kTile / 16;
       constexpr uint32_t kDescS = idesc_f16(kPromptRows, 64, false), kDescO = idesc_f16(kPromptRows, D, true);
       bool ok = true;
       int segs = 0;
@@ -242,11 +248,11 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
         if (!mbar_wait(kfull + st, (i >> 1) & 1, abort_flag, 32, kWaitLimit)) return false;
         if (i && !mbar_wait(sempty, (i - 1) & 1, abort_flag, 33, kWaitLimit)) return false;
         tc_fence_after();
-        const uint32_t ka = kva + st * 2 * Sm::kTile;
+        const uint64_t kd = k_desc + (uint32_t)st * kStage;
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk)
-          umma_bf16(tmem, umma_desc(qa + (kk >> 2) * (kPromptRows * 128) + (kk & 3) * 32),
-                    umma_desc(ka + (kk >> 2) * (64 * 128) + (kk & 3) * 32), kDescS, kk > 0);
+          umma_bf16(tmem, q_desc + ((kk >> 2) * (kPromptRows * 128) + (kk & 3) * 32) / 16,
+                    kd + ((kk >> 2) * (64 * 128) + (kk & 3) * 32) / 16, kDescS, kk > 0);
         umma_commit(sfull);
         return true;
       };
@@ -260,10 +266,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
           ok = mbar_wait(vfull + st, (it >> 1) & 1, abort_flag, 35, kWaitLimit) && mbar_wait(pfull, it & 1, abort_flag, 36, kWaitLimit);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t va = kva + (st * 2 + 1) * Sm::kTile;
+          const uint64_t vd = v_desc + (uint32_t)st * kStage;
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)
-            umma_ts(tmem + kColO, tmem + kColP + kk * 8, desc_channels_inner(va + kk * 16 * 128, 64 * 128), kDescO, (j | kk) > 0);
+            umma_ts(tmem + kColO, tmem + kColP + kk * 8, vd + kk * (16 * 128 / 16), kDescO, (j | kk) > 0);
           umma_commit(kvempty + st);
           umma_commit(odone);
         }
