@@ -63,7 +63,7 @@ struct Smem {
   static constexpr int kBytes = kQ + (F32 ? 2 : 1) * NT * (D / 16) * 32 * 8;
 };
 template <int D, int NT, bool F32>
-__global__ void __launch_bounds__(kThreads, blocks_per_sm(D, 8 * NT)) k_cache_attn(const CacheDev c, const Plan pl) {
+__global__ void __launch_bounds__(kThreads, blocks_per_sm(D, 8 * NT) + (NT == 1)) k_cache_attn(const CacheDev c, const Plan pl) {
   using Sm = Smem<D, NT, F32>;
   constexpr int ROWS = 8 * NT, W16 = D / 16, PC = F32 ? 2 : 1, OP = D + 4;
   constexpr int kDt = F32 ? kDtF32 : kDtBF16;
@@ -444,16 +444,19 @@ __global__ void __launch_bounds__(kThreads) k_cache_combine(const CacheDev c, co
       const int k = c0 + part + i * PARTS;
       return ((int64_t)k * 2 + (k == c0)) * ROWS + r;
     };
-    // the first sums are under way while their weights are found
-    constexpr int kAhead = 8;
-    float first[kAhead][E];
+    // sums come in batches of loads; the first is under way while the weights are found
+    constexpr int kBatch = PARTS > 1 ? 16 : 8;
+    float batch[kBatch][E];
+    const auto load = [&](int j0) {
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j)
-      if (j < cnt) {
-        const float* p = c.part_o + slot(j) * D + lane;
+      for (int j = 0; j < kBatch; ++j)
+        if (j0 + j < cnt) {
+          const float* p = c.part_o + slot(j0 + j) * D + lane;
 #pragma unroll
-        for (int i = 0; i < E; ++i) first[j][i] = p[32 * i];
-      }
+          for (int i = 0; i < E; ++i) batch[j][i] = p[32 * i];
+        }
+    };
+    load(0);
     float2 ml = make_float2(kEmpty, 0.f);
     if (lane < cnt) ml = *reinterpret_cast<const float2*>(c.part_ml + slot(lane) * 2);
     m = ml.x;
@@ -467,23 +470,15 @@ __global__ void __launch_bounds__(kThreads) k_cache_combine(const CacheDev c, co
       }
       const float f = ex2(ml.x - m);
       l = fmaf(f, ml.y, l);
-      const int here = min(32, cnt - k0);
-      int j = 0;
-      if (k0 == 0) {
+      for (int j0 = 0; j0 < 32 && k0 + j0 < cnt; j0 += kBatch) {
+        if (k0 + j0) load(k0 + j0);
 #pragma unroll
-        for (; j < kAhead; ++j) {
-          const float fj = __shfl_sync(0xffffffffu, f, j);
-          if (j < here)
+        for (int j = 0; j < kBatch; ++j) {
+          const float fj = __shfl_sync(0xffffffffu, f, j0 + j);
+          if (k0 + j0 + j < cnt)
 #pragma unroll
-            for (int i = 0; i < E; ++i) o[i] = fmaf(fj, first[j][i], o[i]);
+            for (int i = 0; i < E; ++i) o[i] = fmaf(fj, batch[j][i], o[i]);
         }
-      }
-#pragma unroll 8
-      for (; j < here; ++j) {
-        const float fj = __shfl_sync(0xffffffffu, f, j);
-        const float* p = c.part_o + slot(k0 + j) * D + lane;
-#pragma unroll
-        for (int i = 0; i < E; ++i) o[i] = fmaf(fj, p[32 * i], o[i]);
       }
     }
 #pragma unroll
