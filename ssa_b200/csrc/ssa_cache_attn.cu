@@ -544,7 +544,7 @@ cudaError_t run_combine(const CacheDev& c, const Plan& pl, cudaStream_t st) {
   const int64_t nrows = units * rows_used;
   if (nrows > 0x7fffffff - kWarps) return cudaErrorInvalidConfiguration;
   // a block a row where a unit may be in many ranges and the rows leave the SMs room
-  const bool wide = c.grid > 8 * units && nrows <= 148 * 16;
+  const bool wide = c.grid > 16 * units && nrows <= 148 * 16;
   CacheLaunch join((unsigned)(wide ? nrows : (nrows + kWarps - 1) / kWarps), kThreads, 0, st);
   const cudaError_t e = wide ? cudaLaunchKernelEx(&join.cfg, k_cache_combine<D, NT, F32, kWarps>, c, pl, c.grid, rows_used, (int)nrows)
                              : cudaLaunchKernelEx(&join.cfg, k_cache_combine<D, NT, F32, 1>, c, pl, c.grid, rows_used, (int)nrows);
