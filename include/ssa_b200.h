@@ -368,7 +368,8 @@ SSA_API int32_t ssa_device_error(int32_t clear);
  * a wait run out without faulting or hanging the GPU. The kernel then stops
  * its pipeline, waits for its own copies and MMAs in flight, frees its TMEM
  * and returns; ssa_device_error reports the code and that build's output is
- * undefined. Process-wide; read when each build is launched. */
+ * undefined. The many-row kernel of ssa_cache_attn gives up in the same way.
+ * Process-wide; read when each build or attention is launched. */
 SSA_API int ssa_debug_set_wait_limit(uint32_t polls);
 
 /* Testing aids for the tensor-core hash (no counterpart in the reference;

@@ -32,7 +32,6 @@ constexpr int kConvThreads = kConvWarps * 32;
 // as 72 to the 128 converting threads and 120 to the 128 with a row:
 // 128 * 72 + 128 * 120 + 32 * 96 = 288 * 96.
 constexpr uint32_t kTmemCols = 256, kColP = 64, kColO = 128;  // S at 0
-constexpr uint32_t kWaitLimit = 1u << 24;
 
 template <int D>
 struct PromptSmem {
@@ -206,7 +205,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
       for (int gr = g0; gr < ge; ++gr, ++it) {
         const int st = it & 1;
         unsigned char* tile = sm + Sm::kKV + st * 2 * Sm::kTile;
-        if (!(ok = mbar_wait_warp(kvempty + st, ((it >> 1) & 1) ^ 1, abort_flag, 31, kWaitLimit))) break;
+        if (!(ok = mbar_wait_warp(kvempty + st, ((it >> 1) & 1) ^ 1, abort_flag, 31, c.wait_limit))) break;
         if (w == kSoftWarps && lane < 4) {
           const float va = am.y * (1.f / 127.f), vs = va > 0.f ? va : 1.f;
           // keys without a page: scores of minus infinity; a page of NaN: scores of NaN
@@ -245,8 +244,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
       int segs = 0;
       const auto scores = [&](int i) {
         const int st = i & 1;
-        if (!mbar_wait(kfull + st, (i >> 1) & 1, abort_flag, 32, kWaitLimit)) return false;
-        if (i && !mbar_wait(sempty, (i - 1) & 1, abort_flag, 33, kWaitLimit)) return false;
+        if (!mbar_wait(kfull + st, (i >> 1) & 1, abort_flag, 32, c.wait_limit)) return false;
+        if (i && !mbar_wait(sempty, (i - 1) & 1, abort_flag, 33, c.wait_limit)) return false;
         tc_fence_after();
         const uint64_t kd = k_desc + (uint32_t)st * kStage;
 #pragma unroll
@@ -259,11 +258,11 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
       while (ok && seg.next(c, pl, x, g0, g1, groups)) {
         const int nb = min(g1, (lim_max_of(c, x) + 63) / 64) - g0;
         if (nb <= 0) continue;
-        ok = mbar_wait(qfull, segs++ & 1, abort_flag, 34, kWaitLimit) && scores(it);
+        ok = mbar_wait(qfull, segs++ & 1, abort_flag, 34, c.wait_limit) && scores(it);
         for (int j = 0; ok && j < nb; ++j, ++it) {
           const int st = it & 1;
           if (j + 1 < nb && !(ok = scores(it + 1))) break;
-          ok = mbar_wait(vfull + st, (it >> 1) & 1, abort_flag, 35, kWaitLimit) && mbar_wait(pfull, it & 1, abort_flag, 36, kWaitLimit);
+          ok = mbar_wait(vfull + st, (it >> 1) & 1, abort_flag, 35, c.wait_limit) && mbar_wait(pfull, it & 1, abort_flag, 36, c.wait_limit);
           if (!ok) break;
           tc_fence_after();
           const uint64_t vd = v_desc + (uint32_t)st * kStage;
@@ -293,7 +292,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
       const int lim = !have ? INT32_MAX : c.causal ? x.start + tok + 1 : x.len;
       // this thread's row in q and out (rows behind the last one: the first, never stored)
       const int64_t q_at = x.b * c.q_sb + hd * c.q_sh + tok * c.q_sn, o_at = x.b * c.o_sb + hd * c.o_sh + tok * c.o_sn;
-      float m = kEmpty, l = 0.f;
+      // A row behind the last one computes the first row's scores over all keys,
+      // stale ones too: its offset is out of reach, so that it moves nothing.
+      float m = have ? kEmpty : -kEmpty, l = 0.f;
       if (nb > 0) {
         // Q: rows into their swizzled places as they come, 8 bytes a lane, then
         // each thread turns its own into fp16 where it lies, scaled by a power of
@@ -335,11 +336,11 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
 
         for (int j = 0; j < nb; ++j, ++it) {
           const int st = it & 1, key0 = (g0 + j) * 64;
-          if (!(ok = mbar_wait_warp(kfull + st, (it >> 1) & 1, abort_flag, 37, kWaitLimit))) break;  // the steps
+          if (!(ok = mbar_wait_warp(kfull + st, (it >> 1) & 1, abort_flag, 37, c.wait_limit))) break;  // the steps
           float4 mt[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) mt[k] = meta[st * 4 + k];
-          if (!(ok = mbar_wait_warp(sfull, it & 1, abort_flag, 38, kWaitLimit))) break;
+          if (!(ok = mbar_wait_warp(sfull, it & 1, abort_flag, 38, c.wait_limit))) break;
           tc_fence_after();
           float s[64];
           tmem_ld32(trow, s);
@@ -394,7 +395,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
           }
           if (j > 0) {
             // the product before has read P and added to O
-            if (!(ok = mbar_wait_warp(odone, (it - 1) & 1, abort_flag, 39, kWaitLimit))) break;
+            if (!(ok = mbar_wait_warp(odone, (it - 1) & 1, abort_flag, 39, c.wait_limit))) break;
             tc_fence_after();
             if (__any_sync(0xffffffffu, f != 1.f)) {
 #pragma unroll 1
@@ -416,7 +417,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
           if (lane == 0) mbar_arrive(pfull);
         }
         if (ok) {
-          ok = mbar_wait_warp(odone, (it - 1) & 1, abort_flag, 40, kWaitLimit);
+          ok = mbar_wait_warp(odone, (it - 1) & 1, abort_flag, 40, c.wait_limit);
           tc_fence_after();
         }
       }

@@ -501,6 +501,8 @@ static int check_heads(const ssa_cache_params* p) {
 static ssa::CacheDev cache_dev(const ssa_cache_params* p) {
   ssa::CacheDev c;
   memset(&c, 0, sizeof(c));
+  const uint32_t wl = g_wait_limit.load(std::memory_order_relaxed);
+  c.wait_limit = wl ? wl : (1u << 24);
   c.B = p->B; c.H = p->H; c.n_kv = p->n_kv; c.rep = p->H / p->n_kv; c.n = p->n; c.d = p->d; c.dtype = p->dtype;
   c.bs = p->block_size; c.max_blocks = p->max_blocks; c.num_pages = p->num_pages;
   c.top = p->top; c.sink = p->sink; c.local = p->local; c.causal = p->causal; c.scale = p->scale;
@@ -548,6 +550,7 @@ int ssa_cache_append(const ssa_cache_params* p, const void* k, const void* v, in
   c.k = k; c.v = v; c.k_codes = k_codes; c.v_codes = v_codes; c.amax = amax; c.bounds = bounds; c.tail = tail;
   c.table = table; c.start = start; c.lens = lens; c.k_values = k_values; c.v_values = v_values;
   cudaError_t e = ssa::launch_cache_append(c, static_cast<cudaStream_t>(stream));
+  if (e == cudaErrorInvalidConfiguration) return fail(SSA_ERR_UNSUPPORTED, "B * n_kv * n is too large for one call");
   if (e != cudaSuccess) return cuda_fail(e, "cache append launch");
   return SSA_OK;
 }
@@ -564,10 +567,12 @@ int ssa_cache_select(const ssa_cache_params* p, const void* q, const int8_t* bou
     return fail(SSA_ERR_INVALID, "top=%d must be at least sink (%d >= 0) + local (%d >= 1)", p->top, p->sink, p->local);
   ssa::CacheDev c = cache_dev(p);
   if (ssa::cache_select_smem(c) > ssa::kSelSmemMax)
-    return fail(SSA_ERR_UNSUPPORTED, "too many blocks in a table (%d) for the selection's on-chip scores", p->max_blocks);
+    return fail(SSA_ERR_UNSUPPORTED, "the selection's on-chip scores do not hold %d blocks a table with %d heads a kv head",
+                p->max_blocks, c.rep);
   c.q = q; c.bounds = const_cast<int8_t*>(bounds); c.amax = const_cast<float*>(amax);
   c.table = table; c.start = start; c.lens = lens; c.blocks_out = blocks_out;
   cudaError_t e = ssa::launch_cache_select(c, static_cast<cudaStream_t>(stream));
+  if (e == cudaErrorInvalidConfiguration) return fail(SSA_ERR_UNSUPPORTED, "B * n_kv * n is too large for one call");
   if (e != cudaSuccess) return cuda_fail(e, "cache select launch");
   return SSA_OK;
 }
@@ -602,6 +607,7 @@ int ssa_cache_attn(const ssa_cache_params* p, const void* q, const int8_t* k_cod
   c.q = q; c.k_codes = const_cast<int8_t*>(k_codes); c.v_codes = const_cast<int8_t*>(v_codes);
   c.amax = const_cast<float*>(amax); c.table = table; c.start = start; c.lens = lens; c.out = out; c.lse = lse;
   cudaError_t e = ssa::launch_cache_attn(c, static_cast<cudaStream_t>(stream));
+  if (e == cudaErrorInvalidConfiguration) return fail(SSA_ERR_UNSUPPORTED, "B * H * n is too large for one call");
   if (e != cudaSuccess) return cuda_fail(e, "cache attention launch");
   return SSA_OK;
 }

@@ -200,6 +200,7 @@ struct CacheDev {
   int B, H, n_kv, rep, n, d, dtype, bs, max_blocks, num_pages;
   int top, sink, local, causal;
   float scale;
+  uint32_t wait_limit;  // polls before a wait of the many-row kernel gives up (ssa_debug_set_wait_limit)
   int64_t q_sb, q_sh, q_sn, k_sb, k_sh, k_sn, v_sb, v_sh, v_sn, o_sb, o_sh, o_sn;
   const void* q;
   const void* k;

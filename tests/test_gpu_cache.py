@@ -544,6 +544,69 @@ def test_many_row_kernel_repeats(cuda):
     assert float(differ) == 0 and _lib.load().ssa_device_error(1) == 0
 
 
+def test_many_row_kernel_wait_that_runs_out(cuda):
+    """A wait given a single poll gives up: the kernel ends, reports its code and
+    leaves the GPU usable."""
+    L = _lib.load()
+    pool, q = _filled(len(ATTENDS) - 1, cuda)
+    want = pool.attend(q, 0.1)
+    assert L.ssa_device_error(1) == 0
+    L.ssa_debug_set_wait_limit(1)
+    try:
+        pool.attend(q, 0.1)
+        torch.cuda.synchronize()
+        assert L.ssa_device_error(1) != 0
+    finally:
+        L.ssa_debug_set_wait_limit(0)
+    assert torch.equal(pool.attend(q, 0.1), want) and L.ssa_device_error(1) == 0
+
+
+@pytest.mark.parametrize("n", [1, 100])
+def test_offsets_beyond_32_bits(n, cuda):
+    """Pages whose codes lie past 2^31 bytes, bounds past 2^31 / 32, against the
+    same sequences in the first pages."""
+    n_kv, d, bs, H, B, L = 16, 128, 64, 32, 2, 200
+    P = 2 ** 31 // (n_kv * bs * d) + 40
+    g = torch.Generator().manual_seed(12)
+    far = Pool.__new__(Pool)
+    far.P, far.bs, far.d, far.n_kv, far.B = P, bs, d, n_kv, B
+    far.k, far.v = (torch.empty(P, n_kv, bs, d, dtype=torch.int8, device=cuda) for _ in range(2))
+    far.bounds = torch.empty(P, n_kv, 2, d, dtype=torch.int8, device=cuda)
+    far.amax = torch.empty(P, n_kv, 2, device=cuda)
+    far.tail = torch.zeros(B, n_kv, 2, bs, d, dtype=BF, device=cuda)
+    far.start, far.lens = (torch.zeros(B, dtype=torch.int32, device=cuda) for _ in range(2))
+    far.table = (P - 1 - torch.arange(8, device=cuda)).view(B, 4).int().contiguous()
+    near = Pool(cuda, B, n_kv, d, bs, 4, BF)
+    k, v = _kv(g, B, L, n_kv, d, BF, cuda), _kv(g, B, L, n_kv, d, BF, cuda)
+    q = _kv(g, B, n, H, d, BF, cuda)
+    got = []
+    for p in (far, near):
+        p.advance([L, L - 70])
+        p.append(k, v)
+        p.start = p.lens - n
+        blocks = p.select(q, 3)
+        if n > 1:
+            _widen(p, -(-2 ** 24 // (B * n * H * bs)))  # the many-row kernel
+        whole = p.table[:, :(L - 70) // bs].long()  # pages complete in both sequences: the rest of a page keeps what it held
+        got.append((blocks, p.attend(q, 0.1), p.attend(q, 0.1, blocks=blocks), p.k[whole], p.v[whole], p.bounds[whole], p.amax[whole]))
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+
+
+def test_attention_of_many_sequences(cuda):
+    """More sequences than a thread block has threads."""
+    B, n_kv, H, d, bs = 700, 1, 3, 32, 16
+    g = torch.Generator().manual_seed(13)
+    lens = torch.randint(0, 60, (B,), generator=g).tolist()
+    pool = Pool(cuda, B, n_kv, d, bs, 4, BF)
+    pool.advance(lens)
+    pool.append(_kv(g, B, 60, n_kv, d, BF, cuda), _kv(g, B, 60, n_kv, d, BF, cuda))
+    pool.start = (pool.lens - 1).clamp(min=0)
+    q = _kv(g, B, 1, H, d, BF, cuda)
+    out, lse = pool.attend(q, 0.2, want_lse=True)
+    _check_attention(pool, q, out, lse, 0.2)
+
+
 def test_other_stream(cuda):
     pool, q = _filled(0, cuda)
     want = pool.attend(q, 0.1)
