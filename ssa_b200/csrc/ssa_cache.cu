@@ -381,11 +381,11 @@ template <int DT, int D, int BS>
 __global__ void __launch_bounds__(kAppendThreads<D, BS>, DT == kDtF32 ? 2 : 4) k_cache_append(const CacheDev c, const int nt) {
   __shared__ float4 red[(DT == kDtF32 ? 2 : 1) * kAppendThreads<D, BS>];
   unsigned i = blockIdx.x;
-  const int j = (int)(i % (unsigned)nt);
-  i /= (unsigned)nt;
+  const int kv = (int)(i % (unsigned)c.n_kv);
+  i /= (unsigned)c.n_kv;
   const int s = (int)(i & 1);
   i >>= 1;
-  const int kv = (int)(i % (unsigned)c.n_kv), b = (int)(i / (unsigned)c.n_kv);
+  const int j = (int)(i % (unsigned)nt), b = (int)(i / (unsigned)nt);
   grid_wait();
   int start, len;
   const int fresh = cache_step_tokens(c, b, start, len);
