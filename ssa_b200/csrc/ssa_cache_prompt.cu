@@ -39,8 +39,11 @@ struct PromptSmem {
   static constexpr int kQ = 0;                                         // [kAtoms][128 rows][128 bytes]
   static constexpr int kTile = kAtoms * 64 * 128;                      // [kAtoms][64 keys][128 bytes]
   static constexpr int kKV = kAtoms * kPromptRows * 128;               // [2 stages][K, V] tiles
-  static constexpr int kMeta = kKV + 4 * kTile;                        // [2 stages][4] {step_k, log2 step_v, 1 / step_v, -}
-  static constexpr int kBars = kMeta + 2 * 4 * 16;
+  // [4][4] {step_k, log2 step_v, 1 / step_v, -}: K's stage is filled again when
+  // its scores are there, and a row may read these after that; four blocks of
+  // keys on, every row has read the scores of two blocks further.
+  static constexpr int kMeta = kKV + 4 * kTile;
+  static constexpr int kBars = kMeta + 4 * 4 * 16;
   static constexpr int kBytes = kBars + 128 + 1024;                    // the base is rounded up to 1024
 };
 
@@ -110,8 +113,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
   unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
   float4* meta = reinterpret_cast<float4*>(sm + Sm::kMeta);
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + Sm::kBars);
-  uint64_t *kfull = bars, *vfull = bars + 2, *kvempty = bars + 4, *sfull = bars + 6, *sempty = bars + 7, *pfull = bars + 8,
-           *odone = bars + 9, *qfull = bars + 10, *mma_done = bars + 11;
+  uint64_t *kfull = bars, *vfull = bars + 2, *kempty = bars + 4, *vempty = bars + 6, *sfull = bars + 8, *sempty = bars + 9,
+           *pfull = bars + 10, *odone = bars + 11, *qfull = bars + 12, *mma_done = bars + 13;
   __shared__ RangeSmem rs;
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag_s;
@@ -127,7 +130,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
     for (int i = 0; i < 2; ++i) {
       mbar_init(kfull + i, kConvWarps);
       mbar_init(vfull + i, kConvWarps);
-      mbar_init(kvempty + i, 1);
+      mbar_init(kempty + i, 1);
+      mbar_init(vempty + i, 1);
     }
     mbar_init(sfull, 1);
     mbar_init(sempty, kSoftWarps);
@@ -193,6 +197,15 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
       int pages = cache_checked(c, entry(g0)), ahead = entry(g0 + 1);
       uint4 kr[kLoads], vr[kLoads];
       float2 am = make_float2(0.f, 0.f);
+      float4 mt = make_float4(0.f, -INFINITY, 0.f, 0.f);
+      const auto steps = [&]() {
+        if (w == kSoftWarps && lane < 4) {
+          const float va = am.y * (1.f / 127.f), vs = va > 0.f ? va : 1.f;
+          // keys without a page: scores of minus infinity; a page of NaN: scores of NaN
+          mt = pages >= 0 ? make_float4(am.x * (1.f / 127.f), __log2f(vs) + (va != va ? va : 0.f), 1.f / vs, 0.f)
+                          : make_float4(0.f, -INFINITY, 0.f, 0.f);
+        }
+      };
       const auto load_amax = [&](int pg) {
         return w == kSoftWarps && lane < 4 && pg >= 0
                    ? *(reinterpret_cast<const float2*>(c.amax) + (int64_t)pg * c.n_kv + x.kv) : make_float2(0.f, 0.f);
@@ -201,32 +214,32 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
         load(c.k_codes, g0, pages, kr);
         am = load_amax(pages);
         load(c.v_codes, g0, pages, vr);
+        steps();
       }
       for (int gr = g0; gr < ge; ++gr, ++it) {
         const int st = it & 1;
         unsigned char* tile = sm + Sm::kKV + st * 2 * Sm::kTile;
-        if (!(ok = mbar_wait_warp(kvempty + st, ((it >> 1) & 1) ^ 1, abort_flag, 31, c.wait_limit))) break;
-        if (w == kSoftWarps && lane < 4) {
-          const float va = am.y * (1.f / 127.f), vs = va > 0.f ? va : 1.f;
-          // keys without a page: scores of minus infinity; a page of NaN: scores of NaN
-          meta[st * 4 + lane] = pages >= 0 ? make_float4(am.x * (1.f / 127.f), __log2f(vs) + (va != va ? va : 0.f), 1.f / vs, 0.f)
-                                           : make_float4(0.f, -INFINITY, 0.f, 0.f);
-        }
-        pages = cache_checked(c, ahead);
-        ahead = entry(gr + 2);
+        if (!(ok = mbar_wait_warp(kempty + st, ((it >> 1) & 1) ^ 1, abort_flag, 31, c.wait_limit))) break;
+        if (w == kSoftWarps && lane < 4) meta[(it & 3) * 4 + lane] = mt;
         store(tile, kr);
         fence_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(kfull + st);
+        pages = cache_checked(c, ahead);
+        ahead = entry(gr + 2);
         if (gr + 1 < ge) {
           load(c.k_codes, gr + 1, pages, kr);
           am = load_amax(pages);
         }
+        if (!(ok = mbar_wait_warp(vempty + st, ((it >> 1) & 1) ^ 1, abort_flag, 41, c.wait_limit))) break;
         store(tile + Sm::kTile, vr);
         fence_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(vfull + st);
-        if (gr + 1 < ge) load(c.v_codes, gr + 1, pages, vr);
+        if (gr + 1 < ge) {
+          load(c.v_codes, gr + 1, pages, vr);
+          steps();
+        }
       }
     }
   } else if (w == kSoftWarps + kConvWarps) {
@@ -253,6 +266,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
           umma_bf16(tmem, q_desc + ((kk >> 2) * (kPromptRows * 128) + (kk & 3) * 32) / 16,
                     kd + ((kk >> 2) * (64 * 128) + (kk & 3) * 32) / 16, kDescS, kk > 0);
         umma_commit(sfull);
+        umma_commit(kempty + st);
         return true;
       };
       while (ok && seg.next(c, pl, x, g0, g1, groups)) {
@@ -269,7 +283,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)
             umma_ts(tmem + kColO, tmem + kColP + kk * 8, vd + kk * (16 * 128 / 16), kDescO, (j | kk) > 0);
-          umma_commit(kvempty + st);
+          umma_commit(vempty + st);
           umma_commit(odone);
         }
       }
@@ -339,7 +353,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
           if (!(ok = mbar_wait_warp(kfull + st, (it >> 1) & 1, abort_flag, 37, c.wait_limit))) break;  // the steps
           float4 mt[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) mt[k] = meta[st * 4 + k];
+          for (int k = 0; k < 4; ++k) mt[k] = meta[(it & 3) * 4 + k];
           if (!(ok = mbar_wait_warp(sfull, it & 1, abort_flag, 38, c.wait_limit))) break;
           tc_fence_after();
           float s[64];
