@@ -170,31 +170,37 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
         const int key = gr * 64 + (lane & 3) * 16;
         return gr < ge && key < lim_max ? cache_entry(c, x.b, key >> bs_shift) : -1;
       };
-      const auto load = [&](const int8_t* codes, int gr, int pages, uint4 (&r)[kLoads]) {
+      // where those keys lie, in units of 16 rows of codes
+      const auto place = [&](int gr, int pages) {
+        return (uint32_t)(((int64_t)max(pages, 0) * c.n_kv + x.kv) * (c.bs / 16)) + (uint32_t)((gr * 4 + (lane & 3)) & (c.bs / 16 - 1));
+      };
+      // piece i of a thread: 16 bytes of the tile's id-th, id = i * kConvThreads + ct
+      const auto load = [&](const int8_t* codes, uint32_t at, uint4 (&r)[kLoads]) {
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-          const int id = i * kConvThreads + ct, row = id / (D / 16), part = id % (D / 16), sub = row >> 4;
-          const int64_t pg = max(__shfl_sync(0xffffffffu, pages, sub), 0);
-          const int off = (gr * 64 + sub * 16) & (c.bs - 1);
-          r[i] = *reinterpret_cast<const uint4*>(codes + (((pg * c.n_kv + x.kv) * c.bs + off + (row & 15)) * D + part * 16));
+          const int id = i * kConvThreads + ct;
+          const uint32_t rows = __shfl_sync(0xffffffffu, at, id / D);
+          r[i] = *reinterpret_cast<const uint4*>(codes + ((uint64_t)rows * (16 * D) + (unsigned)(id % D * 16)));
         }
       };
       const auto store = [&](unsigned char* tile, const uint4 (&r)[kLoads]) {
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
           const int id = i * kConvThreads + ct, row = id / (D / 16), part = id % (D / 16);
-          const uint32_t w4[4] = {r[i].x ^ 0x80808080u, r[i].y ^ 0x80808080u, r[i].z ^ 0x80808080u, r[i].w ^ 0x80808080u};
-          uint4 h[2];
-          h[0] = make_uint4(codes_f16<0x4140>(w4[0]), codes_f16<0x4342>(w4[0]), codes_f16<0x4140>(w4[1]), codes_f16<0x4342>(w4[1]));
-          h[1] = make_uint4(codes_f16<0x4140>(w4[2]), codes_f16<0x4342>(w4[2]), codes_f16<0x4140>(w4[3]), codes_f16<0x4342>(w4[3]));
-          unsigned char* at = tile + (part >> 2) * (64 * 128) + row * 128;
           // chunks 2 part, 2 part + 1 of the row; every other group of four lanes the second one first, for the banks
           const int first = (part >> 2) & 1, c0 = (part & 3) * 2;
-          *reinterpret_cast<uint4*>(at + (((c0 + first) ^ (row & 7)) << 4)) = first ? h[1] : h[0];
-          *reinterpret_cast<uint4*>(at + (((c0 + 1 - first) ^ (row & 7)) << 4)) = first ? h[0] : h[1];
+          const uint32_t w4[4] = {(first ? r[i].z : r[i].x) ^ 0x80808080u, (first ? r[i].w : r[i].y) ^ 0x80808080u,
+                                  (first ? r[i].x : r[i].z) ^ 0x80808080u, (first ? r[i].y : r[i].w) ^ 0x80808080u};
+          unsigned char* at = tile + (part >> 2) * (64 * 128) + row * 128;
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            *reinterpret_cast<uint4*>(at + (((c0 + (first ^ e)) ^ (row & 7)) << 4)) =
+                make_uint4(codes_f16<0x4140>(w4[2 * e]), codes_f16<0x4342>(w4[2 * e]), codes_f16<0x4140>(w4[2 * e + 1]),
+                           codes_f16<0x4342>(w4[2 * e + 1]));
         }
       };
       int pages = cache_checked(c, entry(g0)), ahead = entry(g0 + 1);
+      uint32_t at = place(g0, pages);
       uint4 kr[kLoads], vr[kLoads];
       float2 am = make_float2(0.f, 0.f);
       float4 mt = make_float4(0.f, -INFINITY, 0.f, 0.f);
@@ -211,9 +217,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
                    ? *(reinterpret_cast<const float2*>(c.amax) + (int64_t)pg * c.n_kv + x.kv) : make_float2(0.f, 0.f);
       };
       if (g0 < ge) {
-        load(c.k_codes, g0, pages, kr);
+        load(c.k_codes, at, kr);
         am = load_amax(pages);
-        load(c.v_codes, g0, pages, vr);
+        load(c.v_codes, at, vr);
         steps();
       }
       for (int gr = g0; gr < ge; ++gr, ++it) {
@@ -227,8 +233,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
         if (lane == 0) mbar_arrive(kfull + st);
         pages = cache_checked(c, ahead);
         ahead = entry(gr + 2);
+        at = place(gr + 1, pages);
         if (gr + 1 < ge) {
-          load(c.k_codes, gr + 1, pages, kr);
+          load(c.k_codes, at, kr);
           am = load_amax(pages);
         }
         if (!(ok = mbar_wait_warp(vempty + st, ((it >> 1) & 1) ^ 1, abort_flag, 41, c.wait_limit))) break;
@@ -237,7 +244,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
         __syncwarp();
         if (lane == 0) mbar_arrive(vfull + st);
         if (gr + 1 < ge) {
-          load(c.v_codes, gr + 1, pages, vr);
+          load(c.v_codes, at, vr);
           steps();
         }
       }
@@ -364,11 +371,12 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
           __syncwarp();
           if (lane == 0) mbar_arrive(sempty);
 
-          float mx = -INFINITY;
+          // scores less the row's offset, in one step; a row without one yet has them whole
+          const float m0 = m == kEmpty ? 0.f : m;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const float f = mt[k].x * sfac;
-            const unsigned long long f2 = f2_pack(f, f), a2 = f2_pack(mt[k].y, mt[k].y);
+            const float f = mt[k].x * sfac, a = mt[k].y - m0;
+            const unsigned long long f2 = f2_pack(f, f), a2 = f2_pack(a, a);
 #pragma unroll
             for (int i = 0; i < 16; i += 2)
               f2_unpack(f2_fma(f2_pack(s[k * 16 + i], s[k * 16 + i + 1]), f2, a2), s[k * 16 + i], s[k * 16 + i + 1]);
@@ -378,33 +386,37 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
             for (int i = 0; i < 64; ++i)
               if (key0 + i >= lim) s[i] = -INFINITY;
           }
+          float mx4[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-          for (int i = 0; i < 64; ++i) mx = fmaxf(mx, s[i]);
-          const bool move = mx > m + (kHead + kSlack);
+          for (int i = 4; i < 64; i += 4)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mx4[e] = fmaxf(mx4[e], s[i + e]);
+          const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+          const bool move = mx > (m == kEmpty ? kEmpty : kHead + kSlack);
           float f = 1.f;
           if (__any_sync(0xffffffffu, move)) {
-            const float mn = fmaxf(m, mx - kHead);
-            f = ex2(m - mn);
-            m = mn;
-            l *= f;
+            const float by = move ? mx - kHead : 0.f;
+            if (move) {
+              f = m == kEmpty ? 0.f : ex2(-by);
+              m = m0 + by;
+              l *= f;
+            }
+#pragma unroll
+            for (int i = 0; i < 64; ++i) s[i] -= by;
           }
           // weights, fp16; the sum before the rounding
           uint32_t p[32];
-          const float nm = -m;
-          const unsigned long long n2 = f2_pack(nm, nm);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            float sum0 = 0.f, sum1 = 0.f;
+            unsigned long long sum2 = 0ull;
 #pragma unroll
             for (int i = 0; i < 16; i += 2) {
-              float a, e2;
-              f2_unpack(f2_add(f2_pack(s[k * 16 + i], s[k * 16 + i + 1]), n2), a, e2);
-              a = ex2(a);
-              e2 = ex2(e2);
-              sum0 += a;
-              sum1 += e2;
+              const float a = ex2(s[k * 16 + i]), e2 = ex2(s[k * 16 + i + 1]);
+              sum2 = f2_add(sum2, f2_pack(a, e2));
               p[k * 8 + i / 2] = pack_f16(a, e2);
             }
+            float sum0, sum1;
+            f2_unpack(sum2, sum0, sum1);
             l = fmaf(sum0 + sum1, mt[k].z, l);
           }
           if (j > 0) {
