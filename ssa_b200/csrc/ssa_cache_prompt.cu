@@ -59,6 +59,24 @@ __device__ __forceinline__ uint64_t desc_channels_inner(uint32_t saddr, uint32_t
          ((uint64_t)1u << 46) | ((uint64_t)2u << 61);
 }
 
+__device__ __forceinline__ bool elect_one() {
+  uint32_t is;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(is));
+  return is != 0;
+}
+
+// Bounded wait of a warp: one look, then polls that may sleep in the hardware,
+// `limit` in all (mbar_wait's, which reports the one that runs out).
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, volatile int* abort, int code, uint32_t limit) {
+  uint32_t there;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(there)
+               : "r"(smem_u32(bar)), "r"(parity)
+               : "memory");
+  const bool ok = there || mbar_wait(bar, parity, abort, code, limit - 1);
+  return __all_sync(0xffffffffu, ok);
+}
+
 // D (+)= A B with A in TMEM.
 __device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
@@ -225,7 +243,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
       for (int gr = g0; gr < ge; ++gr, ++it) {
         const int st = it & 1;
         unsigned char* tile = sm + Sm::kKV + st * 2 * Sm::kTile;
-        if (!(ok = mbar_wait_warp(kempty + st, ((it >> 1) & 1) ^ 1, abort_flag, 31, c.wait_limit))) break;
+        if (!(ok = wait_for(kempty + st, ((it >> 1) & 1) ^ 1, abort_flag, 31, c.wait_limit))) break;
         if (w == kSoftWarps && lane < 4) meta[(it & 3) * 4 + lane] = mt;
         store(tile, kr);
         fence_async_smem();
@@ -238,7 +256,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
           load(c.k_codes, at, kr);
           am = load_amax(pages);
         }
-        if (!(ok = mbar_wait_warp(vempty + st, ((it >> 1) & 1) ^ 1, abort_flag, 41, c.wait_limit))) break;
+        if (!(ok = wait_for(vempty + st, ((it >> 1) & 1) ^ 1, abort_flag, 41, c.wait_limit))) break;
         store(tile + Sm::kTile, vr);
         fence_async_smem();
         __syncwarp();
@@ -251,50 +269,59 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
     }
   } else if (w == kSoftWarps + kConvWarps) {
     // ------------------------------------------------------------ products
-    if (lane == 0) {
-      // One thread issues everything, an instruction every nine cycles or so:
-      // descriptors are made once, and only their address field moves (16-byte
-      // units). Made in place they took the thread longer than the products.
-      const uint64_t q_desc = umma_desc(smem_u32(sm + Sm::kQ));
-      const uint64_t k_desc = umma_desc(smem_u32(sm + Sm::kKV));
-      const uint64_t v_desc = desc_channels_inner(smem_u32(sm + Sm::kKV + Sm::kTile), 64 * 128);
-      constexpr uint32_t kStage = 2 * Sm::kTile / 16;
-      constexpr uint32_t kDescS = idesc_f16(kPromptRows, 64, false), kDescO = idesc_f16(kPromptRows, D, true);
-      bool ok = true;
-      int segs = 0;
-      const auto scores = [&](int i) {
-        const int st = i & 1;
-        if (!mbar_wait(kfull + st, (i >> 1) & 1, abort_flag, 32, c.wait_limit)) return false;
-        if (i && !mbar_wait(sempty, (i - 1) & 1, abort_flag, 33, c.wait_limit)) return false;
-        tc_fence_after();
-        const uint64_t kd = k_desc + (uint32_t)st * kStage;
+    // The warp stays together and one thread of it issues: addresses and
+    // descriptors are then in uniform registers, where the products want them.
+    const bool lead = elect_one();
+    const auto same = [](auto v) { return __shfl_sync(0xffffffffu, v, 0); };
+    const uint32_t tm = same(tmem);
+    const uint64_t q_desc = same(umma_desc(smem_u32(sm + Sm::kQ)));
+    const uint64_t k_desc = same(umma_desc(smem_u32(sm + Sm::kKV)));
+    const uint64_t v_desc = same(desc_channels_inner(smem_u32(sm + Sm::kKV + Sm::kTile), 64 * 128));
+    constexpr uint32_t kStage = 2 * Sm::kTile / 16;
+    constexpr uint32_t kDescS = idesc_f16(kPromptRows, 64, false), kDescO = idesc_f16(kPromptRows, D, true);
+    bool ok = true;
+    int segs = 0;
+    const auto scores = [&](int i) {
+      const int st = i & 1;
+      if (!wait_for(kfull + st, (i >> 1) & 1, abort_flag, 32, c.wait_limit)) return false;
+      if (i && !wait_for(sempty, (i - 1) & 1, abort_flag, 33, c.wait_limit)) return false;
+      tc_fence_after();
+      const uint64_t kd = k_desc + (uint32_t)st * kStage;
+      if (lead) {
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk)
-          umma_bf16(tmem, q_desc + ((kk >> 2) * (kPromptRows * 128) + (kk & 3) * 32) / 16,
+          umma_bf16(tm, q_desc + ((kk >> 2) * (kPromptRows * 128) + (kk & 3) * 32) / 16,
                     kd + ((kk >> 2) * (64 * 128) + (kk & 3) * 32) / 16, kDescS, kk > 0);
         umma_commit(sfull);
         umma_commit(kempty + st);
-        return true;
-      };
-      while (ok && seg.next(c, pl, x, g0, g1, groups)) {
-        const int nb = min(g1, (lim_max_of(c, x) + 63) / 64) - g0;
-        if (nb <= 0) continue;
-        ok = mbar_wait(qfull, segs++ & 1, abort_flag, 34, c.wait_limit) && scores(it);
-        for (int j = 0; ok && j < nb; ++j, ++it) {
-          const int st = it & 1;
-          if (j + 1 < nb && !(ok = scores(it + 1))) break;
-          ok = mbar_wait(vfull + st, (it >> 1) & 1, abort_flag, 35, c.wait_limit) && mbar_wait(pfull, it & 1, abort_flag, 36, c.wait_limit);
-          if (!ok) break;
-          tc_fence_after();
-          const uint64_t vd = v_desc + (uint32_t)st * kStage;
+      }
+      __syncwarp();
+      return true;
+    };
+    while (ok && seg.next(c, pl, x, g0, g1, groups)) {
+      const int nb = same(min(g1, (lim_max_of(c, x) + 63) / 64) - g0);
+      if (nb <= 0) continue;
+      ok = wait_for(qfull, segs++ & 1, abort_flag, 34, c.wait_limit) && scores(it);
+      for (int j = 0; ok && j < nb; ++j, ++it) {
+        const int st = it & 1;
+        if (j + 1 < nb && !(ok = scores(it + 1))) break;
+        ok = wait_for(vfull + st, (it >> 1) & 1, abort_flag, 35, c.wait_limit) &&
+             wait_for(pfull, it & 1, abort_flag, 36, c.wait_limit);
+        if (!ok) break;
+        tc_fence_after();
+        const uint64_t vd = v_desc + (uint32_t)st * kStage;
+        if (lead) {
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)
-            umma_ts(tmem + kColO, tmem + kColP + kk * 8, vd + kk * (16 * 128 / 16), kDescO, (j | kk) > 0);
+            umma_ts(tm + kColO, tm + kColP + kk * 8, vd + kk * (16 * 128 / 16), kDescO, (j | kk) > 0);
           umma_commit(vempty + st);
           umma_commit(odone);
         }
+        __syncwarp();
       }
-      // Products still in flight (also after a wait that ran out) end before TMEM is freed.
+    }
+    // Products still in flight (also after a wait that ran out) end before TMEM is freed.
+    if (lead) {
       umma_commit(mma_done);
       mbar_drain(mma_done, 0);
     }
@@ -357,11 +384,11 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
 
         for (int j = 0; j < nb; ++j, ++it) {
           const int st = it & 1, key0 = (g0 + j) * 64;
-          if (!(ok = mbar_wait_warp(kfull + st, (it >> 1) & 1, abort_flag, 37, c.wait_limit))) break;  // the steps
+          if (!(ok = wait_for(kfull + st, (it >> 1) & 1, abort_flag, 37, c.wait_limit))) break;  // the steps
           float4 mt[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) mt[k] = meta[(it & 3) * 4 + k];
-          if (!(ok = mbar_wait_warp(sfull, it & 1, abort_flag, 38, c.wait_limit))) break;
+          if (!(ok = wait_for(sfull, it & 1, abort_flag, 38, c.wait_limit))) break;
           tc_fence_after();
           float s[64];
           tmem_ld32(trow, s);
@@ -421,7 +448,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
           }
           if (j > 0) {
             // the product before has read P and added to O
-            if (!(ok = mbar_wait_warp(odone, (it - 1) & 1, abort_flag, 39, c.wait_limit))) break;
+            if (!(ok = wait_for(odone, (it - 1) & 1, abort_flag, 39, c.wait_limit))) break;
             tc_fence_after();
             if (__any_sync(0xffffffffu, f != 1.f)) {
 #pragma unroll 1
@@ -443,7 +470,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
           if (lane == 0) mbar_arrive(pfull);
         }
         if (ok) {
-          ok = mbar_wait_warp(odone, (it - 1) & 1, abort_flag, 40, c.wait_limit);
+          ok = wait_for(odone, (it - 1) & 1, abort_flag, 40, c.wait_limit);
           tc_fence_after();
         }
       }
