@@ -451,9 +451,9 @@ __global__ void __launch_bounds__(kThreads) k_cache_combine(const CacheDev c, co
 #pragma unroll
       for (int j = 0; j < kBatch; ++j)
         if (j0 + j < cnt) {
-          const float* p = c.part_o + slot(j0 + j) * D + lane;
+          const float* p = c.part_o + (slot(j0 + j) - r) * D;
 #pragma unroll
-          for (int i = 0; i < E; ++i) batch[j][i] = p[32 * i];
+          for (int i = 0; i < E; ++i) batch[j][i] = p[part_at<ROWS, D>(r, lane + 32 * i)];
         }
     };
     load(0);

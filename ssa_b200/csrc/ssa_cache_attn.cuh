@@ -49,6 +49,13 @@ constexpr int64_t kPromptWork = 1 << 24;
 // Groups of 64 keys that are worth a thread block and its share of the join.
 constexpr int least_groups(int rows) { return rows == kPromptRows ? 4 : 1; }
 
+// Element (row, channel) of a tile's partial sums: row by row, or for 128 rows,
+// written a row a thread, four channels of all rows side by side.
+template <int ROWS, int D>
+__device__ __forceinline__ int part_at(int row, int ch) {
+  return ROWS == kPromptRows ? ((ch >> 2) * ROWS + row) * 4 + (ch & 3) : row * D + ch;
+}
+
 // Blocks that share an SM (registers for 16 and 32 rows, the rings for 8).
 constexpr int blocks_per_sm(int d, int rows) { return rows >= 32 ? 2 : rows == 16 || d >= 96 ? 3 : 4; }
 

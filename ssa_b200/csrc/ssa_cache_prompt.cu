@@ -497,9 +497,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
                 make_uint2(f32_to_bf16_bits(o[i] * inv) | (uint32_t)f32_to_bf16_bits(o[i + 1] * inv) << 16,
                            f32_to_bf16_bits(o[i + 2] * inv) | (uint32_t)f32_to_bf16_bits(o[i + 3] * inv) << 16);
         } else {
-          float* to = c.part_o + (slot + r) * D + ch;
+          float* to = c.part_o + slot * D + part_at<kPromptRows, D>(r, ch);
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(to + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          for (int i = 0; i < 32; i += 4)
+            *reinterpret_cast<float4*>(to + i * kPromptRows) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
         }
       }
       tc_fence_before();
