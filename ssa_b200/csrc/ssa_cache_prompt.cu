@@ -39,11 +39,9 @@ struct PromptSmem {
   static constexpr int kQ = 0;                                         // [kAtoms][128 rows][128 bytes]
   static constexpr int kTile = kAtoms * 64 * 128;                      // [kAtoms][64 keys][128 bytes]
   static constexpr int kKV = kAtoms * kPromptRows * 128;               // [2 stages][K, V] tiles
-  // [4][4] {step_k, log2 step_v, 1 / step_v, -}: K's stage is filled again when
-  // its scores are there, and a row may read these after that; four blocks of
-  // keys on, every row has read the scores of two blocks further.
+  // [2 stages][4] {step_k, log2 step_v, 1 / step_v, -}
   static constexpr int kMeta = kKV + 4 * kTile;
-  static constexpr int kBars = kMeta + 4 * 4 * 16;
+  static constexpr int kBars = kMeta + 2 * 4 * 16;
   static constexpr int kBytes = kBars + 128 + 1024;                    // the base is rounded up to 1024
 };
 
@@ -148,7 +146,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
     for (int i = 0; i < 2; ++i) {
       mbar_init(kfull + i, kConvWarps);
       mbar_init(vfull + i, kConvWarps);
-      mbar_init(kempty + i, 1);
+      mbar_init(kempty + i, 1 + kSoftWarps);
       mbar_init(vempty + i, 1);
     }
     mbar_init(sfull, 1);
@@ -244,7 +242,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
         const int st = it & 1;
         unsigned char* tile = sm + Sm::kKV + st * 2 * Sm::kTile;
         if (!(ok = wait_for(kempty + st, ((it >> 1) & 1) ^ 1, abort_flag, 31, c.wait_limit))) break;
-        if (w == kSoftWarps && lane < 4) meta[(it & 3) * 4 + lane] = mt;
+        if (w == kSoftWarps && lane < 4) meta[st * 4 + lane] = mt;
         store(tile, kr);
         fence_async_smem();
         __syncwarp();
@@ -387,7 +385,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
           if (!(ok = wait_for(kfull + st, (it >> 1) & 1, abort_flag, 37, c.wait_limit))) break;  // the steps
           float4 mt[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) mt[k] = meta[(it & 3) * 4 + k];
+          for (int k = 0; k < 4; ++k) mt[k] = meta[st * 4 + k];
+          __syncwarp();
+          if (lane == 0) mbar_arrive(kempty + st);  // seen: the stage's next phase may come
           if (!(ok = wait_for(sfull, it & 1, abort_flag, 38, c.wait_limit))) break;
           tc_fence_after();
           float s[64];
