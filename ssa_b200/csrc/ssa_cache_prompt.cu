@@ -2,9 +2,9 @@
 // rows (a prompt's chunk, drafts of a multi-query model), on the
 // 5th-generation tensor cores.
 //
-// The mathematics is k_cache_attn's (ssa_cache_attn.cu); with 64 rows and more
-// a kv head the products bound it, and turning codes into fp16 once for every
-// 32 rows. Here 128 rows share the conversion:
+// The mathematics is k_cache_attn's (ssa_cache_attn.cu), whose tiles of 8 to
+// 32 rows read and convert the codes again for every tile. Here 128 rows share
+// that:
 //   warps 4-7 load the codes of 64 keys a block of steps ahead, convert them
 //             to fp16 and store K and V as swizzled 128-byte rows (two stages);
 //   warp 8    issues S = Q K^T (128 x 64 x d, fp32 in TMEM) for the next keys,
@@ -12,9 +12,16 @@
 //             it lies;
 //   warps 0-3 own a row a thread: read S, mask, move the row's offset when a
 //             score outgrows it, and write P = 2^(s - m) as fp16 to TMEM.
-// Two thread blocks share an SM, so one's products run under the other's
-// exponentials: 64 keys take a block 512 cycles of tensor pipe, as many of the
-// exponential unit, and about 500 of issue.
+// It takes over from k_cache_attn at 96 rows a kv head and 2^24 rows x keys
+// (ssa_cache_attn.cuh has the table). Two sequences' 256 tokens behind up to
+// 7936, 32 heads over 8, d 128: 89 us, 440 TFLOP/s of 1679, tensor pipe a
+// quarter busy; the codes are read from L2 at a few percent of its rate. What
+// bounds it is the converting warps: 64 keys take a block about 2700 cycles
+// from store to store, of which they wait some 700, while the rows need 1650
+// and the products 700. Two blocks share an SM, so one's products run under
+// the other's conversion; rows that run further ahead (P in two buffers, a
+// barrier of their own for the steps) only take issue slots from the
+// converting warps and cost 5 and 30 %, and half of Q in TMEM costs 5.
 #include "ssa_cache_attn.cuh"
 #include "ssa_tcgen05.cuh"
 
@@ -190,21 +197,30 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
       const auto place = [&](int gr, int pages) {
         return (uint32_t)(((int64_t)max(pages, 0) * c.n_kv + x.kv) * (c.bs / 16)) + (uint32_t)((gr * 4 + (lane & 3)) & (c.bs / 16 - 1));
       };
-      // piece i of a thread: 16 bytes of the tile's id-th, id = i * kConvThreads + ct
+      // Piece i of a thread: 16 codes of a row, the id-th of the tile. Eight lanes
+      // store 16 bytes at a time: with 128 channels they take four pieces of two
+      // rows, whose swizzled chunks are the even and the odd ones of 128 bytes.
+      const auto piece_of = [&](int i, int& row, int& part) {
+        const int id = i * kConvThreads + ct;
+        row = D == 128 ? (id >> 4) * 2 + (id >> 2 & 1) : id / (D / 16);
+        part = D == 128 ? (id & 3) + (id >> 3 & 1) * 4 : id % (D / 16);
+      };
       const auto load = [&](const int8_t* codes, uint32_t at, uint4 (&r)[kLoads]) {
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-          const int id = i * kConvThreads + ct;
-          const uint32_t rows = __shfl_sync(0xffffffffu, at, id / D);
-          r[i] = *reinterpret_cast<const uint4*>(codes + ((uint64_t)rows * (16 * D) + (unsigned)(id % D * 16)));
+          int row, part;
+          piece_of(i, row, part);
+          const uint32_t rows = __shfl_sync(0xffffffffu, at, row >> 4);
+          r[i] = *reinterpret_cast<const uint4*>(codes + ((uint64_t)rows * (16 * D) + (unsigned)((row & 15) * D + part * 16)));
         }
       };
       const auto store = [&](unsigned char* tile, const uint4 (&r)[kLoads]) {
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-          const int id = i * kConvThreads + ct, row = id / (D / 16), part = id % (D / 16);
-          // chunks 2 part, 2 part + 1 of the row; every other group of four lanes the second one first, for the banks
-          const int first = (part >> 2) & 1, c0 = (part & 3) * 2;
+          int row, part;
+          piece_of(i, row, part);
+          // chunks 2 part, 2 part + 1 of the row (96 channels: the last two pieces' second one first, for the banks)
+          const int first = D == 96 ? part >> 2 : 0, c0 = (part & 3) * 2;
           const uint32_t w4[4] = {(first ? r[i].z : r[i].x) ^ 0x80808080u, (first ? r[i].w : r[i].y) ^ 0x80808080u,
                                   (first ? r[i].x : r[i].z) ^ 0x80808080u, (first ? r[i].y : r[i].w) ^ 0x80808080u};
           unsigned char* at = tile + (part >> 2) * (64 * 128) + row * 128;
@@ -223,8 +239,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
       const auto steps = [&]() {
         if (w == kSoftWarps && lane < 4) {
           const float va = am.y * (1.f / 127.f), vs = va > 0.f ? va : 1.f;
-          // keys without a page: scores of minus infinity; a page of NaN: scores of NaN
-          mt = pages >= 0 ? make_float4(am.x * (1.f / 127.f), __log2f(vs) + (va != va ? va : 0.f), 1.f / vs, 0.f)
+          // keys without a page: scores of minus infinity; a page of NaN: scores of NaN;
+          // 1 / step to two units of the last place is enough for a sum of weights
+          mt = pages >= 0 ? make_float4(am.x * (1.f / 127.f), __log2f(vs) + (va != va ? va : 0.f), __fdividef(1.f, vs), 0.f)
                           : make_float4(0.f, -INFINITY, 0.f, 0.f);
         }
       };
