@@ -34,18 +34,21 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
 }
 
 // Rows of a tile for the kernel that takes many (ssa_cache_prompt.cu). It is
-// taken from 96 rows a kv head where rows x keys, by the table's width, come
-// to 2^24. Measured (us; two kv heads, d 128 / 64):
+// taken from 64 rows a kv head where rows x keys, by the table's width, come
+// to 2^24, or from 256 rows and 2^23. Measured (us; two kv heads, d 128 / 64):
 //   rows  sequences x keys   32-row tiles   128-row tiles
-//     64    32 x 8192          64 / 46         69 / 49
-//    128     1 x 16384         29 / 22         35 / 23
-//    128     8 x 8192          40 / 30         41 / 30     2^24
-//    128    32 x 8192         107 / 77         79 / 55
-//    512     1 x 16384         55 / 40         44 / 31     2^24
-//    512    32 x 8192         403 / 279       223 / 156
-//   2048    32 x 8192        1533 / 1066      735 / 521
-constexpr int kPromptRows = 128, kPromptMin = 96;
-constexpr int64_t kPromptWork = 1 << 24;
+//     64     8 x 8192          30 / 23         32 / 25      2^23
+//     64    32 x 8192          63 / 46         56 / 44
+//    128     1 x 16384         27 / 21         32 / 21
+//    128     8 x 8192          40 / 31         39 / 30      2^24
+//    128    32 x 8192         107 / 77         65 / 49
+//    256     1 x 16384         36 / 28         37 / 24      2^23
+//    512     1 x 2048          24 / 19         26 / 22      2^21
+//    512    32 x 8192         401 / 279       176 / 137
+//   2048     1 x 2048          38 / 30         27 / 21      2^23
+//   2048    32 x 8192        1531 / 1064      575 / 455
+constexpr int kPromptRows = 128, kPromptMin = 64;
+constexpr int64_t prompt_work(int64_t rows) { return rows >= 256 ? 1 << 23 : 1 << 24; }
 // Groups of 64 keys that are worth a thread block and its share of the join.
 constexpr int least_groups(int rows) { return rows == kPromptRows ? 4 : 1; }
 

@@ -12,8 +12,7 @@
 //             it lies;
 //   warps 0-3 own a row a thread: read S, mask, move the row's offset when a
 //             score outgrows it, and write P = 2^(s - m) as fp16 to TMEM.
-// It takes over from k_cache_attn at 96 rows a kv head and 2^24 rows x keys
-// (ssa_cache_attn.cuh has the table). Two sequences' 256 tokens behind up to
+// Where it takes over from k_cache_attn, ssa_cache_attn.cuh has measured. Two sequences' 256 tokens behind up to
 // 7936, 32 heads over 8, d 128: 89 us, 440 TFLOP/s of 1679, tensor pipe a
 // quarter busy; the codes are read from L2 at a few percent of its rate. What
 // bounds it is the converting warps: 64 keys take a block about 2700 cycles

@@ -5,7 +5,7 @@
 //
 // A decoding step makes a few launches of a few microseconds each for every
 // layer, so the way from Python to the launch counts: through ctypes one such
-// call took 14 to 24 us, through this module 5 to 12.
+// call took 14 to 24 us, through this module it takes 5 to 9, launch included.
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>

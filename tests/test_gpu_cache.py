@@ -282,14 +282,15 @@ ATTENDS = [  # dtype, H, n_kv, d, bs, n, lens after the step
     (BF, 8, 8, 32, 16, 70, [300, 70, 75]),
     (BF, 16, 2, 128, 64, 19, [200, 1, 64]),
     (F32, 12, 4, 128, 32, 11, [64, 100]),
-    # the many-row kernel (96 rows a kv head and a wide table)
+    # the many-row kernel (64 rows a kv head and more, and a wide table)
+    (BF, 4, 1, 64, 32, 16, [500, 16, 65]),
     (BF, 6, 2, 96, 32, 40, [200, 41, 0]),
     (BF, 32, 1, 128, 16, 5, [1000, 5, 64]),
     (BF, 4, 2, 64, 64, 300, [1100, 300, 17]),
     (BF, 3, 1, 32, 32, 33, [65, 2000]),
     (BF, 16, 1, 128, 64, 6, [640, 3000, 6, 0]),
 ]
-MANY_ROWS = len(ATTENDS) - 5  # cases from here on
+MANY_ROWS = len(ATTENDS) - 6  # cases from here on
 
 
 def _widen(pool, blocks):
