@@ -460,9 +460,9 @@ __global__ void __launch_bounds__(kThreads) k_cache_combine(const CacheDev c, co
 #pragma unroll
       for (int j = 0; j < kBatch; ++j)
         if (j0 + j < cnt) {
-          const float* p = c.part_o + (slot(j0 + j) - r) * D;
+          const float* p = c.part_o + slot(j0 + j) * D + lane;
 #pragma unroll
-          for (int i = 0; i < E; ++i) batch[j][i] = p[part_at<ROWS, D>(r, lane + 32 * i)];
+          for (int i = 0; i < E; ++i) batch[j][i] = p[32 * i];
         }
     };
     load(0);
@@ -576,10 +576,7 @@ template <int D, bool F32>
 cudaError_t run_attn_rows(const CacheDev& c, cudaStream_t st) {
   const Plan pl = plan_of(c);
   if constexpr (!F32)
-    if (pl.rows == kPromptRows) {
-      const cudaError_t e = launch_cache_prompt(c, pl, st);
-      return e != cudaSuccess ? e : run_combine<D, kPromptRows / 8, false>(c, pl, st);
-    }
+    if (pl.rows == kPromptRows) return launch_cache_prompt(c, pl, st);
   return pl.rows == 8 ? run_attn<D, 1, F32>(c, pl, st) : pl.rows == 16 ? run_attn<D, 2, F32>(c, pl, st)
                                                                        : run_attn<D, 4, F32>(c, pl, st);
 }

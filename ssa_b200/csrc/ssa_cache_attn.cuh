@@ -35,29 +35,24 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
 
 // Rows of a tile for the kernel that takes many (ssa_cache_prompt.cu). It is
 // taken from 64 rows a kv head where rows x keys, by the table's width, come
-// to 2^24, or from 256 rows and 2^23. Measured (us; two kv heads, d 128 / 64):
+// to 3 * 2^22, or from 256 rows and 2^23. Measured (us; two kv heads, d 128 / 64):
 //   rows  sequences x keys   32-row tiles   128-row tiles
-//     64     8 x 8192          30 / 23         32 / 25      2^23
-//     64    32 x 8192          63 / 46         56 / 44
-//    128     1 x 16384         27 / 21         32 / 21
-//    128     8 x 8192          40 / 31         39 / 30      2^24
-//    128    32 x 8192         107 / 77         65 / 49
-//    256     1 x 16384         36 / 28         37 / 24      2^23
-//    512     1 x 2048          24 / 19         26 / 22      2^21
-//    512    32 x 8192         401 / 279       176 / 137
-//   2048     1 x 2048          38 / 30         27 / 21      2^23
-//   2048    32 x 8192        1531 / 1064      575 / 455
+//     64     8 x 8192          30 / 23         29 / 24      2^23
+//     64    32 x 8192          63 / 46         58 / 47
+//     96     8 x 8192          37 / 28         30 / 25      3 * 2^22
+//    128     1 x 16384         27 / 21         28 / 22
+//    128     8 x 8192          40 / 31         31 / 25      2^24
+//    128    32 x 8192         107 / 77         63 / 50
+//    256     1 x 2048          20 / 16         21 / 18
+//    256     1 x 16384         36 / 28         33 / 26      2^23
+//    512     1 x 2048          24 / 19         22 / 19
+//    512    32 x 8192         401 / 279       160 / 124
+//   2048     1 x 2048          38 / 30         29 / 25      2^23
+//   2048    32 x 8192        1531 / 1064      520 / 407
 constexpr int kPromptRows = 128, kPromptMin = 64;
-constexpr int64_t prompt_work(int64_t rows) { return rows >= 256 ? 1 << 23 : 1 << 24; }
+constexpr int64_t prompt_work(int64_t rows) { return rows >= 256 ? 1 << 23 : 3 << 22; }
 // Groups of 64 keys that are worth a thread block and its share of the join.
 constexpr int least_groups(int rows) { return rows == kPromptRows ? 4 : 1; }
-
-// Element (row, channel) of a tile's partial sums: row by row, or for 128 rows,
-// written a row a thread, four channels of all rows side by side.
-template <int ROWS, int D>
-__device__ __forceinline__ int part_at(int row, int ch) {
-  return ROWS == kPromptRows ? ((ch >> 2) * ROWS + row) * 4 + (ch & 3) : row * D + ch;
-}
 
 // Blocks that share an SM (registers for 16 and 32 rows, the rings for 8).
 constexpr int blocks_per_sm(int d, int rows) { return rows >= 32 ? 2 : rows == 16 || d >= 96 ? 3 : 4; }

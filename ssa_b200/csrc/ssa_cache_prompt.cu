@@ -13,8 +13,8 @@
 //   warps 0-3 own a row a thread: read S, mask, move the row's offset when a
 //             score outgrows it, and write P = 2^(s - m) as fp16 to TMEM.
 // Where it takes over from k_cache_attn, ssa_cache_attn.cuh has measured. Two sequences' 256 tokens behind up to
-// 7936, 32 heads over 8, d 128: 89 us, 440 TFLOP/s of 1679, tensor pipe a
-// quarter busy; the codes are read from L2 at a few percent of its rate. What
+// 7936, 32 heads over 8, d 128: 81 us with the join, 487 TFLOP/s of 1679, the
+// tensor pipe 30 % busy; the codes come from L2 at a tenth of its rate. What
 // bounds it is the converting warps: 64 keys take a block about 2700 cycles
 // from store to store, of which they wait some 700, while the rows need 1650
 // and the products 700. Two blocks share an SM, so one's products run under
@@ -38,6 +38,11 @@ constexpr int kConvThreads = kConvWarps * 32;
 // as 72 to the 128 converting threads and 120 to the 128 with a row:
 // 128 * 72 + 128 * 120 + 32 * 96 = 288 * 96.
 constexpr uint32_t kTmemCols = 256, kColP = 64, kColO = 128;  // S at 0
+
+// Element (row, channel) of a tile's partial sums: four channels of all rows
+// side by side, as a row a thread writes them.
+template <int D>
+__device__ __forceinline__ int part_at(int row, int ch) { return ((ch >> 2) * kPromptRows + row) * 4 + (ch & 3); }
 
 template <int D>
 struct PromptSmem {
@@ -513,7 +518,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
                 make_uint2(f32_to_bf16_bits(o[i] * inv) | (uint32_t)f32_to_bf16_bits(o[i + 1] * inv) << 16,
                            f32_to_bf16_bits(o[i + 2] * inv) | (uint32_t)f32_to_bf16_bits(o[i + 3] * inv) << 16);
         } else {
-          float* to = c.part_o + slot * D + part_at<kPromptRows, D>(r, ch);
+          float* to = c.part_o + slot * D + part_at<D>(r, ch);
 #pragma unroll
           for (int i = 0; i < 32; i += 4)
             *reinterpret_cast<float4*>(to + i * kPromptRows) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
@@ -533,15 +538,139 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
 }
 
+// Joins the partial sums of 16 rows of a unit that several blocks worked on, in
+// range order, and writes zeros to rows without work: 16 threads have the rows
+// side by side, as they lie, each of eight such groups every eighth four
+// channels. PARTS groups of 128 threads share the sums where few units have
+// many. One set-up serves 16 rows: with k_cache_combine's warp a row the call
+// above took 89 us. Batches of two sums leave registers for twice the blocks
+// that batches of four do (81 against 85 us).
+constexpr int kJoinRows = 16, kJoinThreads = 128;
+
+template <int D, int PARTS>
+__global__ void __launch_bounds__(kJoinThreads * PARTS) k_cache_join(const CacheDev c, const Plan pl, const int ngrid) {
+  constexpr int E = D / 32, kBatch = 2, kBlocks = kPromptRows / kJoinRows;
+  __shared__ __align__(16) float s_o[PARTS][kJoinRows][D + 4];
+  __shared__ float2 s_ml[PARTS][kJoinRows];
+  const int t = threadIdx.x % kJoinThreads, part = threadIdx.x / kJoinThreads, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int jr = t % kJoinRows, cg = t / kJoinRows;
+  const unsigned unit = blockIdx.x / kBlocks, units_b = (unsigned)pl.tiles_max * c.n_kv;
+  const int r0 = (int)(blockIdx.x % kBlocks) * kJoinRows;
+  const int b = (int)(unit / units_b), u = (int)(unit % units_b);
+  // Lengths may be read before the wait: the other kernel lets this one come up
+  // only after its own.
+  int tiles, groups;
+  const int mine = seq_work(c, pl, b, kPromptRows, &tiles, &groups);
+  const Unit x = unit_of<kPromptRows>(c, pl, b, u, pl.tiles_max);
+  int total = 0, base = 0;
+  if (c.B <= 128) {
+    for (int i = lane; i < c.B; i += 32) {
+      int a, e;
+      const int v = seq_work(c, pl, i, kPromptRows, &a, &e);
+      total += v;
+      base += i < b ? v : 0;
+    }
+    total = __reduce_add_sync(0xffffffffu, total);
+    base = __reduce_add_sync(0xffffffffu, base);
+  }
+  grid_wait();
+  const int rows = min(kPromptRows, c.n * c.rep - x.row0) - r0;  // of this block, in the padded step
+  if (rows <= 0) return;
+  int c0 = 0, c1 = 0;
+  const bool work = x.tile < tiles && mine > 0;
+  if (work) {
+    if (c.B > 128) {
+      total = c.prefix[c.B];
+      base = c.prefix[b];
+    }
+    const int ubeg = base + (x.kv * tiles + x.tile) * groups;
+    const Ranges rg(total, ngrid, least_groups(kPromptRows));
+    c0 = rg.of(ubeg);
+    c1 = rg.of(ubeg + groups - 1);
+  }
+  const auto joined = [&](int row) { return work && row < x.nrows; };
+  if (work && c0 == c1 && r0 + min(rows, kJoinRows) <= x.nrows) return;  // that block stored the rows
+
+  const int r = r0 + jr;
+  float m = kEmpty, l = 0.f;
+  float4 o[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (joined(r) && c0 != c1) {
+    const int cnt = (c1 - c0 + PARTS - part) / PARTS;  // sums part, part + PARTS, ...
+    const auto slot = [&](int i) {
+      const int k = c0 + part + i * PARTS;
+      return ((int64_t)k * 2 + (k == c0)) * kPromptRows;
+    };
+    for (int i = 0; i < cnt; ++i) m = fmaxf(m, c.part_ml[(slot(i) + r) * 2]);
+    for (int i0 = 0; i0 < cnt; i0 += kBatch) {
+      float4 v[kBatch][E];
+      float2 ml[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i)
+        if (i0 + i < cnt) {
+          const int64_t s = slot(i0 + i);
+          ml[i] = *reinterpret_cast<const float2*>(c.part_ml + (s + r) * 2);
+#pragma unroll
+          for (int e = 0; e < E; ++e) v[i][e] = *reinterpret_cast<const float4*>(c.part_o + s * D + part_at<D>(r, (cg + 8 * e) * 4));
+        }
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i)
+        if (i0 + i < cnt) {
+          const float f = ex2(ml[i].x - m);
+          l = fmaf(f, ml[i].y, l);
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            o[e].x = fmaf(f, v[i][e].x, o[e].x);
+            o[e].y = fmaf(f, v[i][e].y, o[e].y);
+            o[e].z = fmaf(f, v[i][e].z, o[e].z);
+            o[e].w = fmaf(f, v[i][e].w, o[e].w);
+          }
+        }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) *reinterpret_cast<float4*>(&s_o[part][jr][(cg + 8 * e) * 4]) = o[e];
+  if (cg == 0) s_ml[part][jr] = make_float2(m, l);
+  __syncthreads();
+
+  for (int j = w; j < min(rows, kJoinRows); j += kJoinThreads * PARTS / 32) {
+    if (joined(r0 + j) && c0 == c1) continue;
+    float mj = kEmpty, lj = 0.f;
+#pragma unroll
+    for (int k = 0; k < PARTS; ++k) mj = fmaxf(mj, s_ml[k][j].x);
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < PARTS; ++k) {
+      const float f = PARTS == 1 ? 1.f : ex2(s_ml[k][j].x - mj);
+      lj = fmaf(f, s_ml[k][j].y, lj);
+      if (lane < D / 4) {
+        const float4 a = *reinterpret_cast<const float4*>(&s_o[k][j][lane * 4]);
+        v = make_float4(fmaf(f, a.x, v.x), fmaf(f, a.y, v.y), fmaf(f, a.z, v.z), fmaf(f, a.w, v.w));
+      }
+    }
+    const float inv = lj == 0.f ? 0.f : 1.f / lj;
+    if (lane < D / 4) store_out<false>(c, x, r0 + j, lane * 4, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+    if (lane == 0 && c.lse) store_lse(c, x, r0 + j, mj, lj);
+  }
+}
+
 template <int D>
 cudaError_t run_prompt(const CacheDev& c, const Plan& pl, cudaStream_t st) {
   constexpr size_t smem = PromptSmem<D>::kBytes;
-  const cudaError_t e = allow_smem<k_cache_prompt<D>>(smem);
+  cudaError_t e = allow_smem<k_cache_prompt<D>>(smem);
   if (e != cudaSuccess) return e;
+  const int64_t units = (int64_t)c.B * c.n_kv * pl.tiles_max, joins = units * (kPromptRows / kJoinRows);
+  if (joins > 0x7fffffff) return cudaErrorInvalidConfiguration;
   CacheLaunch l((unsigned)c.grid, kThreads, smem, st);
-  const cudaError_t e2 = cudaLaunchKernelEx(&l.cfg, k_cache_prompt<D>, c, pl);
+  e = cudaLaunchKernelEx(&l.cfg, k_cache_prompt<D>, c, pl);
   note_launch();
-  return e2;
+  if (e != cudaSuccess) return e;
+  const bool wide = c.grid > 16 * units;  // a unit may have more sums than a batch or two
+  CacheLaunch j((unsigned)joins, kJoinThreads * (wide ? 4 : 1), 0, st);
+  e = wide ? cudaLaunchKernelEx(&j.cfg, k_cache_join<D, 4>, c, pl, c.grid) : cudaLaunchKernelEx(&j.cfg, k_cache_join<D, 1>, c, pl, c.grid);
+  note_launch();
+  return e;
 }
 
 }  // namespace
