@@ -12,15 +12,17 @@
 //             it lies;
 //   warps 0-3 own a row a thread: read S, mask, move the row's offset when a
 //             score outgrows it, and write P = 2^(s - m) as fp16 to TMEM.
-// Where it takes over from k_cache_attn, ssa_cache_attn.cuh has measured. Two sequences' 256 tokens behind up to
-// 7936, 32 heads over 8, d 128: 81 us with the join, 487 TFLOP/s of 1679, the
-// tensor pipe 30 % busy; the codes come from L2 at a tenth of its rate. What
-// bounds it is the converting warps: 64 keys take a block about 2700 cycles
-// from store to store, of which they wait some 700, while the rows need 1650
-// and the products 700. Two blocks share an SM, so one's products run under
-// the other's conversion; rows that run further ahead (P in two buffers, a
-// barrier of their own for the steps) only take issue slots from the
-// converting warps and cost 5 and 30 %, and half of Q in TMEM costs 5.
+// Where it takes over from k_cache_attn, ssa_cache_attn.cuh has measured.
+//
+// Two sequences' 256 tokens behind up to 7936, 32 heads over 8, d 128: 81 us
+// with the join, 487 TFLOP/s of 1679, the tensor pipe 30 % busy; the codes come
+// from L2 at a tenth of its rate. What bounds it is the converting warps: by
+// the clock, 64 keys take them about 3200 cycles, of which they wait 700, while
+// the rows compute for 1650 and the products are issued in 700. Two blocks
+// share an SM, so one's products run under the other's conversion. Rows that
+// run further ahead only take issue slots from the converting warps (P in two
+// buffers: 5 % slower; a barrier of their own for the steps: 30 %); half of Q
+// in TMEM, which spares the products shared memory: 5 % slower.
 #include "ssa_cache_attn.cuh"
 #include "ssa_tcgen05.cuh"
 
