@@ -40,6 +40,11 @@ void need_cuda(const Tensor& t) {
     raise(PyExc_RuntimeError, "ssa_b200 runs on CUDA tensors only (there is no CPU path); got a tensor on " + t.device().str());
 }
 
+void no_gradient(const Tensor& t, const char* what) {
+  if (t.requires_grad() && at::GradMode::is_enabled())
+    raise(PyExc_RuntimeError, std::string(what) + " has no gradient: call it under torch.no_grad()");
+}
+
 int dtype_code(const Tensor& t) {
   if (t.scalar_type() == at::kFloat) return SSA_F32;
   if (t.scalar_type() == at::kBFloat16) return SSA_BF16;
@@ -149,6 +154,8 @@ optional<std::tuple<Tensor, Tensor>> cache_append(const Tensor& k_in, const Tens
                                                   const Tensor& lens, bool want_values) {
   need_cuda(k_in);
   need_cuda(v_in);
+  no_gradient(k_in, "cache_append");
+  no_gradient(v_in, "cache_append");
   if (k_in.scalar_type() != v_in.scalar_type() || k_in.sizes() != v_in.sizes() || k_in.device() != v_in.device())
     raise(PyExc_ValueError, "k " + shape_of(k_in) + " and v " + shape_of(v_in) + " differ in type, shape or device");
   const Tensor k = rows(k_in), v = rows(v_in);
@@ -215,8 +222,7 @@ std::tuple<Tensor, optional<Tensor>> cache_attention(const Tensor& q_in, const T
                                                      const Tensor& lens, double scale, const optional<Tensor>& blocks,
                                                      bool causal, bool want_lse) {
   need_cuda(q_in);
-  if (q_in.requires_grad() && at::GradMode::is_enabled())
-    raise(PyExc_RuntimeError, "cache_attention has no gradient: call it under torch.no_grad()");
+  no_gradient(q_in, "cache_attention");
   const Tensor q = rows(q_in);
   const int64_t B = q.size(0), H = q.size(1), n = q.size(2), d = q.size(3);
   if (k_codes.dim() != 4) raise(PyExc_ValueError, "k_codes (num_pages, n_kv, block_size, d) expected, got " + shape_of(k_codes));

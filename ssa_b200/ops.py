@@ -448,7 +448,8 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, k_codes: torch.Tensor, v_code
     position start[b] + i, rows from lens[b] - start[b] on are padding -- to
     the cache in 8 bits (ssa_cache_append). Writes k_codes, v_codes, amax,
     bounds and tail in place; with want_values returns (k, v) as the cache now
-    holds them, (B, n_kv, n, d) in the input's type, 0 for padding."""
+    holds them, (B, n_kv, n, d) in the input's type, 0 for padding. No
+    gradient: refuses tensors that ask for one."""
     return (_torch_ext or _load_torch()).cache_append(k, v, k_codes, v_codes, amax, bounds, tail, table, start, lens,
                                                       want_values)
 

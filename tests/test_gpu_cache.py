@@ -594,18 +594,36 @@ def test_offsets_beyond_32_bits(n, cuda):
         assert torch.equal(a, b)
 
 
-def test_attention_of_many_sequences(cuda):
-    """More sequences than a thread block has threads."""
+@pytest.mark.parametrize("n", [1, 24])
+def test_attention_of_many_sequences(n, cuda):
+    """More sequences than a thread block has threads; n = 24 with a wide table
+    is the many-row kernel's."""
     B, n_kv, H, d, bs = 700, 1, 3, 32, 16
     g = torch.Generator().manual_seed(13)
     lens = torch.randint(0, 60, (B,), generator=g).tolist()
     pool = Pool(cuda, B, n_kv, d, bs, 4, BF)
     pool.advance(lens)
     pool.append(_kv(g, B, 60, n_kv, d, BF, cuda), _kv(g, B, 60, n_kv, d, BF, cuda))
-    pool.start = (pool.lens - 1).clamp(min=0)
-    q = _kv(g, B, 1, H, d, BF, cuda)
+    pool.start = (pool.lens - n).clamp(min=0)
+    if n > 1:
+        _widen(pool, 24)
+    q = _kv(g, B, n, H, d, BF, cuda)
     out, lse = pool.attend(q, 0.2, want_lse=True)
     _check_attention(pool, q, out, lse, 0.2)
+
+
+def test_gradients_are_refused(cuda):
+    pool, q = _filled(0, cuda)
+    want = pool.attend(q, 0.1)
+    k = torch.randn(pool.B, pool.n_kv, 1, pool.d, device=cuda, dtype=BF, requires_grad=True)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        pool.attend(q.clone().requires_grad_(), 0.1)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        pool.append(k, k.detach())
+    with pytest.raises(RuntimeError, match="no gradient"):
+        pool.append(k.detach(), k)
+    with torch.no_grad():
+        assert torch.equal(pool.attend(q.clone().requires_grad_(), 0.1), want)
 
 
 def test_other_stream(cuda):
