@@ -251,7 +251,8 @@ __device__ __forceinline__ void append_block(const CacheDev& c, int b, int kv, i
   constexpr int kSize = DT == kDtF32 ? 4 : 2;
   const int tid = threadIdx.x, cv = tid % kVec, r0 = tid / kVec;
   const int p0 = blk * BS;
-  const int page = p0 < len ? cache_page(c, b, blk) : -1;  // a block of padding is only cleared in the values
+  // a block of padding, or of a sequence without new tokens, is only cleared in the values
+  const int page = p0 < len && start < len ? cache_page(c, b, blk) : -1;
   // rows of the block: [0, old) from the tail, [old, end) from the input, the rest absent
   const int old = page < 0 ? 0 : max(0, min(BS, start - p0)), end = page < 0 ? 0 : min(BS, len - p0);
   char* values = static_cast<char*>(s ? c.v_values : c.k_values);

@@ -199,6 +199,30 @@ def test_reserve_equals_sequential(B, n, bs, max_blocks, free, cuda):
             assert torch.equal(L.cpu(), lens) and torch.equal(St.cpu(), state)
 
 
+@pytest.mark.parametrize("want_values", [False, True])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_append_leaves_sequences_without_new_tokens_alone(dtype, want_values, cuda):
+    """A sequence whose length stays (within a block, at its edge, empty) keeps
+    its pages, bounds and tail, whatever they hold; its values are 0."""
+    g = torch.Generator().manual_seed(14)
+    lens = [21, 32, 0, 16 * 3 - 1, 40]
+    pool = Pool(cuda, 5, 2, 64, 16, 5, dtype, seed=3)
+    pool.lens = torch.tensor(lens, dtype=torch.int32, device=cuda)
+    pool.start = pool.lens.clone()
+    pool.start[4] = 38  # the last one gets two tokens
+    pool.tail = torch.randn(pool.tail.shape, generator=g).to(dtype).to(cuda)
+    before = [t.clone() for t in (pool.k, pool.v, pool.amax, pool.bounds, pool.tail)]
+    x = _kv(g, 5, 2, 2, 64, dtype, cuda)
+    out = pool.append(x, x, want_values=want_values)
+    mine = pool.table[4].long()
+    for t, old in zip((pool.k, pool.v, pool.amax, pool.bounds), before):
+        t[mine] = old[mine]
+        assert torch.equal(t, old)
+    assert torch.equal(pool.tail[:4], before[4][:4])
+    if want_values:
+        assert all(float(o[:4].abs().max()) == 0 and float(o[4].abs().max()) > 0 for o in out)
+
+
 # ---------------------------------------------------------------- select
 SELECTS = [  # dtype, H, n_kv, d, bs, n, lens after the step, top, sink, local
     (BF, 8, 2, 128, 64, 1, [64 * 40, 1, 700], 8, 1, 1),
