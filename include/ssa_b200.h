@@ -337,7 +337,8 @@ SSA_API int ssa_cache_append(const ssa_cache_params* p, const void* k, const voi
  * upper bound of q8 . key over the block's keys, q8 the token's q in 8 bits
  * under one amax for the group's heads. Blocks up to the token's own stand for
  * election; the first `sink` and last `local` >= 1 of them are always listed
- * (sink + local <= top); ties go to the lowest block. blocks_out (B, n, n_kv,
+ * (sink + local <= top); ties go to the lowest block, and a block whose score is
+ * NaN (it stands for NaN) comes before every other. blocks_out (B, n, n_kv,
  * top) int32, ascending, -1 behind (tokens behind a sequence's last: all -1).
  */
 SSA_API int ssa_cache_select(const ssa_cache_params* p, const void* q, const int8_t* bounds, const float* amax,

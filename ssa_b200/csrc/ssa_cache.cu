@@ -453,12 +453,11 @@ __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, ui
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Ordered like the double, above 0 and below ~0 - 1 (which no number reaches,
-// but a NaN might).
+// Ordered like the double, above 0 and below ~0 - 1. A NaN (of a block that
+// stands for NaN) comes before every number, whatever its bits.
 __device__ __forceinline__ unsigned long long order_key(double v) {
   const unsigned long long u = (unsigned long long)__double_as_longlong(v + 0.0);  // -0 -> 0
-  const unsigned long long k = (u >> 63) ? ~u : u | (1ull << 63);
-  return max(1ull, min(k, ~0ull - 2));
+  return v != v ? ~0ull - 2 : (u >> 63) ? ~u : u | (1ull << 63);
 }
 
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
@@ -742,7 +741,8 @@ __global__ void __launch_bounds__(kSelThreads, 2) k_cache_select(const CacheDev 
       }
       __syncthreads();
       const unsigned long long from = lo + ((unsigned long long)s_bin << sh);
-      const unsigned long long upto = from + ((1ull << sh) - 1);
+      // a bin's end may lie beyond hi, and for infinite scores beyond 64 bits
+      const unsigned long long width = 1ull << sh, upto = hi - from < width ? hi : from + (width - 1);
       const int cnt = s_cnt;
       rem -= s_above;
       if (cnt <= rem) {  // the whole bin
