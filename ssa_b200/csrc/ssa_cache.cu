@@ -79,15 +79,25 @@ __global__ void __launch_bounds__(kReserveThreads) k_cache_reserve(const Reserve
       const int64_t want = (after + r.bs - 1) / r.bs;
       const bool wide = want > r.max_blocks;
       const int need = wide ? 0 : (int)(want - held);
-      int total;
-      const int upto = block_scan(need, part, total);
+      // 1024 needs of 2^21 pages each would pass 32 bits: wider tables add them up in two halves
+      int64_t upto, total;
+      if (r.max_blocks < (1 << 21)) {
+        int sum;
+        upto = block_scan(need, part, sum);
+        total = sum;
+      } else {
+        int high, low;
+        upto = (int64_t)block_scan(need >> 16, part, high) << 16;
+        upto += block_scan(need & 0xffff, part, low);
+        total = ((int64_t)high << 16) + low;
+      }
       const bool ok = !wide && (need == 0 || before + upto <= count);
       if (lengths) {
         if (b < r.B) {
           r.start_out[b] = len;
           r.lens_out[b] = ok ? (int)after : len;
         }
-        const int given = __reduce_max_sync(0xffffffffu, ok && need ? (int)before + upto : 0);
+        const int given = __reduce_max_sync(0xffffffffu, ok && need ? (int)(before + upto) : 0);
         const int refused = __popc(__ballot_sync(0xffffffffu, b < r.B && !ok));
         if (lane == 0 && given) atomicMax(&s_given, given);
         if (lane == 0 && refused) atomicAdd(&s_refused, refused);
