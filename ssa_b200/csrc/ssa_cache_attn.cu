@@ -46,12 +46,17 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   return y;
 }
 
-// High part and remainder of a pair.
+// High part and remainder of a pair; of a pair of weights.
 __device__ __forceinline__ void split_f16(float a, float b, uint32_t& hi, uint32_t& lo) {
   const __half2 h = __floats2half2_rn(a, b);
   const float2 f = __half22float2(h);
   hi = *reinterpret_cast<const uint32_t*>(&h);
   lo = pack_f16(a - f.x, b - f.y);
+}
+__device__ __forceinline__ void split_weights(float a, float b, uint32_t& hi, uint32_t& lo) {
+  hi = pack_weights(a, b);
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+  lo = pack_weights(a - f.x, b - f.y);
 }
 
 // Shared memory of a block: for each warp a ring of staged tiles (keys and
@@ -263,7 +268,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, 8 * NT) + (NT == 1)
       }
 
       // weights 2^(s' + log2(step_v) - m + 13)
-      const float vs = va > 0.f ? va : 1.f;  // a page of zeros: any step does
+      const float vs = va > 0.f ? va : 1.f;
+      const float head = va == 0.f ? kHead + kZeroHead : kHead;
       const float lv = (F32 ? log2f(vs) : __log2f(vs)) + (va != va ? va : 0.f), iv = 1.f / vs;
       const bool edge = kbj + 16 > lim_min;
       bool move = false;
@@ -274,7 +280,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, 8 * NT) + (NT == 1)
           float v = fmaf(s[nt][k] + s2[nt][k], ka * sfac[nt][k & 1], lv);
           if (edge && kbj + g + 8 * (k >> 1) >= lim[nt][k & 1]) v = -INFINITY;
           s[nt][k] = v;
-          move |= v > mref[nt][k & 1] + (kHead + kSlack);
+          move |= v > mref[nt][k & 1] + (head + kSlack);
         }
       if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
@@ -285,7 +291,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, 8 * NT) + (NT == 1)
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-            m = fmaxf(mref[nt][k], m - kHead);
+            m = fmaxf(mref[nt][k], m - head);
             const float f = ex2(mref[nt][k] - m);
             mref[nt][k] = m;
             lsum[nt][k] *= f;
@@ -306,15 +312,15 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, 8 * NT) + (NT == 1)
         lsum[nt][1] = fmaf(p[1] + p[3], iv, lsum[nt][1]);
         if constexpr (F32) {
           uint32_t h0, l0, h1, l1;
-          split_f16(p[0], p[1], h0, l0);
-          split_f16(p[2], p[3], h1, l1);
+          split_weights(p[0], p[1], h0, l0);
+          split_weights(p[2], p[3], h1, l1);
           pf[0][nt][0] = transpose8x8(h0);
           pf[0][nt][1] = transpose8x8(h1);
           pf[PC - 1][nt][0] = transpose8x8(l0);
           pf[PC - 1][nt][1] = transpose8x8(l1);
         } else {
-          pf[0][nt][0] = transpose8x8(pack_f16(p[0], p[1]));
-          pf[0][nt][1] = transpose8x8(pack_f16(p[2], p[3]));
+          pf[0][nt][0] = transpose8x8(pack_weights(p[0], p[1]));
+          pf[0][nt][1] = transpose8x8(pack_weights(p[2], p[3]));
         }
       }
 

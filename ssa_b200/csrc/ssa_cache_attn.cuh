@@ -13,6 +13,13 @@ constexpr int kGroup = 64;       // keys a block takes at a time
 constexpr float kEmpty = -1e30f; // offset of a row that has seen no key
 constexpr float kHead = 13.f;    // weights run up to 2^13, and 2^15 before the offset moves
 constexpr float kSlack = 2.f;
+// A page of V that is all zeros has a share in the weights' sum only. Its step
+// counts as one, and its scores move the offset only so that its weights stay
+// below 2^(13 + 48): at a step of one they would hide pages whose values are
+// small (a score 12 octaves up beside an amax of 1e-4 cost 8 % of the output).
+// 48 octaves keep the bits of every page with an amax above 2^-57, and the
+// weights' sum right for those below 2^60.
+constexpr float kZeroHead = 48.f;
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -31,6 +38,13 @@ __device__ __forceinline__ uint32_t codes_f16(uint32_t biased) {
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
+}
+// Weights: those of a page of zeros may lie beyond fp16's range and become its
+// largest number (infinity times a code of 0 would be NaN).
+__device__ __forceinline__ uint32_t pack_weights(float lo, float hi) {
+  uint32_t v;
+  asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(v) : "f"(hi), "f"(lo));
+  return v;
 }
 
 // Rows of a tile for the kernel that takes many (ssa_cache_prompt.cu). It is

@@ -52,7 +52,7 @@ struct PromptSmem {
   static constexpr int kQ = 0;                                         // [kAtoms][128 rows][128 bytes]
   static constexpr int kTile = kAtoms * 64 * 128;                      // [kAtoms][64 keys][128 bytes]
   static constexpr int kKV = kAtoms * kPromptRows * 128;               // [2 stages][K, V] tiles
-  // [2 stages][4] {step_k, log2 step_v, 1 / step_v, -}
+  // [2 stages][4] {step_k, log2 step_v, 1 / step_v, octaves kept from moving the offset}
   static constexpr int kMeta = kKV + 4 * kTile;
   static constexpr int kBars = kMeta + 2 * 4 * 16;
   static constexpr int kBytes = kBars + 128 + 1024;                    // the base is rounded up to 1024
@@ -247,7 +247,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
           const float va = am.y * (1.f / 127.f), vs = va > 0.f ? va : 1.f;
           // keys without a page: scores of minus infinity; a page of NaN: scores of NaN;
           // 1 / step to two units of the last place is enough for a sum of weights
-          mt = pages >= 0 ? make_float4(am.x * (1.f / 127.f), __log2f(vs) + (va != va ? va : 0.f), __fdividef(1.f, vs), 0.f)
+          mt = pages >= 0 ? make_float4(am.x * (1.f / 127.f), __log2f(vs) + (va != va ? va : 0.f), __fdividef(1.f, vs),
+                                        va == 0.f ? kZeroHead : 0.f)
                           : make_float4(0.f, -INFINITY, 0.f, 0.f);
         }
       };
@@ -436,11 +437,13 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
             for (int i = 0; i < 64; ++i)
               if (key0 + i >= lim) s[i] = -INFINITY;
           }
-          float mx4[4] = {s[0], s[1], s[2], s[3]};
+          float mx4[4] = {s[0], s[16], s[32], s[48]};
 #pragma unroll
-          for (int i = 4; i < 64; i += 4)
+          for (int i = 1; i < 16; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) mx4[e] = fmaxf(mx4[e], s[i + e]);
+            for (int k = 0; k < 4; ++k) mx4[k] = fmaxf(mx4[k], s[k * 16 + i]);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) mx4[k] -= mt[k].w;
           const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
           const bool move = mx > (m == kEmpty ? kEmpty : kHead + kSlack);
           float f = 1.f;
@@ -463,7 +466,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
             for (int i = 0; i < 16; i += 2) {
               const float a = ex2(s[k * 16 + i]), e2 = ex2(s[k * 16 + i + 1]);
               sum2 = f2_add(sum2, f2_pack(a, e2));
-              p[k * 8 + i / 2] = pack_f16(a, e2);
+              p[k * 8 + i / 2] = pack_weights(a, e2);
             }
             float sum0, sum1;
             f2_unpack(sum2, sum0, sum1);
