@@ -350,7 +350,8 @@ SSA_API int ssa_cache_select(const ssa_cache_params* p, const void* q, const int
  * or the distinct blocks that `blocks` (B, n, n_kv, top) lists for the token
  * and kv head (entries out of range are left out). out (B, H, n, d) per o_s*
  * strides; lse (B, H, n) fp32, optional. Rows without a key, and rows behind a
- * sequence's last token, are 0 with lse -inf. Needs
+ * sequence's last token, are 0 with lse -inf. A seen page of V that stands for
+ * NaN makes out NaN; lse is of the keys alone. Needs
  * ssa_cache_attn_workspace_size(p, blocks != NULL) bytes.
  */
 SSA_API size_t ssa_cache_attn_workspace_size(const ssa_cache_params* p, int32_t with_blocks);

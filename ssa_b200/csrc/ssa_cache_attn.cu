@@ -268,9 +268,9 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, 8 * NT) + (NT == 1)
       }
 
       // weights 2^(s' + log2(step_v) - m + 13)
-      const float vs = va > 0.f ? va : 1.f;
-      const float head = va == 0.f ? kHead + kZeroHead : kHead;
-      const float lv = (F32 ? log2f(vs) : __log2f(vs)) + (va != va ? va : 0.f), iv = 1.f / vs;
+      const bool plain = va > 0.f && va < INFINITY;
+      const float vs = plain ? va : 1.f, head = plain ? kHead : kHead + kZeroHead;
+      const float lv = F32 ? log2f(vs) : __log2f(vs), iv = 1.f / vs;
       const bool edge = kbj + 16 > lim_min;
       bool move = false;
 #pragma unroll
@@ -340,6 +340,15 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, 8 * NT) + (NT == 1)
             mma_f16(acc[i][nt], a, pf[pc][nt][0], pf[pc][nt][1]);
             mma_f16(acc[i + 1][nt], e, pf[pc][nt][0], pf[pc][nt][1]);
           }
+      }
+      if (!(va < INFINITY)) {  // V stands for NaN where a key is seen; the weights' sum is K's alone
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+            if (kbj < lim[nt][k])
+#pragma unroll
+              for (int i = 0; i < W16; ++i) acc[i][nt][k] = acc[i][nt][k + 2] = NAN;
       }
     }
     __syncwarp();

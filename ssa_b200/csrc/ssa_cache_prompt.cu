@@ -52,7 +52,7 @@ struct PromptSmem {
   static constexpr int kQ = 0;                                         // [kAtoms][128 rows][128 bytes]
   static constexpr int kTile = kAtoms * 64 * 128;                      // [kAtoms][64 keys][128 bytes]
   static constexpr int kKV = kAtoms * kPromptRows * 128;               // [2 stages][K, V] tiles
-  // [2 stages][4] {step_k, log2 step_v, 1 / step_v, octaves kept from moving the offset}
+  // [2 stages][4] {step_k, log2 step_v, 1 / step_v (negative where V stands for NaN), octaves kept from moving the offset}
   static constexpr int kMeta = kKV + 4 * kTile;
   static constexpr int kBars = kMeta + 2 * 4 * 16;
   static constexpr int kBytes = kBars + 128 + 1024;                    // the base is rounded up to 1024
@@ -244,11 +244,13 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
       float4 mt = make_float4(0.f, -INFINITY, 0.f, 0.f);
       const auto steps = [&]() {
         if (w == kSoftWarps && lane < 4) {
-          const float va = am.y * (1.f / 127.f), vs = va > 0.f ? va : 1.f;
-          // keys without a page: scores of minus infinity; a page of NaN: scores of NaN;
+          const float va = am.y * (1.f / 127.f);
+          const bool plain = va > 0.f && va < INFINITY;
+          const float vs = plain ? va : 1.f;
+          // keys without a page: scores of minus infinity; a page of K that stands for NaN: scores of NaN;
           // 1 / step to two units of the last place is enough for a sum of weights
-          mt = pages >= 0 ? make_float4(am.x * (1.f / 127.f), __log2f(vs) + (va != va ? va : 0.f), __fdividef(1.f, vs),
-                                        va == 0.f ? kZeroHead : 0.f)
+          mt = pages >= 0 ? make_float4(am.x * (1.f / 127.f), __log2f(vs), va < INFINITY ? __fdividef(1.f, vs) : -1.f,
+                                        plain ? 0.f : kZeroHead)
                           : make_float4(0.f, -INFINITY, 0.f, 0.f);
         }
       };
@@ -365,6 +367,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
       // A row behind the last one computes the first row's scores over all keys,
       // stale ones too: its offset is out of reach, so that it moves nothing.
       float m = have ? kEmpty : -kEmpty, l = 0.f;
+      bool bad = false;  // the row sees a page of V that stands for NaN: its output is NaN, the weights' sum is K's alone
       if (nb > 0) {
         // Q: rows into their swizzled places as they come, 8 bytes a lane, then
         // each thread turns its own into fp16 where it lies, scaled by a power of
@@ -412,6 +415,11 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
           for (int k = 0; k < 4; ++k) mt[k] = meta[st * 4 + k];
           __syncwarp();
           if (lane == 0) mbar_arrive(kempty + st);  // seen: the stage's next phase may come
+          if (fminf(fminf(mt[0].z, mt[1].z), fminf(mt[2].z, mt[3].z)) < 0.f) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (mt[k].z < 0.f && key0 + 16 * k < lim) bad = true;
+          }
           if (!(ok = wait_for(sfull, it & 1, abort_flag, 38, c.wait_limit))) break;
           tc_fence_after();
           float s[64];
@@ -470,7 +478,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
             }
             float sum0, sum1;
             f2_unpack(sum2, sum0, sum1);
-            l = fmaf(sum0 + sum1, mt[k].z, l);
+            l = fmaf(sum0 + sum1, fabsf(mt[k].z), l);
           }
           if (j > 0) {
             // the product before has read P and added to O
@@ -515,6 +523,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_cache_prompt(const CacheDev c, 
           for (int i = 0; i < 32; ++i) o[i] = 0.f;
         }
         if (!have) continue;
+        if (bad)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = NAN;
         if (full) {
           uint16_t* to = static_cast<uint16_t*>(c.out) + o_at + ch;
 #pragma unroll

@@ -1,5 +1,5 @@
 """Cache attention where the pages of V differ: a page of zeros beside small
-values."""
+values, and pages that stand for NaN, which only the output may see."""
 import math
 
 import pytest
@@ -102,3 +102,40 @@ def test_only_zeros(cuda):
             reach = float((q[b, h, t].cpu().double().abs() @ ks.abs().T * 0.125).max())
             ref = float(torch.logsumexp(s * 0.125, 0))
             assert abs(float(lse[b, h, t]) - ref) <= (d + 8) * 2.0 ** -23 * reach + 2.0 ** -17 + abs(ref) * 2.0 ** -22
+
+@pytest.mark.parametrize("listed", [False, True])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("case", range(len(ZEROS)))
+def test_lse_does_not_depend_on_values(case, value, listed, cuda):
+    """A page of V that is not finite makes the outputs of the rows that see it
+    NaN. Their lse, and rows before the page or without it in their list, do not
+    see it."""
+    dtype, _, H, d = ZEROS[case]
+    n, bs, L = 20, 16, 70
+    g = torch.Generator().manual_seed(case)
+    pool = Pool(cuda, 2, 1, d, bs, 6, dtype, seed=case)
+    k, v = _kv(g, 2, L, 1, d, dtype, cuda), _kv(g, 2, L, 1, d, dtype, cuda)
+    v[1, 0, 58, 7] = value  # block 3, positions 48 .. 63
+    pool.advance([L, L])
+    pool.append(k, v)
+    pool.start = pool.lens - n  # rows at 50 .. 69 ...
+    pool.start[1] = 40          # ... and 40 .. 59 of a sequence of 60: the first eight end before the block
+    pool.lens[1] = 60
+    q = _kv(g, 2, n, H, d, dtype, cuda)
+    blocks = None
+    if listed:
+        blocks = torch.tensor([0, 2, 3, -1], dtype=torch.int32).expand(2, n, 1, 4).contiguous()
+        blocks[1, ::3] = torch.tensor([2, 1, -1, 0], dtype=torch.int32)
+        blocks = blocks.to(cuda)
+    elif H >= 64:
+        _widen(pool, -(-2 ** 24 // (2 * n * H * bs)))
+    out, lse = pool.attend(q, 0.1, blocks=blocks, want_lse=True)
+    count = 0
+    for b, h, t, s, vs, ks in _rows(pool, q, None if blocks is None else blocks.cpu()):
+        bad = bool(torch.isnan(vs).any() | torch.isinf(vs).any())
+        count += bad
+        assert bool(torch.isnan(out[b, h, t]).all()) == bad and bool(torch.isfinite(out[b, h, t]).all()) != bad, (b, h, t)
+        reach = float((q[b, h, t].cpu().double().abs() @ ks.abs().T * 0.1).max())
+        ref = float(torch.logsumexp(s * 0.1, 0))
+        assert abs(float(lse[b, h, t]) - ref) <= (d + 8) * 2.0 ** -23 * reach + 2.0 ** -17 + abs(ref) * 2.0 ** -22, (b, h, t)
+    assert count == H * (8 if listed else 12)
