@@ -446,16 +446,23 @@ class SparseAttention(nn.Module):
 
     @torch.no_grad()
     def prefill(self, x: torch.Tensor, cache: BlockCache, layer: int = 0) -> torch.Tensor:
-        """`forward` of a prompt x (B, N, d_model) over its sparse graph, storing
-        its keys and values as the step's tokens: call `cache.reserve(N)` before
-        (once for all layers). Returns (B, N, d_model)."""
+        """`forward` of prompts x (B, N, d_model) over their sparse graph, storing
+        their keys and values as the step's tokens: call `cache.reserve(N,
+        prompt=True)`, or with each sequence's own length, before (once for all
+        layers). As in `step`, rows behind a sequence's new tokens come from zero
+        attention, and so do all rows of one that `reserve` refused or that had
+        tokens before. Returns (B, N, d_model)."""
         B, N, _ = x.shape
         q = self._split_q(self.Wq(x))
         k = self._split_kv_grouped(self.Wk(x))
         v = self._split_kv_grouped(self.Wv(x))
         cache.append(k, v, layer)
         nb, valid = self._graph(q, k, N, self.config.causal, False)
+        new = torch.where(cache.start == 0, cache.lens, 0)
+        if cache.ragged:  # every row has the global tokens among its neighbors, in the padding too
+            valid.masked_fill_(nb >= new[:, None, None, None], 0)
         out = ops.gather_attention(q, k, v, nb, valid, self.scale, self.config.fp32_attn_weights)
+        out.masked_fill_((torch.arange(N, device=x.device) >= new[:, None])[:, None, :, None], 0.0)
         return self.Wo(out.transpose(1, 2).reshape(B, N, self.H * self.d_head))
 
     @torch.no_grad()
@@ -529,10 +536,19 @@ class SparseTransformer(nn.Module):
                           num_blocks=num_blocks, top_blocks=top_blocks, dtype=w.dtype, device=w.device)
 
     @torch.no_grad()
-    def prefill(self, x, cache: BlockCache) -> torch.Tensor:
-        """`forward` of the prompts x ((B, N) ids or (B, N, d_model)) of an empty
-        cache, over the sparse graph, filling the cache. Returns (B, N, d_model)."""
-        return self._cached(x, cache, x.shape[1], True)
+    def prefill(self, x, cache: BlockCache, new_lens: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """`forward` of the prompts x ((B, N) ids or (B, N, d_model)) over the
+        sparse graph, filling the cache. new_lens (B,) int32: how many of a row's
+        N tokens are real; 0 for the sequences of a running batch that get no
+        prompt now, which stay as they are. (The graph's bucket planes follow N,
+        so a short row's graph is that of the padded batch.) Only an empty sequence
+        takes a prompt: one that has tokens keeps them and is counted in
+        `cache.refused()`, as one is that the cache has no room for. Rows behind a
+        sequence's tokens, and all rows of a refused one, come from zero attention.
+        Returns (B, N, d_model)."""
+        if new_lens is not None and not self.layers[0].attn.config.causal:
+            raise ValueError("SparseTransformer.prefill: new_lens needs config.causal=True: the tokens would attend the padding")
+        return self._cached(x, cache, x.shape[1] if new_lens is None else new_lens, True)
 
     @torch.no_grad()
     def step(self, x, cache: BlockCache, new_lens: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -545,7 +561,7 @@ class SparseTransformer(nn.Module):
     def _cached(self, x, cache, new_lens, prompt):
         if self.embed is not None:
             x = self.embed(x)
-        cache.reserve(new_lens)
+        cache.reserve(new_lens, prompt)
         for i, layer in enumerate(self.layers):
             x = layer.step(x, cache, i, prompt)
         return self.norm(x)

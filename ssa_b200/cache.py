@@ -71,19 +71,29 @@ class BlockCache:
         self.lens = torch.zeros(batch, dtype=torch.int32, device=device)
         self.free = torch.arange(P - 1, -1, -1, dtype=torch.int32, device=device)
         self.state = torch.tensor([P, 0], dtype=torch.int32, device=device)
+        self.ragged = False  # the present step's lengths may differ
         # the layers' tensors, sliced once: a slice costs as much as a launch
         self._layers = [(self.k_codes[i], self.v_codes[i], self.amax[i], self.bounds[i], self.tail[i]) for i in range(L)]
 
     # -- lengths and pages ---------------------------------------------------
-    def reserve(self, new_lens: Union[int, torch.Tensor]) -> None:
+    def reserve(self, new_lens: Union[int, torch.Tensor], prompt: bool = False) -> None:
         """Begins a step of new_lens more tokens (an int for all sequences, or
         (batch,) int32 on the device): start becomes the present lengths, lens
         the new ones, and the blocks they open get pages. A sequence for which
         the table or the pool has no room keeps its length -- its tokens of
-        this step are not stored and their outputs are 0 -- and is counted in
-        `refused()`."""
-        if not torch.is_tensor(new_lens):
+        this step are not stored and their attention is 0 -- and is counted in
+        `refused()`. With `prompt` the same holds for a sequence that has
+        tokens already and is given more."""
+        self.ragged = torch.is_tensor(new_lens)
+        if not self.ragged:
             new_lens = torch.full_like(self.lens, new_lens)
+        elif new_lens.shape != self.lens.shape or new_lens.dtype != torch.int32 or new_lens.device != self.lens.device:
+            raise ValueError(f"BlockCache.reserve: new_lens must be a ({self.batch},) int32 tensor on {self.lens.device}, got "
+                             f"{new_lens.dtype} {tuple(new_lens.shape)} on {new_lens.device}")
+        if prompt:
+            late = (self.lens > 0) & (new_lens > 0)
+            new_lens = new_lens.masked_fill(late, 0)
+            self.state[1] += late.sum()
         ops.cache_reserve(self.lens, new_lens, self.table, self.free, self.state, self.block_size,
                           out=(self.start, self.lens, self.state))
 
