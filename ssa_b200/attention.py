@@ -554,14 +554,15 @@ class SparseTransformer(nn.Module):
     def step(self, x, cache: BlockCache, new_lens: Optional[torch.Tensor] = None) -> torch.Tensor:
         """The model over the next tokens of every sequence, x (B, n) ids or
         (B, n, d_model), reading and extending `cache`. new_lens (B,) int32: how
-        many of a row's n tokens are real (the others' outputs mean nothing).
+        many of a row's n tokens are real (the others' outputs mean nothing; more
+        than n counts as n).
         Returns (B, n, d_model)."""
         return self._cached(x, cache, x.shape[1] if new_lens is None else new_lens, False)
 
     def _cached(self, x, cache, new_lens, prompt):
         if self.embed is not None:
             x = self.embed(x)
-        cache.reserve(new_lens, prompt)
+        cache.reserve(new_lens, prompt, x.shape[1])
         for i, layer in enumerate(self.layers):
             x = layer.step(x, cache, i, prompt)
         return self.norm(x)

@@ -72,24 +72,33 @@ class BlockCache:
         self.free = torch.arange(P - 1, -1, -1, dtype=torch.int32, device=device)
         self.state = torch.tensor([P, 0], dtype=torch.int32, device=device)
         self.ragged = False  # the present step's lengths may differ
+        self.rows: Optional[int] = None  # the most tokens a sequence has in it, where the host knows
         # the layers' tensors, sliced once: a slice costs as much as a launch
         self._layers = [(self.k_codes[i], self.v_codes[i], self.amax[i], self.bounds[i], self.tail[i]) for i in range(L)]
 
     # -- lengths and pages ---------------------------------------------------
-    def reserve(self, new_lens: Union[int, torch.Tensor], prompt: bool = False) -> None:
+    def reserve(self, new_lens: Union[int, torch.Tensor], prompt: bool = False, limit: Optional[int] = None) -> None:
         """Begins a step of new_lens more tokens (an int for all sequences, or
         (batch,) int32 on the device): start becomes the present lengths, lens
         the new ones, and the blocks they open get pages. A sequence for which
         the table or the pool has no room keeps its length -- its tokens of
         this step are not stored and their attention is 0 -- and is counted in
         `refused()`. With `prompt` the same holds for a sequence that has
-        tokens already and is given more."""
+        tokens already and is given more. limit: the rows that the step's
+        tensors have; greater entries of a tensor new_lens are cut to it (without
+        it they must not be greater: a token that is counted and never appended
+        stands for whatever its page held before)."""
         self.ragged = torch.is_tensor(new_lens)
+        self.rows = limit if self.ragged else new_lens
         if not self.ragged:
+            if limit is not None and new_lens > limit:
+                raise ValueError(f"BlockCache.reserve: {new_lens} new tokens, but {limit} rows")
             new_lens = torch.full_like(self.lens, new_lens)
         elif new_lens.shape != self.lens.shape or new_lens.dtype != torch.int32 or new_lens.device != self.lens.device:
             raise ValueError(f"BlockCache.reserve: new_lens must be a ({self.batch},) int32 tensor on {self.lens.device}, got "
                              f"{new_lens.dtype} {tuple(new_lens.shape)} on {new_lens.device}")
+        elif limit is not None:
+            new_lens = new_lens.clamp(max=limit)
         if prompt:
             late = (self.lens > 0) & (new_lens > 0)
             new_lens = new_lens.masked_fill(late, 0)
@@ -119,7 +128,10 @@ class BlockCache:
 
     # -- one layer -----------------------------------------------------------
     def append(self, k: torch.Tensor, v: torch.Tensor, layer: int = 0, want_values: bool = False):
-        """Stores the step's k, v (batch, n_kv, n, d) (ops.cache_append)."""
+        """Stores the step's k, v (batch, n_kv, n, d) (ops.cache_append), n at
+        least what `reserve` was given."""
+        if self.rows is not None and k.dim() == 4 and k.shape[2] < self.rows:
+            raise ValueError(f"BlockCache.append: {k.shape[2]} rows, but up to {self.rows} new tokens were reserved")
         kc, vc, am, bd, tail = self._layers[layer]
         return ops.cache_append(k, v, kc, vc, am, bd, tail, self.table, self.start, self.lens, want_values)
 

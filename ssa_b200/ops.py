@@ -445,8 +445,8 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, k_codes: torch.Tensor, v_code
                  bounds: torch.Tensor, tail: torch.Tensor, table: torch.Tensor, start: torch.Tensor,
                  lens: torch.Tensor, want_values: bool = False):
     """Appends the step's tokens k, v (B, n_kv, n, d) -- row i of sequence b is
-    position start[b] + i, rows from lens[b] - start[b] on are padding -- to
-    the cache in 8 bits (ssa_cache_append). Writes k_codes, v_codes, amax,
+    position start[b] + i, rows from lens[b] - start[b] (at most n) on are padding --
+    to the cache in 8 bits (ssa_cache_append). Writes k_codes, v_codes, amax,
     bounds and tail in place; with want_values returns (k, v) as the cache now
     holds them, (B, n_kv, n, d) in the input's type, 0 for padding. No
     gradient: refuses tensors that ask for one."""
