@@ -481,7 +481,9 @@ class SparseAttention(nn.Module):
         if cache.top_blocks is not None:
             sink, local = self.cached_blocks(cache.block_size)
             blocks = cache.select(q, layer, sink=sink, local=local)
-        out = cache.attend(q, self.scale, layer, blocks)
+        # the kernels keep an fp32 q's weights to 22 bits, a bf16 q's to fp16's 11
+        wide = q.float() if self.config.fp32_attn_weights else q
+        out = cache.attend(wide, self.scale, layer, blocks).to(q.dtype)
         return self.Wo(out.transpose(1, 2).reshape(B, n, self.H * self.d_head))
 
 

@@ -473,7 +473,9 @@ def cache_attention(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tenso
     at position start[b] + i and sees keys up to itself (causal) or all lens[b].
     Returns out (B, H, n, d) in the (B, n, H, d) layout the output projection
     reads and, with want_lse, the fp32 log of the weights' sum (B, H, n). Rows
-    without a key and padding rows are 0 and -inf. Inference only: no gradient."""
+    without a key and padding rows are 0 and -inf. The weights that meet V are
+    rounded to 11 bits (fp16) for a bf16 q, to 22 for an fp32 one; the sums are
+    fp32. Inference only: no gradient."""
     out, lse = (_torch_ext or _load_torch()).cache_attention(q, k_codes, v_codes, amax, table, start, lens, scale, blocks,
                                                              causal, want_lse)
     return (out, lse) if want_lse else out

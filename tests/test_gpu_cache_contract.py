@@ -1,0 +1,43 @@
+"""What a step promises beside its values: fp32 weights where the config asks
+for them."""
+import pytest
+import torch
+
+import cache_ref as R
+from ssa_b200 import BlockCache, SSAConfig, SparseAttention
+from test_gpu_serving import CFG
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("top", [None, 3])
+def test_step_with_fp32_weights(top, cuda):
+    """config.fp32_attn_weights: two tokens of nearly the same weight whose values
+    nearly cancel. Weights of 11 bits leave up to 2^-12 of the values each; the
+    output has to be right to 2^-19 of them and its own rounding."""
+    torch.manual_seed(0)
+    cfg = SSAConfig(d_model=128, num_heads=1, **{**CFG, "fp32_attn_weights": True})
+    attn = SparseAttention(cfg).to(cuda, torch.bfloat16)
+    eye = torch.eye(128, dtype=torch.bfloat16, device=cuda)
+    with torch.no_grad():
+        for w in (attn.Wq, attn.Wk, attn.Wv, attn.Wo):
+            w.weight.copy_(eye)
+        attn.Wk.weight[64:] = 0  # scores are of the first half
+    g = torch.Generator().manual_seed(2)
+    for _ in range(8):
+        x = torch.zeros(1, 3, 128)
+        x[0, :, :64] = 0.1 * torch.randn(3, 64, generator=g)
+        far = 8 * torch.randn(64, generator=g)
+        x[0, 0, 64:], x[0, 1, 64:] = far, -far
+        cache = BlockCache(1, 1, 128, 64, block_size=16, top_blocks=top, dtype=torch.bfloat16)
+        cache.reserve(3)
+        out = attn.step(x.to(cuda, torch.bfloat16), cache)[0, 2].double().cpu()
+        k, v = (t[0, 0, :3].double().cpu() for t in cache.values())
+        q = x[0, 2].to(torch.bfloat16).double()
+        ref, _, vmax, reach = R.attend(q[None], k, v, torch.ones(1, 3, dtype=torch.bool), attn.scale)
+        ref, vmax, reach = ref[0], float(vmax[0]), float(reach[0])
+        # weights to 2^-21 with the exponential's 2^-21 and the scores' error; bf16 output, and Wo's rounding of it
+        tol = 2 * 2.0 ** -8 * ref.abs() + (2 * 136 * 2.0 ** -23 * reach + 2.0 ** -19) * vmax
+        err = (out - ref).abs()
+        assert (err <= tol).all(), float((err / tol).max())
+        assert ref.abs().max() > 0
