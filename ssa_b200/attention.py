@@ -444,6 +444,25 @@ class SparseAttention(nn.Module):
         G = self.config.num_global_tokens if idx is None else max(idx, default=-1) + 1
         return -(-max(G, 0) // block_size), 1 + -(-self.config.window_size // block_size)
 
+    def check_cache(self, x: torch.Tensor, cache: BlockCache, prompt: bool = False) -> None:
+        """Raises where `prefill` (prompt) or `step` of x's rows cannot use
+        `cache`. A model asks before it reserves, so that a call that is refused
+        leaves the cache as it was."""
+        for name, want, have in (("batch", x.shape[0], cache.batch), ("num_kv_heads", self.n_kv, cache.num_kv_heads),
+                                 ("head_dim", self.d_head, cache.head_dim)):
+            if want != have:
+                raise ValueError(f"the cache's {name} is {have}, {want} needed")
+        if not torch.is_autocast_enabled(x.device.type) and cache.tail.dtype != self.Wk.weight.dtype:
+            raise ValueError(f"the cache's dtype is {cache.tail.dtype}, {self.Wk.weight.dtype} needed")
+        if prompt:
+            return
+        if not self.config.causal:
+            raise ValueError("SparseAttention.step needs config.causal=True: a token cannot attend what is not there yet")
+        if cache.top_blocks is not None and sum(self.cached_blocks(cache.block_size)) > cache.top_blocks:
+            sink, local = self.cached_blocks(cache.block_size)
+            raise ValueError(f"the cache's top_blocks is {cache.top_blocks}: less than the global tokens' ({sink}) and the window's "
+                             f"({local}) blocks of {cache.block_size}")
+
     @torch.no_grad()
     def prefill(self, x: torch.Tensor, cache: BlockCache, layer: int = 0) -> torch.Tensor:
         """`forward` of prompts x (B, N, d_model) over their sparse graph, storing
@@ -452,6 +471,7 @@ class SparseAttention(nn.Module):
         layers). As in `step`, rows behind a sequence's new tokens come from zero
         attention, and so do all rows of one that `reserve` refused or that had
         tokens before. Returns (B, N, d_model)."""
+        self.check_cache(x, cache, True)
         B, N, _ = x.shape
         q = self._split_q(self.Wq(x))
         k = self._split_kv_grouped(self.Wk(x))
@@ -472,8 +492,7 @@ class SparseAttention(nn.Module):
         global tokens' and the window's blocks and those of the highest bound of
         q.k up to that number. Call `cache.reserve(n)` before (once for all
         layers). Rows behind a sequence's new tokens come from zero attention."""
-        if not self.config.causal:
-            raise ValueError("SparseAttention.step needs config.causal=True: a token cannot attend what is not there yet")
+        self.check_cache(x, cache)
         B, n, _ = x.shape
         q = self._split_q(self.Wq(x))
         cache.append(self._split_kv_grouped(self.Wk(x)), self._split_kv_grouped(self.Wv(x)), layer)
@@ -562,6 +581,9 @@ class SparseTransformer(nn.Module):
         return self._cached(x, cache, x.shape[1] if new_lens is None else new_lens, False)
 
     def _cached(self, x, cache, new_lens, prompt):
+        if cache.num_layers < len(self.layers):
+            raise ValueError(f"the cache's num_layers is {cache.num_layers}, {len(self.layers)} needed")
+        self.layers[0].attn.check_cache(x, cache, prompt)
         if self.embed is not None:
             x = self.embed(x)
         cache.reserve(new_lens, prompt, x.shape[1])

@@ -1,11 +1,11 @@
 """What a step promises beside its values: fp32 weights where the config asks
-for them."""
+for them, and refusals that leave the cache as it was."""
 import pytest
 import torch
 
 import cache_ref as R
-from ssa_b200 import BlockCache, SSAConfig, SparseAttention
-from test_gpu_serving import CFG
+from ssa_b200 import BlockCache, SSAConfig, SparseAttention, SparseTransformer
+from test_gpu_serving import CFG, _model
 
 pytestmark = pytest.mark.gpu
 
@@ -41,3 +41,31 @@ def test_step_with_fp32_weights(top, cuda):
         err = (out - ref).abs()
         assert (err <= tol).all(), float((err / tol).max())
         assert ref.abs().max() > 0
+
+
+def _snapshot(cache):
+    return [t.clone() for t in (cache.lens, cache.start, cache.state, cache.table, cache.k_codes, cache.v_codes, cache.amax,
+                                cache.bounds, cache.tail)]
+
+
+def test_a_refused_step_leaves_the_cache(cuda):
+    """What step and prefill can refuse they refuse before a page is taken."""
+    m = _model(torch.bfloat16, cuda)
+    ids = torch.randint(0, 50, (2, 5), device=cuda)
+    mk = lambda **kw: BlockCache(**{**dict(batch=2, num_kv_heads=2, head_dim=64, max_tokens=64, num_layers=2, block_size=16), **kw})  # noqa: E731
+    wide = {**CFG, "global_token_indices": [0, 100]}  # seven leading blocks of 16 are always attended
+    far = SparseTransformer(SSAConfig(d_model=256, num_heads=4, num_kv_heads=2, **wide), 2, 50).to(cuda, torch.bfloat16).eval()
+    full = SparseTransformer(SSAConfig(d_model=256, num_heads=4, num_kv_heads=2, **{**CFG, "causal": False}), 2, 50).to(
+        cuda, torch.bfloat16).eval()
+    for model, cache, what in ((m, mk(batch=3), "batch"), (m, mk(num_kv_heads=1), "num_kv_heads"), (m, mk(head_dim=32), "head_dim"),
+                               (m, mk(num_layers=1), "num_layers"), (far, mk(top_blocks=8), "top_blocks"), (full, mk(), "causal")):
+        before = _snapshot(cache)
+        calls = [lambda: model.step(ids, cache)]
+        if what not in ("top_blocks", "causal"):
+            calls.append(lambda: model.prefill(ids, cache))
+        for call in calls:
+            with pytest.raises(ValueError, match=what):
+                call()
+        for a, b in zip(before, _snapshot(cache)):
+            assert torch.equal(a, b), what
+    far.step(ids, mk(top_blocks=9))
