@@ -43,6 +43,8 @@ void need_cuda(const Tensor& t) {
 void no_gradient(const Tensor& t, const char* what) {
   if (t.requires_grad() && at::GradMode::is_enabled())
     raise(PyExc_RuntimeError, std::string(what) + " has no gradient: call it under torch.no_grad()");
+  if (t._fw_grad(/*level=*/0).defined())  // a dual tensor: no_grad() does not end forward mode
+    raise(PyExc_RuntimeError, std::string(what) + " has no gradient: its tensors may not have tangents (forward mode)");
 }
 
 int dtype_code(const Tensor& t) {

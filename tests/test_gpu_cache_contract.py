@@ -1,10 +1,11 @@
 """What a step promises beside its values: fp32 weights where the config asks
-for them, and refusals that leave the cache as it was."""
+for them, refusals that leave the cache as it was, and no silent tangents."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import cache_ref as R
-from ssa_b200 import BlockCache, SSAConfig, SparseAttention, SparseTransformer
+from ssa_b200 import BlockCache, SSAConfig, SparseAttention, SparseTransformer, ops
 from test_gpu_serving import CFG, _model
 
 pytestmark = pytest.mark.gpu
@@ -69,3 +70,22 @@ def test_a_refused_step_leaves_the_cache(cuda):
         for a, b in zip(before, _snapshot(cache)):
             assert torch.equal(a, b), what
     far.step(ids, mk(top_blocks=9))
+
+
+def test_tangents_are_refused(cuda):
+    """A dual tensor's tangent is not dropped without a word, under no_grad either."""
+    cache = BlockCache(1, 2, 64, 64, block_size=16)
+    x = torch.randn(1, 2, 3, 64, device=cuda, dtype=torch.bfloat16)
+    cache.reserve(3)
+    cache.append(x, x)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for grad in (torch.enable_grad, torch.no_grad):
+            with grad():
+                for call in (lambda: cache.append(dual, x), lambda: cache.append(x, dual), lambda: cache.attend(dual, 0.1)):
+                    with pytest.raises(RuntimeError, match="no gradient"):
+                        call()
+        plain = forward_ad.unpack_dual(dual).primal
+        assert torch.equal(cache.attend(plain, 0.1), cache.attend(x, 0.1))
+        assert ops.cache_select(dual, cache.bounds[0], cache.amax[0], cache.table, cache.start, cache.lens, 2, 16).dtype == torch.int32
+    assert torch.equal(cache.attend(dual, 0.1), cache.attend(x, 0.1))  # the level is over: no tangent
