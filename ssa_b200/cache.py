@@ -4,8 +4,8 @@ and values, and the single-token (or few-token) step over it.
 `SparseAttention`'s LSH graph is a function of the whole key set (bucket
 tables, first-C members, a plane count that follows the length), so it is not
 carried forward by a token; the reference has no serving form either. A step
-takes its neighbours from the cache instead: the blocks whose bound of q.k is
-highest stand in for the LSH candidates, beside the window's and the global
+takes its neighbours from the cache instead: the blocks whose bound of q.k (q
+in 8 bits) is highest stand in for the LSH candidates, beside the window's and the global
 tokens' blocks, or -- without a block budget -- the whole sequence.
 
 A `BlockCache` holds the buffers of `num_layers` layers that share one block
@@ -34,7 +34,8 @@ class BlockCache:
     One step is `reserve` (once), then for each layer `append` and `attend`
     (with `select` between them for a block budget) -- what
     `SparseAttention.step` does. start / lens (batch,) are the lengths before
-    and after the current step.
+    and after the current step. Tokens are not taken back: a completed block no
+    longer has its tokens as they came.
     """
 
     def __init__(self, batch: int, num_kv_heads: int, head_dim: int, max_tokens: int, *, num_layers: int = 1,

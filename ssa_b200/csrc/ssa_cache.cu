@@ -248,9 +248,10 @@ constexpr int kAppendThreads = BS * D / 16 < (D == 96 ? 192 : 256) ? BS * D / 16
 //
 // Bound by HBM and, nearly as much, by the arithmetic of the codes (a multiply
 // and two additions each, packed in pairs): 16 prompts of up to 8192 tokens, 8
-// heads of 128 channels, read 402 MB and write 594 MB in 214 us, 4.65 TB/s of
-// a copy's 6.55 at 57 % of the issue slots. More than half of it is writes,
-// and writes alone (a fill) run at 3.9 TB/s. Resident thread blocks that send
+// heads of 128 channels, read 388 MB and write 582 MB in 209 to 216 us, 4.5 TB/s
+// of a copy's 6.55 at 57 % of the issue slots. More than half of it is writes,
+// and writes alone (a fill of 563 MB) run at 3.85 TB/s. Without the values, as
+// the models call it, it reads 388 MB and writes 194 in 165 us. Resident thread blocks that send
 // for the next block's rows while they write this one were slower (235 us).
 template <int DT, int D, int BS>
 __device__ __forceinline__ void append_block(const CacheDev& c, int b, int kv, int s, int blk, int start, int len,

@@ -13,6 +13,10 @@ namespace ssa {
 // still run, and waits for its end -- with it everything that one waited for
 // -- before it reads anything; then it lets the next one come up. Loads are
 // plain ones: a read-only load might be moved above the wait.
+// Two kernels read before their wait: k_cache_combine and k_cache_join take
+// start and lens while the attention they join still runs. That is sound only
+// because they are launched directly behind it and it lets them come up after
+// its own wait, so launch_dependents has to stay behind the wait.
 __device__ __forceinline__ void grid_wait() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");

@@ -9,18 +9,20 @@
 //   O^T (channels x rows) = V^T . P^T  (V codes as fp16, exact)
 // so eight rows fill an instruction; q and the weights P are fp16 -- q scaled
 // by a power of two for each row (a bf16 q is then exact), P below 2^15 -- or,
-// for fp32 tensors, fp16 pairs (high part and remainder, 22 bits). Sums are
-// fp32. The step of V, which differs from page to page, goes into the
+// for fp32 tensors, fp16 pairs (high part and remainder, 22 bits). fp16 is what
+// the products take beside codes that are exact in it: a weight is then off by
+// 2^-12 of itself where a bf16 output is by 2^-9, and the weights' sum takes
+// them before that rounding. Sums are fp32. The step of V, which differs from page to page, goes into the
 // exponent: P = 2^(s' + log2(step) - m), and the weights' sum takes P / step.
 // mma.sync rather than tcgen05: with 8 to 32 rows the operation is bound by
 // reading the codes, and a 128-row tile would be mostly padding.
 //
 // Measured: 32 sequences of up to 8192 keys, 32 heads over 8, d 128 (408 MB):
-// 72 to 78 us, 5.2 to 5.7 TB/s of a copy's 6.55. The same of 64 listed blocks
-// for 16 sequences (135 MB): 33 us, 4.1 TB/s -- as long as a launch's start,
+// 74 to 80 us, 5.1 to 5.5 TB/s of a copy's 6.55. The same of 64 listed blocks
+// for 16 sequences (135 MB): 33 to 34 us, 4.0 TB/s -- as long as a launch's start,
 // the first look-ups and the join weigh at that size. One fp32 sequence of 333
 // keys: 8 us, two launches. Four drafts of 32 heads over one (8 x 8192 keys,
-// d 64, four tiles of 32 rows): 22 us, bound by latency and the exponentials.
+// d 64, four tiles of 32 rows): 23 us, bound by latency and the exponentials.
 //
 // Work is counted in groups of 64 keys over all (sequence, row tile, kv head)
 // units and cut into one equal range for each thread block, so ragged batches

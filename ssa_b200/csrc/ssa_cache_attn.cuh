@@ -63,6 +63,13 @@ __device__ __forceinline__ uint32_t pack_weights(float lo, float hi) {
 //    512    32 x 8192         401 / 279       160 / 124
 //   2048     1 x 2048          38 / 30         29 / 25      2^23
 //   2048    32 x 8192        1531 / 1064      520 / 407
+// Those tables are as wide as the sequences are long; the host knows no lengths,
+// so a wider one may bring the 128-row tiles to shorter sequences. Measured at
+// the same lengths (us, d 128, table of the length against 64 times it):
+//     64    32 x 512  22.5 -> 19.2     64    8 x 1024  15.8 -> 16.6
+//     64    32 x 1024 28.2 -> 24.5     64    1 x 2048  12.7 -> 16.4
+//    128     8 x 1024 21.9 -> 17.3     64   64 x 128   20.5 -> 24.1
+//    256     8 x 512  22.4 -> 18.7    512    2 x 512   15.9 -> 16.6
 constexpr int kPromptRows = 128, kPromptMin = 64;
 constexpr int64_t prompt_work(int64_t rows) { return rows >= 256 ? 1 << 23 : 3 << 22; }
 // Groups of 64 keys that are worth a thread block and its share of the join.

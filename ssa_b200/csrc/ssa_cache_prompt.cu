@@ -14,8 +14,8 @@
 //             score outgrows it, and write P = 2^(s - m) as fp16 to TMEM.
 // Where it takes over from k_cache_attn, ssa_cache_attn.cuh has measured.
 //
-// Two sequences' 256 tokens behind up to 7936, 32 heads over 8, d 128: 81 us
-// with the join, 487 TFLOP/s of 1679, the tensor pipe 30 % busy; the codes come
+// Two sequences' 256 tokens behind up to 7936, 32 heads over 8, d 128: 82 to 84
+// us with the join, 475 TFLOP/s of 1679, the tensor pipe 29 % busy; the codes come
 // from L2 at a tenth of its rate. What bounds it is the converting warps: by
 // the clock, 64 keys take them about 3200 cycles, of which they wait 700, while
 // the rows compute for 1650 and the products are issued in 700. Two blocks

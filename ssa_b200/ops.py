@@ -458,9 +458,11 @@ def cache_select(q: torch.Tensor, bounds: torch.Tensor, amax: torch.Tensor, tabl
                  start: torch.Tensor, lens: torch.Tensor, top: int, block_size: int, sink: int = 1,
                  local: int = 1) -> torch.Tensor:
     """For each token of q (B, H, n, d) and kv head the `top` blocks of its
-    sequence that may hold the largest q.k (ssa_cache_select): (B, n, n_kv,
-    top) int32 block numbers, ascending, -1 behind. The first `sink` blocks and
-    the last `local` up to the token's own are always among them."""
+    sequence with the highest bound of q8.k, q8 being q in 8 bits
+    (ssa_cache_select): (B, n, n_kv, top) int32 block numbers, ascending, -1
+    behind. The first `sink` blocks and the last `local` up to the token's own
+    are always among them. The scores of a table's row are kept on chip: about
+    15 000 blocks at head dim 128."""
     return (_torch_ext or _load_torch()).cache_select(q, bounds, amax, table, start, lens, top, block_size, sink, local)
 
 
