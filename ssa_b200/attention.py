@@ -452,8 +452,10 @@ class SparseAttention(nn.Module):
                                  ("head_dim", self.d_head, cache.head_dim)):
             if want != have:
                 raise ValueError(f"the cache's {name} is {have}, {want} needed")
-        if not torch.is_autocast_enabled(x.device.type) and cache.tail.dtype != self.Wk.weight.dtype:
-            raise ValueError(f"the cache's dtype is {cache.tail.dtype}, {self.Wk.weight.dtype} needed")
+        kind = x.device.type
+        dtype = torch.get_autocast_dtype(kind) if torch.is_autocast_enabled(kind) else self.Wk.weight.dtype
+        if cache.tail.dtype != dtype:
+            raise ValueError(f"the cache's dtype is {cache.tail.dtype}, {dtype} needed")
         if prompt:
             return
         if not self.config.causal:
@@ -561,8 +563,8 @@ class SparseTransformer(nn.Module):
         """`forward` of the prompts x ((B, N) ids or (B, N, d_model)) over the
         sparse graph, filling the cache. new_lens (B,) int32: how many of a row's
         N tokens are real; 0 for the sequences of a running batch that get no
-        prompt now, which stay as they are. (The graph's bucket planes follow N,
-        so a short row's graph is that of the padded batch.) Only an empty sequence
+        prompt now, which stay as they are. Padding is neither stored nor attended
+        (the graph's bucket planes follow N, the padded length). Only an empty sequence
         takes a prompt: one that has tokens keeps them and is counted in
         `cache.refused()`, as one is that the cache has no room for. Rows behind a
         sequence's tokens, and all rows of a refused one, come from zero attention.

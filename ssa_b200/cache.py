@@ -5,8 +5,8 @@ and values, and the single-token (or few-token) step over it.
 tables, first-C members, a plane count that follows the length), so it is not
 carried forward by a token; the reference has no serving form either. A step
 takes its neighbours from the cache instead: the blocks whose bound of q.k (q
-in 8 bits) is highest stand in for the LSH candidates, beside the window's and the global
-tokens' blocks, or -- without a block budget -- the whole sequence.
+in 8 bits) is highest stand in for the LSH candidates, beside the window's and
+the global tokens' blocks, or -- without a block budget -- the whole sequence.
 
 A `BlockCache` holds the buffers of `num_layers` layers that share one block
 table. Pages are handed out on the GPU (`reserve`), so a decoding step makes no

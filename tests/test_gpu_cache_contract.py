@@ -72,6 +72,22 @@ def test_a_refused_step_leaves_the_cache(cuda):
     far.step(ids, mk(top_blocks=9))
 
 
+def test_a_cache_of_another_type_is_refused(cuda):
+    """The type is the projections': under autocast its, else the weights'."""
+    m = _model(torch.float32, cuda)
+    ids = torch.randint(0, 50, (2, 5), device=cuda)
+    for dt, auto in ((torch.bfloat16, False), (torch.float32, True)):
+        cache = BlockCache(2, 2, 64, 64, num_layers=2, block_size=16, dtype=dt)
+        with torch.autocast("cuda", torch.bfloat16, enabled=auto), pytest.raises(ValueError, match="dtype"):
+            m.step(ids, cache)
+        assert cache.lens.tolist() == [0, 0] and int(cache.state[0]) == cache.num_blocks
+    cache = BlockCache(2, 2, 64, 64, num_layers=2, block_size=16, dtype=torch.bfloat16)
+    with torch.autocast("cuda", torch.bfloat16):
+        m.prefill(ids, cache)
+        out = m.step(ids[:, :1], cache)
+    assert cache.lens.tolist() == [6, 6] and torch.isfinite(out).all()
+
+
 def test_tangents_are_refused(cuda):
     """A dual tensor's tangent is not dropped without a word, under no_grad either."""
     cache = BlockCache(1, 2, 64, 64, block_size=16)
