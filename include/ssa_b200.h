@@ -351,7 +351,9 @@ SSA_API int ssa_cache_select(const ssa_cache_params* p, const void* q, const int
  * and kv head (entries out of range are left out). out (B, H, n, d) per o_s*
  * strides; lse (B, H, n) fp32, optional. Rows without a key, and rows behind a
  * sequence's last token, are 0 with lse -inf. A seen page of V that stands for
- * NaN makes out NaN; lse is of the keys alone. Needs
+ * NaN makes out NaN; lse is of the keys alone. The amax of V of the pages a row
+ * sees may differ by factors of up to 2^120 (a page of zeros counts as one of
+ * 2^-50): beyond, the smaller one's share of the weights' sum is lost. Needs
  * ssa_cache_attn_workspace_size(p, blocks != NULL) bytes.
  */
 SSA_API size_t ssa_cache_attn_workspace_size(const ssa_cache_params* p, int32_t with_blocks);
